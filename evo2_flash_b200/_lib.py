@@ -13,7 +13,7 @@ from ._build import LIB_PATH
 
 HYENA_KIND_FIR = 0
 HYENA_KIND_IIR = 1
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 
 class StateView(C.Structure):
@@ -101,6 +101,73 @@ class DecodeArgs(C.Structure):
     ]
 
 
+class PagedKV(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_page_stride", C.c_int64),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_page_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("page_table", C.c_void_p),
+        ("page_table_stride", C.c_int64),
+        ("pages_per_request", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+    ]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("q_out", C.c_void_p),
+        ("q_out_token_stride", C.c_int64),
+        ("q_out_head_stride", C.c_int64),
+        ("k", C.c_void_p),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v", C.c_void_p),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("positions", C.c_void_p),
+        ("query_start_loc", C.c_void_p),
+        ("T", C.c_int32),
+        ("num_requests", C.c_int32),
+        ("heads", C.c_int32),
+        ("kv", PagedKV),
+        ("rope_theta", C.c_double),
+        ("error_flags", C.c_void_p),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("out", C.c_void_p),
+        ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("seq_lens", C.c_void_p),
+        ("query_start_loc", C.c_void_p),
+        ("shared_lens", C.c_void_p),
+        ("group_start", C.c_void_p),
+        ("T", C.c_int32),
+        ("num_requests", C.c_int32),
+        ("num_groups", C.c_int32),
+        ("heads", C.c_int32),
+        ("scale", C.c_float),
+        ("kv", PagedKV),
+        ("error_flags", C.c_void_p),
+    ]
+
+
 # Every symbol include/hyena_b200.h declares, with its ctypes signature.
 SIGNATURES = {
     "hyena_abi_version": (C.c_int, []),
@@ -119,6 +186,13 @@ SIGNATURES = {
     "hyena_gemm_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                   C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                   C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hyena_kv_append": (C.c_int, [C.POINTER(KvAppendArgs), C.c_void_p]),
+    "hyena_paged_attention_workspace_size": (C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
+    "hyena_paged_attention": (C.c_int, [C.POINTER(PagedAttentionArgs), C.c_void_p, C.c_size_t,
+                                        C.c_void_p]),
+    "hyena_gemm_gated_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                        C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
+                                        C.c_int32, C.c_int32, C.c_void_p]),
     "hyena_rms_norm": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                  C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                  C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int32,

@@ -61,6 +61,14 @@ int spec_record_prefill_launch(const int32_t* blocks, int64_t block_stride, int 
                                const int32_t* seq_lens, float* stamps, int64_t stamp_stride,
                                int num_blocks, int32_t* error_flags, cudaStream_t st);
 
+int kv_append_launch(const hyena_kv_append_args& A, cudaStream_t st);
+size_t paged_attention_workspace_size(const hyena_paged_attention_args& A);
+int paged_attention_launch(const hyena_paged_attention_args& A, void* ws, size_t ws_bytes,
+                           cudaStream_t st);
+int gemm_gated_bf16_launch(const void* A, int64_t lda, const void* B1, int64_t ldb1, const void* B2,
+                           int64_t ldb2, void* out, int64_t ldo, int M, int N, int K, int act,
+                           cudaStream_t st);
+
 static int check_params(const hyena_layer_params* p) {
   HB_REQUIRE(p != nullptr, "null layer params");
   HB_REQUIRE(p->H > 0 && p->H % 64 == 0, "H must be a positive multiple of 64");
@@ -223,6 +231,30 @@ int hyena_gemm_fp8_emulated(const void* A, int64_t lda, const void* B, int64_t l
                             const float* scale_b, void* stream) {
   return hb::gemm_fp8_emulated_launch(A, lda, B, ldb, out, ldo, N, M, K, scale_a, scale_b,
                                       static_cast<cudaStream_t>(stream));
+}
+
+int hyena_kv_append(const hyena_kv_append_args* a, void* stream) {
+  HB_REQUIRE(a != nullptr, "null kv_append args");
+  return hb::kv_append_launch(*a, static_cast<cudaStream_t>(stream));
+}
+
+size_t hyena_paged_attention_workspace_size(const hyena_paged_attention_args* a) {
+  return a == nullptr ? 0 : hb::paged_attention_workspace_size(*a);
+}
+
+int hyena_paged_attention(const hyena_paged_attention_args* a, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  HB_REQUIRE(a != nullptr, "null paged_attention args");
+  return hb::paged_attention_launch(*a, workspace, workspace_bytes,
+                                    static_cast<cudaStream_t>(stream));
+}
+
+int hyena_gemm_gated_bf16(const void* A, int64_t lda, const void* B1, int64_t ldb1, const void* B2,
+                          int64_t ldb2, void* out, int64_t ldo, int32_t M, int32_t N, int32_t K,
+                          int32_t act, void* stream) {
+  HB_REQUIRE(M <= 0 || N <= 0 || (A && B1 && B2 && out), "null gated gemm pointer");
+  return gemm_gated_bf16_launch(A, lda, B1, ldb1, B2, ldb2, out, ldo, M, N, K, act,
+                                static_cast<cudaStream_t>(stream));
 }
 
 int hyena_gemm_wait_timeouts(int32_t* count, int32_t reset) {

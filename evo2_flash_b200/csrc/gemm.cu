@@ -2,6 +2,10 @@
 //
 //   in_proj : out(M,N) bf16 = (A e4m3 . B e4m3^T) * sa * sb     (kind::f8f6f4)
 //   out_proj: out(M,N) bf16 =  A bf16 . B bf16^T + bias          (kind::f16)
+//   gated   : out(M,N) bf16 = act(A . B1^T) * (A . B2^T), bf16 (kind::f16): the
+//             two projections of the gated MLP as one GEMM whose B tile is half
+//             rows of B1, half the same rows of B2, so that both products of an
+//             output sit in one TMEM lane and the epilogue joins them in fp32
 // Both operands K-major (activations (M,K) row-major, nn.Linear weights (N,K)).
 //
 // Persistent kernel, one CTA per SM, walking 128 x BN output tiles (N fastest)
@@ -134,6 +138,11 @@ __device__ __forceinline__ uint64_t policy_evict_last() {
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
   return p;
 }
+__device__ __forceinline__ uint64_t policy_evict_normal() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
 // 16-byte store marked streaming (evict-first in L2): GEMM outputs are read
 // once, later, by another kernel, and must not push the weights out of L2.
 __device__ __forceinline__ void st_stream16(void* p, const uint4& v) {
@@ -216,12 +225,39 @@ __host__ __device__ constexpr uint32_t idesc() {
          (uint32_t(BN >> 3) << 17) | (uint32_t(BM >> 4) << 24);
 }
 
-template <bool FP8, int BN>
-__global__ void __launch_bounds__(THREADS, 1)
-gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-            bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
-            const float* __restrict__ sa, const float* __restrict__ sb,
-            const bf16* __restrict__ bias) {
+// act(z1) * z2 in fp32 (model.py:77-101: gelu is torch's erf form, x Phi(x)).
+__device__ __forceinline__ float gate(float z1, float z2, int act) {
+  if (act == HYENA_ACT_GELU) z1 *= normcdff(z1);
+  if (act == HYENA_ACT_SILU) z1 /= 1.0f + expf(-z1);
+  return z1 * z2;
+}
+
+// Tile order.  Plain GEMMs go N fastest: their weight (<= 50 MB at the 7B shape)
+// stays in L2 while the activations stream through once.  The gated pair of
+// weights (180 MB) does not fit, so its tiles go in groups of GATED_GROUP row
+// tiles, rows fastest: the group's activations stay in L2 and the weights are
+// read once a group instead of once a row tile.  N fastest against grouped: see
+// gemm_gated_bf16_launch.
+constexpr int GATED_GROUP = 8;
+template <bool GATED>
+__device__ __forceinline__ void tile_mn(int tile, int m_tiles, int n_tiles, int& m, int& n) {
+  if constexpr (GATED) {
+    const int g = tile / (GATED_GROUP * n_tiles), rem = tile - g * (GATED_GROUP * n_tiles);
+    const int left = m_tiles - g * GATED_GROUP, gm = left < GATED_GROUP ? left : GATED_GROUP;
+    n = rem / gm;
+    m = g * GATED_GROUP + rem - n * gm;
+  } else {
+    m = tile / n_tiles;
+    n = tile - m * n_tiles;
+  }
+}
+
+template <bool FP8, int BN, bool GATED>
+__device__ __forceinline__ void
+gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
+          bf16* __restrict__ out, int64_t ldo, int M, int N, int K, const float* __restrict__ sa,
+          const float* __restrict__ sb, const bf16* __restrict__ bias, int act) {
+  constexpr int HN = GATED ? BN / 2 : BN;  // output columns of a tile
   constexpr int STAGES = Cfg<BN>::STAGES;
   constexpr int STAGE_BYTES = Cfg<BN>::STAGE_BYTES;
   constexpr uint32_t TMEM_COLS = Cfg<BN>::TMEM_COLS;
@@ -232,11 +268,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   constexpr int ELEM = FP8 ? 1 : 2;
   constexpr int KE = BKB / ELEM;  // K elements per stage
   const int kblocks = K / KE;
-  // Tiles in N-fastest order: CTAs resident together share A row panels, and the
-  // whole weight (<= 50 MB at the 7B shape) stays in L2 while the activations
-  // stream through once.
-  const int n_tiles = (N + BN - 1) / BN;
-  const int total = n_tiles * ((M + BM - 1) / BM);
+  const int n_tiles = (N + HN - 1) / HN, m_tiles = (M + BM - 1) / BM;
+  const int total = n_tiles * m_tiles;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -265,8 +298,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   // While the previous kernel drains: this CTA's first weight tiles into L2
   // (a prefetch cannot observe stale data: L2 is the point of coherence).
   if (warp == 0 && lane == 0 && (int)blockIdx.x < total) {
-    const int n0 = ((int)blockIdx.x % n_tiles) * BN;
-    for (int kb = 0; kb < kblocks && kb < STAGES; ++kb) tma_prefetch_l2(&tmB, kb * KE, n0);
+    int mt, nt;
+    tile_mn<GATED>((int)blockIdx.x, m_tiles, n_tiles, mt, nt);
+    for (int kb = 0; kb < kblocks && kb < STAGES; ++kb) {
+      tma_prefetch_l2(&tmB, kb * KE, nt * HN);
+      if constexpr (GATED) tma_prefetch_l2(&tmB2, kb * KE, nt * HN);
+    }
   }
   pdl_wait();
   pdl_trigger();  // after the wait: see common.cuh
@@ -277,18 +314,23 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       // activations once per N tile -> keep B, stream A.  Few M tiles (decode):
       // A is reused by every N tile, the weight streamed once per call.
       const bool many_m = (M + BM - 1) / BM > 8;
-      const uint64_t pol_a = many_m ? policy_evict_first() : policy_evict_last();
-      const uint64_t pol_b = many_m ? policy_evict_last() : policy_evict_first();
+      const uint64_t pol_a = many_m && !GATED ? policy_evict_first() : policy_evict_last();
+      const uint64_t pol_b = !many_m ? policy_evict_first() : GATED ? policy_evict_normal()
+                                                                    : policy_evict_last();
       uint32_t it = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-        const int m0 = (tile / n_tiles) * BM, n0 = (tile % n_tiles) * BN;
+        int mt, nt;
+        tile_mn<GATED>(tile, m_tiles, n_tiles, mt, nt);
+        const int m0 = mt * BM, n0 = nt * HN;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
           mbar_expect_tx(&S.full[s], STAGE_BYTES);
           tma_load_2d(&tmA, &S.full[s], S.a[s], kb * KE, m0, pol_a);
           tma_load_2d(&tmB, &S.full[s], S.b[s], kb * KE, n0, pol_b);
+          if constexpr (GATED)
+            tma_load_2d(&tmB2, &S.full[s], S.b[s] + HN * BKB, kb * KE, n0, pol_b);
         }
       }
       // Drain: every issued copy has landed before the CTA can exit.
@@ -329,17 +371,29 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     }
     uint32_t ti = 0;
     for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++ti) {
-      const int m0 = (tile / n_tiles) * BM, n0 = (tile % n_tiles) * BN;
+      int mt, nt;
+      tile_mn<GATED>(tile, m_tiles, n_tiles, mt, nt);
+      const int m0 = mt * BM, n0 = nt * HN;
       const int b = ti & 1;
       const bool ok = mbar_wait(&S.acc_full[b], (ti >> 1) & 1);
       if (!ok) break;  // the MMA warp gave up: stop rather than time out per tile
       fence_after();
       const int row = m0 + 32 * q + lane;
 #pragma unroll 1
-      for (int cb = 0; cb < BN / 32; ++cb) {
+      for (int cb = 0; cb < HN / 32; ++cb) {
         uint32_t r[32];
-        tmem_ld32(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + cb * 32), r);
-        if (cb == BN / 32 - 1) {  // accumulator fully read: hand it back to the MMA warp
+        if constexpr (GATED) {
+          uint32_t r2[32];
+          tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + cb * 32), r);
+          tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + HN + cb * 32), r2);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            r[j] = __float_as_uint(gate(__uint_as_float(r[j]), __uint_as_float(r2[j]), act));
+        } else {
+          tmem_ld32(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + cb * 32), r);
+        }
+        if (cb == HN / 32 - 1) {  // accumulator fully read: hand it back to the MMA warp
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&S.acc_empty[b]);
@@ -382,6 +436,22 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                  "r"(TMEM_COLS)
                  : "memory");
   }
+}
+
+template <bool FP8, int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+            bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
+            const float* __restrict__ sa, const float* __restrict__ sb,
+            const bf16* __restrict__ bias) {
+  gemm_body<FP8, BN, false>(tmA, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0);
+}
+template <int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB1,
+                  const __grid_constant__ CUtensorMap tmB2, bf16* __restrict__ out, int64_t ldo,
+                  int M, int N, int K, int act) {
+  gemm_body<false, BN, true>(tmA, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr, act);
 }
 
 // ---------------------------------------------------------------- small M
@@ -473,12 +543,13 @@ __host__ __device__ constexpr uint32_t pow2_cols() {
 // bias and store bf16 rows coalesced.  A second split barrier (arrive once the
 // inbox is full, wait before exit) keeps every staging area alive until all
 // copies have landed.
-template <bool FP8, int BN>
-__global__ void __launch_bounds__(THREADS, 1)
-gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
-                    const __grid_constant__ CUtensorMap tmB, bf16* __restrict__ out, int64_t ldo,
-                    int M, int N, int K, const float* __restrict__ sa,
-                    const float* __restrict__ sb, const bf16* __restrict__ bias) {
+template <bool FP8, int BN, bool GATED>
+__device__ __forceinline__ void
+gemm_cluster_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
+                  bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
+                  const float* __restrict__ sa, const float* __restrict__ sb,
+                  const bf16* __restrict__ bias, int act) {
+  constexpr int HN = GATED ? BN / 2 : BN;  // output columns of a tile
   constexpr int STAGES = Cfg<BN>::STAGES;
   constexpr int STAGE_BYTES = Cfg<BN>::STAGE_BYTES;
   constexpr uint32_t TMEM_COLS = pow2_cols<BN>();
@@ -494,9 +565,9 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
   const int splits = (int)gridDim.x;
   const int rank = (int)cluster_rank();
   const int rows_per = (BM + splits - 1) / splits;
-  const int n_tiles = (N + BN - 1) / BN;
+  const int n_tiles = (N + HN - 1) / HN;
   const int tile = (int)blockIdx.y;
-  const int m0 = (tile / n_tiles) * BM, n0 = (tile % n_tiles) * BN;
+  const int m0 = (tile / n_tiles) * BM, n0 = (tile % n_tiles) * HN;
   const int kb0 = rank * kblocks / splits, kb1 = (rank + 1) * kblocks / splits;
   const int rows = M - m0 < BM ? M - m0 : BM;  // valid rows of the tile
   // Rows [o R, o R + owned(o)) belong to rank o.
@@ -534,7 +605,10 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
   const uint32_t tmem = S.tmem_base;
   // While the previous kernel drains: this CTA's first weight tiles into L2.
   if (warp == 0 && lane == 0) {
-    for (int kb = kb0; kb < kb1 && kb < kb0 + STAGES; ++kb) tma_prefetch_l2(&tmB, kb * KE, n0);
+    for (int kb = kb0; kb < kb1 && kb < kb0 + STAGES; ++kb) {
+      tma_prefetch_l2(&tmB, kb * KE, n0);
+      if constexpr (GATED) tma_prefetch_l2(&tmB2, kb * KE, n0);
+    }
   }
   pdl_wait();
   pdl_trigger();  // after the wait: see common.cuh
@@ -551,6 +625,8 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
         mbar_expect_tx(&S.full[s], STAGE_BYTES);
         tma_load_2d(&tmA, &S.full[s], S.u.ring.a[s], kb * KE, m0, pol_a);
         tma_load_2d(&tmB, &S.full[s], S.u.ring.b[s], kb * KE, n0, pol_b);
+        if constexpr (GATED)
+          tma_load_2d(&tmB2, &S.full[s], S.u.ring.b[s] + HN * BKB, kb * KE, n0, pol_b);
       }
       // Drain: every issued copy has landed before the ring is reused.
       for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i)
@@ -583,7 +659,7 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
   }
   if (warp >= 2) {
     // While the main loop runs: epilogue constants into registers / shared memory.
-    if constexpr (!FP8) {
+    if constexpr (!FP8 && !GATED) {
       for (int j = threadIdx.x - 64; j < BN; j += 128)
         S.bias_s[j] = (bias != nullptr && n0 + j < N) ? __bfloat162float(bias[n0 + j]) : 0.0f;
     }
@@ -610,7 +686,8 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
         uint32_t r[2][32];
         if (have) {
           tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(cb * 32), r[0]);
-          tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(cb * 32 + 32), r[1]);
+          if ((cb + 1) * 32 < BN)
+            tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(cb * 32 + 32), r[1]);
           tmem_wait_ld();
         } else {
 #pragma unroll
@@ -618,12 +695,14 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
         }
         if (row < rows) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            if ((cb + h) * 32 >= BN) continue;
 #pragma unroll
             for (int v = 0; v < 8; ++v)
               dst[(cb + h) * 8 + v] =
                   make_float4(__uint_as_float(r[h][4 * v]), __uint_as_float(r[h][4 * v + 1]),
                               __uint_as_float(r[h][4 * v + 2]), __uint_as_float(r[h][4 * v + 3]));
+          }
         }
       }
     }
@@ -657,16 +736,19 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
   // bias added, 4 bf16 stored (consecutive threads: consecutive 16-byte float4
   // reads, conflict-free, and consecutive 8-byte pieces of a row).
   if (__syncthreads_and(ready ? 1 : 0)) {
-    constexpr int CPR = BN / 4;  // 4-column pieces per row
-    constexpr int U = 8;
+    constexpr int CPR = HN / 4;  // 4-column pieces per row
+    constexpr int U = GATED ? 4 : 8;
     constexpr int MAXS = max_cluster_splits<BN>();
     const int n_items = my_rows * CPR;
     const int base = rank * rows_per;
 #pragma unroll 1
     for (int i0 = (int)threadIdx.x; i0 < n_items; i0 += U * THREADS) {
-      float4 acc[U];
+      float4 acc[U], acc2[GATED ? U : 1];
 #pragma unroll
-      for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int u = 0; u < U; ++u) {
+        acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (GATED) acc2[u] = acc[u];
+      }
 #pragma unroll
       for (int p = 0; p < MAXS; ++p) {  // unrolled: every partial's loads in flight together
         if (p >= splits) break;
@@ -682,6 +764,14 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
             acc[u].y += x.y;
             acc[u].z += x.z;
             acc[u].w += x.w;
+            if constexpr (GATED) {
+              const float4 y =
+                  *reinterpret_cast<const float4*>(pb + (it / CPR) * LD + HN + (it % CPR) * 4);
+              acc2[u].x += y.x;
+              acc2[u].y += y.y;
+              acc2[u].z += y.z;
+              acc2[u].w += y.w;
+            }
           }
         }
       }
@@ -695,6 +785,9 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
         for (int e = 0; e < 4; ++e) {
           if constexpr (FP8) {
             v[e] = (v[e] * scale) * scale_b;  // (acc * sx) * sw, fp8_emul.py:87
+          } else if constexpr (GATED) {
+            v[e] = gate(v[e], e == 0 ? acc2[u].x : e == 1 ? acc2[u].y : e == 2 ? acc2[u].z : acc2[u].w,
+                        act);
           } else {
             v[e] += S.bias_s[c + e];
           }
@@ -719,6 +812,24 @@ gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
                  "r"(TMEM_COLS)
                  : "memory");
   }
+}
+
+template <bool FP8, int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
+                    const __grid_constant__ CUtensorMap tmB, bf16* __restrict__ out, int64_t ldo,
+                    int M, int N, int K, const float* __restrict__ sa,
+                    const float* __restrict__ sb, const bf16* __restrict__ bias) {
+  gemm_cluster_body<FP8, BN, false>(tmA, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0);
+}
+template <int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_gated_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
+                          const __grid_constant__ CUtensorMap tmB1,
+                          const __grid_constant__ CUtensorMap tmB2, bf16* __restrict__ out,
+                          int64_t ldo, int M, int N, int K, int act) {
+  gemm_cluster_body<false, BN, true>(tmA, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr,
+                                     act);
 }
 
 // ---------------------------------------------------------------- 2-SM tiles
@@ -801,12 +912,14 @@ __host__ __device__ constexpr uint32_t idesc_pair() {
          (uint32_t(BN2 >> 3) << 17) | (uint32_t((2 * BM) >> 4) << 24);
 }
 
-template <bool FP8>
-__global__ void __launch_bounds__(THREADS, 1)
-gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
-                 const float* __restrict__ sa, const float* __restrict__ sb,
-                 const bf16* __restrict__ bias) {
+template <bool FP8, bool GATED>
+__device__ __forceinline__ void
+gemm_pair_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
+               bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
+               const float* __restrict__ sa, const float* __restrict__ sb,
+               const bf16* __restrict__ bias, int act) {
+  // Gated: the even CTA's B rows are B1's, the odd CTA's the same rows of B2.
+  constexpr int HN = GATED ? BN2 / 2 : BN2;  // output columns of a tile
   pdl_trigger();
   constexpr int STAGES = Cfg2::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -818,8 +931,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const int kblocks = K / KE;
   const uint32_t rank = cluster_rank();  // 0: the MMA-issuing CTA
   const int pair = (int)blockIdx.x / 2, npairs = (int)gridDim.x / 2;
-  const int n_tiles = (N + BN2 - 1) / BN2;
-  const int total = n_tiles * ((M + 2 * BM - 1) / (2 * BM));
+  const int n_tiles = (N + HN - 1) / HN, m_tiles = (M + 2 * BM - 1) / (2 * BM);
+  const int total = n_tiles * m_tiles;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -853,21 +966,25 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   if (warp == 0) {
     if (lane == 0) {
       const bool many_m = (M + BM - 1) / BM > 8;
-      const uint64_t pol_a = many_m ? policy_evict_first() : policy_evict_last();
-      const uint64_t pol_b = many_m ? policy_evict_last() : policy_evict_first();
+      const uint64_t pol_a = many_m && !GATED ? policy_evict_first() : policy_evict_last();
+      const uint64_t pol_b = !many_m ? policy_evict_first() : GATED ? policy_evict_normal()
+                                                                    : policy_evict_last();
+      const CUtensorMap* map_b = GATED && rank != 0 ? &tmB2 : &tmB;
       const uint32_t full0 = map_to_rank(su32(&S.full[0]), 0);
       uint32_t it = 0;
       bool ok = true;
       for (int tile = pair; tile < total && ok; tile += npairs) {
-        const int m0 = (tile / n_tiles) * 2 * BM + (int)rank * BM;
-        const int n0 = (tile % n_tiles) * BN2 + (int)rank * (BN2 / 2);
+        int mt, nt;
+        tile_mn<GATED>(tile, m_tiles, n_tiles, mt, nt);
+        const int m0 = mt * 2 * BM + (int)rank * BM;
+        const int n0 = nt * HN + (GATED ? 0 : (int)rank * (BN2 / 2));
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
           if (rank == 0) mbar_expect_tx(&S.full[s], 2 * Cfg2::STAGE_BYTES);
           const uint32_t bar = full0 + uint32_t(s * sizeof(uint64_t));
           tma_load_2d_pair(&tmA, bar, S.a[s], kb * KE, m0, pol_a);
-          tma_load_2d_pair(&tmB, bar, S.b[s], kb * KE, n0, pol_b);
+          tma_load_2d_pair(map_b, bar, S.b[s], kb * KE, n0, pol_b);
         }
       }
       // Drain: every issued copy has landed before the CTA can exit.  The
@@ -915,17 +1032,29 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const uint32_t acc_empty0 = map_to_rank(su32(&S.acc_empty[0]), 0);
     uint32_t ti = 0;
     for (int tile = pair; tile < total; tile += npairs, ++ti) {
-      const int m0 = (tile / n_tiles) * 2 * BM + (int)rank * BM, n0 = (tile % n_tiles) * BN2;
+      int mt, nt;
+      tile_mn<GATED>(tile, m_tiles, n_tiles, mt, nt);
+      const int m0 = mt * 2 * BM + (int)rank * BM, n0 = nt * HN;
       const int b = ti & 1;
       const bool ok = mbar_wait(&S.acc_full[b], (ti >> 1) & 1);
       if (!ok) break;  // the MMA warp gave up: stop rather than time out per tile
       fence_after();
       const int row = m0 + 32 * q + lane;
 #pragma unroll 1
-      for (int cb = 0; cb < BN2 / 32; ++cb) {
+      for (int cb = 0; cb < HN / 32; ++cb) {
         uint32_t r[32];
-        tmem_ld32(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN2 + cb * 32), r);
-        if (cb == BN2 / 32 - 1) {  // accumulator fully read: hand it back to the MMA warp
+        if constexpr (GATED) {
+          uint32_t r2[32];
+          tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN2 + cb * 32), r);
+          tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN2 + HN + cb * 32), r2);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            r[j] = __float_as_uint(gate(__uint_as_float(r[j]), __uint_as_float(r2[j]), act));
+        } else {
+          tmem_ld32(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN2 + cb * 32), r);
+        }
+        if (cb == HN / 32 - 1) {  // accumulator fully read: hand it back to the MMA warp
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acc_empty0 + uint32_t(b * sizeof(uint64_t)));
@@ -971,6 +1100,22 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                  "r"(Cfg2::TMEM_COLS)
                  : "memory");
   }
+}
+
+template <bool FP8>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
+                 const float* __restrict__ sa, const float* __restrict__ sb,
+                 const bf16* __restrict__ bias) {
+  gemm_pair_body<FP8, false>(tmA, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0);
+}
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_gated_pair_kernel(const __grid_constant__ CUtensorMap tmA,
+                       const __grid_constant__ CUtensorMap tmB1,
+                       const __grid_constant__ CUtensorMap tmB2, bf16* __restrict__ out, int64_t ldo,
+                       int M, int N, int K, int act) {
+  gemm_pair_body<false, true>(tmA, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr, act);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1252,7 +1397,152 @@ static int launch(const void* A, int64_t lda, const void* B, int64_t ldb, void* 
   }
 }
 
+// ---------------------------------------------------------------- gated launch
+template <int BN>
+static int launch_gated_bn(const CUtensorMap& ta, const CUtensorMap& t1, const CUtensorMap& t2,
+                           bf16* out, int64_t ldo, int M, int N, int K, int act, cudaStream_t st) {
+  const size_t smem = sizeof(Smem<BN>) + 1024;
+  if (!smem_attr<gemm_gated_kernel<BN>>((int)smem))
+    return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_gated) failed");
+  const long long tiles = (long long)((N + BN / 2 - 1) / (BN / 2)) * ((M + BM - 1) / BM);
+  long long cap = num_sms();
+  const int lim = g_max_ctas.load(std::memory_order_relaxed);
+  if (lim > 0 && lim < cap) cap = lim;
+  launch_kernel(gemm_gated_kernel<BN>, dim3((unsigned)(tiles < cap ? tiles : cap)), dim3(THREADS),
+                smem, st, 0u, ta, t1, t2, out, ldo, M, N, K, act);
+  return check_launch("gemm_gated_kernel");
+}
+
+template <int BN>
+static int launch_gated_cluster(const CUtensorMap& ta, const CUtensorMap& t1, const CUtensorMap& t2,
+                                bf16* out, int64_t ldo, int M, int N, int K, int act, int splits,
+                                cudaStream_t st) {
+  const size_t smem = sizeof(SmemSK<BN>) + 1024;
+  if (!smem_attr<gemm_gated_cluster_kernel<BN>>((int)smem))
+    return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_gated_cluster) failed");
+  const int tiles = ((N + BN / 2 - 1) / (BN / 2)) * ((M + BM - 1) / BM);
+  launch_kernel(gemm_gated_cluster_kernel<BN>, dim3((unsigned)splits, (unsigned)tiles, 1),
+                dim3(THREADS), smem, st, (unsigned)splits, ta, t1, t2, out, ldo, M, N, K, act);
+  return check_launch("gemm_gated_cluster_kernel");
+}
+
+// Launched like gemm_pair_kernel: without programmatic serialisation.
+static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& t1, const CUtensorMap& t2,
+                             bf16* out, int64_t ldo, int M, int N, int K, int act,
+                             cudaStream_t st) {
+  const size_t smem = sizeof(Smem2) + 1024;
+  if (!smem_attr<gemm_gated_pair_kernel>((int)smem))
+    return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_gated_pair) failed");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2, 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  static std::atomic<int> resident_pairs{0};
+  int rp = resident_pairs.load(std::memory_order_relaxed);
+  if (rp == 0) {
+    if (cudaOccupancyMaxActiveClusters(&rp, gemm_gated_pair_kernel, &cfg) != cudaSuccess || rp <= 0) {
+      cudaGetLastError();
+      rp = num_sms() / 2;
+    }
+    resident_pairs.store(rp, std::memory_order_relaxed);
+  }
+  const long long tiles = (long long)((N + BN2 / 2 - 1) / (BN2 / 2)) * ((M + 2 * BM - 1) / (2 * BM));
+  long long cap = rp;
+  const int lim = g_max_ctas.load(std::memory_order_relaxed);
+  if (lim > 0 && lim / 2 < cap) cap = lim / 2 > 0 ? lim / 2 : 1;
+  cfg.gridDim = dim3((unsigned)(2 * (tiles < cap ? tiles : cap)));
+  cudaLaunchKernelEx(&cfg, gemm_gated_pair_kernel, ta, t1, t2, out, ldo, M, N, K, act);
+  return check_launch("gemm_gated_pair_kernel");
+}
+
+// Cost of a choice: operand bytes (rows of 128 B) through the busiest SM, i.e.
+// waves x (BM + BN) x K blocks of its slice.  One row tile (decode batches): the
+// cheapest of the cluster kernel's one-wave (BN, splits) and the persistent
+// kernel's BN (7B shape, 11008 outputs: BN 160 makes 138 tiles on 148 SMs).
+static Plan plan_gated(int M, int N, int K) {
+  const long long mt = (M + BM - 1) / BM;
+  const int sms = num_sms(), kblocks = K / (BKB / 2);
+  if (M >= PAIR_MIN_M && N >= BN2 / 2) return {BN2, 0, true};
+  Plan best = {0, 0};
+  long long best_cost = 0;
+  for (int bn : {256, 192, 128, 64}) {
+    const long long tiles = mt * ((N + bn / 2 - 1) / (bn / 2));
+    const long long cost = ((tiles + sms - 1) / sms) * (BM + bn) * kblocks;
+    if (best.bn == 0 || cost < best_cost) {
+      best = {bn, 0};
+      best_cost = cost;
+    }
+  }
+  if (mt == 1) {
+    for (int bn : {256, 192, 160, 128, 64}) {
+      const long long tiles = (N + bn / 2 - 1) / (bn / 2);
+      for (int sp = 1; sp <= (bn >= 256 ? 3 : 4); ++sp) {
+        if (tiles * sp > sms || (sp > 1 && kblocks / sp < 2)) break;
+        const long long cost = (long long)(BM + bn) * ((kblocks + sp - 1) / sp);
+        if (cost < best_cost) {
+          best = {bn, sp};
+          best_cost = cost;
+        }
+      }
+    }
+  }
+  return best;
+}
+
+static int launch_gated(const void* A, int64_t lda, const void* B1, int64_t ldb1, const void* B2,
+                        int64_t ldb2, void* outv, int64_t ldo, int M, int N, int K, int act,
+                        cudaStream_t st) {
+  HB_REQUIRE(act == HYENA_ACT_NONE || act == HYENA_ACT_GELU || act == HYENA_ACT_SILU,
+             "gated GEMM: unknown activation");
+  if (M <= 0 || N <= 0) return HYENA_OK;
+  HB_REQUIRE(K > 0 && K % 64 == 0, "gated GEMM needs K % 64 == 0");
+  HB_REQUIRE(N % 8 == 0 && ldo % 8 == 0, "gated GEMM needs N % 8 == 0 and ldo % 8 == 0");
+  HB_REQUIRE(aligned16(A) && aligned16(B1) && aligned16(B2) && aligned16(outv),
+             "gated GEMM operands must be 16-byte aligned");
+  HB_REQUIRE(lda % 8 == 0 && ldb1 % 8 == 0 && ldb2 % 8 == 0,
+             "gated GEMM row strides must be multiples of 16 bytes");
+  HB_REQUIRE(lda >= K && ldb1 >= K && ldb2 >= K && ldo >= N,
+             "gated GEMM leading dimensions too small");
+  bf16* out = static_cast<bf16*>(outv);
+  const Plan pl = plan_gated(M, N, K);
+  CUtensorMap ta, t1, t2;
+  int rc = make_map(&ta, A, false, (uint64_t)K, (uint64_t)M, (uint64_t)lda, BM);
+  if (!rc) rc = make_map(&t1, B1, false, (uint64_t)K, (uint64_t)N, (uint64_t)ldb1, (uint32_t)pl.bn / 2);
+  if (!rc) rc = make_map(&t2, B2, false, (uint64_t)K, (uint64_t)N, (uint64_t)ldb2, (uint32_t)pl.bn / 2);
+  if (rc) return rc;
+  if (pl.pair) return launch_gated_pair(ta, t1, t2, out, ldo, M, N, K, act, st);
+  if (pl.splits > 0) {
+    switch (pl.bn) {
+      case 256: return launch_gated_cluster<256>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      case 192: return launch_gated_cluster<192>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      case 160: return launch_gated_cluster<160>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      case 128: return launch_gated_cluster<128>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      default: return launch_gated_cluster<64>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+    }
+  }
+  switch (pl.bn) {
+    case 256: return launch_gated_bn<256>(ta, t1, t2, out, ldo, M, N, K, act, st);
+    case 192: return launch_gated_bn<192>(ta, t1, t2, out, ldo, M, N, K, act, st);
+    case 128: return launch_gated_bn<128>(ta, t1, t2, out, ldo, M, N, K, act, st);
+    default: return launch_gated_bn<64>(ta, t1, t2, out, ldo, M, N, K, act, st);
+  }
+}
+
 }  // namespace gemm
+
+int gemm_gated_bf16_launch(const void* A, int64_t lda, const void* B1, int64_t ldb1, const void* B2,
+                           int64_t ldb2, void* out, int64_t ldo, int M, int N, int K, int act,
+                           cudaStream_t st) {
+  return gemm::launch_gated(A, lda, B1, ldb1, B2, ldb2, out, ldo, M, N, K, act, st);
+}
 
 // `ws` / `ws_bytes` are accepted for ABI stability and not used: small-M
 // calls reduce their K slices inside a cluster.

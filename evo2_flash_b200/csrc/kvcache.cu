@@ -1,0 +1,198 @@
+// Appending a step's keys and values to the paged attention cache, with the
+// rotary embedding of queries and keys on the way (hyena_kv_append): the
+// rotation of Evo2Attention (model.py:104-152, neox halves) and the cache write
+// that follows it, one pass over q, k and v.
+//
+//   a = x[i], b = x[i + D/2], i < D/2, at position p:
+//   x'[i] = a cos(p f_i) - b sin(p f_i),  x'[i + D/2] = b cos(p f_i) + a sin(p f_i),
+//   f_i = theta^(-2i/D)
+//
+// in fp32, rounded once to bf16 (the caches hold bf16, as every activation of
+// the model).  The angle is formed in turns in fp64, t = p f_i / 2 pi, and
+// reduced to t - rint(t) before it is narrowed: an fp32 p f_i is off by up to
+// 2^-24 p radians, 0.06 at a position of one million.
+//
+// HBM-bound: 12 bytes an element pair of heads read and written once.  A block
+// owns TB tokens; their cos / sin go to shared memory once and serve every
+// head; a thread then moves U independent items of 8 + 8 elements (16-byte
+// accesses), U loads in flight.
+#include <cmath>
+
+#include "attention.cuh"
+
+namespace hb {
+
+constexpr int KV_THREADS = 256;
+constexpr int KV_MAX_HALF = 64;  // head_dim / 2
+
+struct KvAppendParams {
+  hyena_kv_append_args a;
+  double turns[KV_MAX_HALF];  // f_i / (2 pi)
+};
+
+// Page of `pos` of request r, or -1 (flagged) where the table does not have it.
+__device__ __forceinline__ int page_of(const hyena_paged_kv& kv, int r, int page_index,
+                                       int32_t* flags) {
+  int page = -1;
+  if (page_index < kv.pages_per_request)
+    page = __ldg(kv.page_table + (long long)r * kv.page_table_stride + page_index);
+  if (page < 0 || page >= kv.num_pages) {
+    flag_error(flags, HYENA_FLAG_BLOCK_RANGE);
+    return -1;
+  }
+  return page;
+}
+
+template <int TB>
+__global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_constant__ KvAppendParams P) {
+  __shared__ float2 cs[TB][KV_MAX_HALF];
+  __shared__ long long koff[TB], voff[TB];  // element offset of the token's row; -1: not written
+  __shared__ int live[TB];
+  pdl_entry();
+  const hyena_kv_append_args& A = P.a;
+  const int tid = (int)threadIdx.x;
+  const int half = A.kv.head_dim / 2;
+  const long long t0 = (long long)blockIdx.x * TB;
+  if (tid < TB) {
+    const long long t = t0 + tid;
+    int ok = 0;
+    long long ko = -1, vo = -1;
+    if (t < A.T) {
+      int r = (int)t;
+      bool owned = r < A.num_requests;
+      if (A.query_start_loc != nullptr) {
+        r = find_segment(A.query_start_loc, A.num_requests, (int)t);
+        owned = __ldg(A.query_start_loc + r) <= t && t < __ldg(A.query_start_loc + r + 1);
+      }
+      const int pos = owned ? __ldg(A.positions + t) : -1;
+      if (pos >= 0) {
+        ok = 1;
+        const int pi = pos / A.kv.page_size, at = pos - pi * A.kv.page_size;
+        const int page = page_of(A.kv, r, pi, A.error_flags);
+        if (page >= 0) {
+          ko = page * A.kv.k_page_stride + at * A.kv.k_token_stride;
+          vo = page * A.kv.v_page_stride + at * A.kv.v_token_stride;
+        }
+      }
+    }
+    live[tid] = ok;
+    koff[tid] = ko;
+    voff[tid] = vo;
+  }
+  for (int i = tid; i < TB * half; i += KV_THREADS) {
+    const int tok = i / half, p = i - tok * half;
+    if (t0 + tok < A.T) {
+      const double turn = (double)__ldg(A.positions + t0 + tok) * P.turns[p];
+      float s, c;
+      sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
+      cs[tok][p] = make_float2(c, s);
+    }
+  }
+  __syncthreads();
+
+  const int octs = half / 8;
+  const int hq = A.q != nullptr ? A.heads : 0, hkv = A.kv.kv_heads;
+  const int items = (hq + 2 * hkv) * octs;
+  constexpr int U = 3;
+  for (int tok = 0; tok < TB; ++tok) {
+    if (!live[tok]) continue;
+    const long long t = t0 + tok;
+    for (int i0 = tid; i0 < items; i0 += U * KV_THREADS) {
+      uint4 a[U], b[U];
+      bf16* dst[U];
+      int oct[U];
+      bool turned[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * KV_THREADS;
+        dst[u] = nullptr;
+        if (i >= items) continue;
+        int h = i / octs;
+        oct[u] = i - h * octs;
+        const bf16* src;
+        turned[u] = h < hq + hkv;
+        if (h < hq) {
+          src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
+          dst[u] = static_cast<bf16*>(A.q_out) + t * A.q_out_token_stride + h * A.q_out_head_stride;
+        } else if (turned[u]) {
+          h -= hq;
+          src = static_cast<const bf16*>(A.k) + t * A.k_token_stride + h * A.k_head_stride;
+          if (koff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.k) + koff[tok] + h * A.kv.k_head_stride;
+        } else {
+          h -= hq + hkv;
+          src = static_cast<const bf16*>(A.v) + t * A.v_token_stride + h * A.v_head_stride;
+          if (voff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.v) + voff[tok] + h * A.kv.v_head_stride;
+        }
+        if (dst[u] == nullptr) continue;
+        a[u] = *reinterpret_cast<const uint4*>(src + oct[u] * 8);
+        b[u] = *reinterpret_cast<const uint4*>(src + half + oct[u] * 8);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (dst[u] == nullptr) continue;
+        if (turned[u]) {
+          uint32_t* aw = reinterpret_cast<uint32_t*>(&a[u]);
+          uint32_t* bw = reinterpret_cast<uint32_t*>(&b[u]);
+          const float4* tab = reinterpret_cast<const float4*>(&cs[tok][oct[u] * 8]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float4 r = tab[w];  // cos, sin of two pairs
+            const float2 x = unpack2(as_bf162(aw[w])), y = unpack2(as_bf162(bw[w]));
+            aw[w] = as_u32(pack2_rn(make_float2(x.x * r.x - y.x * r.y, x.y * r.z - y.y * r.w)));
+            bw[w] = as_u32(pack2_rn(make_float2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w)));
+          }
+        }
+        *reinterpret_cast<uint4*>(dst[u] + oct[u] * 8) = a[u];
+        *reinterpret_cast<uint4*>(dst[u] + half + oct[u] * 8) = b[u];
+      }
+    }
+  }
+}
+
+int check_paged_kv(const hyena_paged_kv& kv) {
+  HB_REQUIRE(kv.k != nullptr && kv.v != nullptr && kv.page_table != nullptr, "paged cache: null pointer");
+  HB_REQUIRE(aligned16(kv.k) && aligned16(kv.v), "paged cache: k / v must be 16-byte aligned");
+  HB_REQUIRE(kv.k_page_stride % 8 == 0 && kv.k_token_stride % 8 == 0 && kv.k_head_stride % 8 == 0 &&
+                 kv.v_page_stride % 8 == 0 && kv.v_token_stride % 8 == 0 && kv.v_head_stride % 8 == 0,
+             "paged cache: strides must be multiples of 8 elements");
+  HB_REQUIRE(kv.page_size > 0 && kv.page_size % 16 == 0, "paged cache: page_size must be a positive multiple of 16");
+  HB_REQUIRE(kv.num_pages > 0 && kv.pages_per_request > 0 && kv.page_table_stride >= 0,
+             "paged cache: no pages");
+  HB_REQUIRE((long long)kv.pages_per_request * kv.page_size < (1ll << 31) - 65536,
+             "paged cache: a request's pages must hold fewer than 2^31 - 65536 positions");
+  HB_REQUIRE(kv.kv_heads > 0, "paged cache: kv_heads must be positive");
+  HB_REQUIRE(kv.head_dim == 64 || kv.head_dim == 128, "paged cache: head_dim must be 64 or 128");
+  return HYENA_OK;
+}
+
+int kv_append_launch(const hyena_kv_append_args& A, cudaStream_t st) {
+  HB_REQUIRE(A.T >= 0 && A.num_requests >= 0, "kv_append: negative sizes");
+  if (A.T == 0 || A.num_requests == 0) return HYENA_OK;
+  const int rc = check_paged_kv(A.kv);
+  if (rc) return rc;
+  HB_REQUIRE(A.k && A.v && A.positions, "kv_append: null pointer");
+  HB_REQUIRE((A.q == nullptr) == (A.q_out == nullptr), "kv_append: q and q_out go together");
+  HB_REQUIRE(A.q == nullptr || A.heads > 0, "kv_append: heads must be positive");
+  HB_REQUIRE(aligned16(A.q) && aligned16(A.q_out) && aligned16(A.k) && aligned16(A.v),
+             "kv_append: q, k, v must be 16-byte aligned");
+  HB_REQUIRE(A.q_token_stride % 8 == 0 && A.q_head_stride % 8 == 0 && A.q_out_token_stride % 8 == 0 &&
+                 A.q_out_head_stride % 8 == 0 && A.k_token_stride % 8 == 0 && A.k_head_stride % 8 == 0 &&
+                 A.v_token_stride % 8 == 0 && A.v_head_stride % 8 == 0,
+             "kv_append: strides must be multiples of 8 elements");
+  HB_REQUIRE(A.rope_theta > 0.0 && std::isfinite(A.rope_theta), "kv_append: rope_theta must be positive");
+  KvAppendParams P;
+  P.a = A;
+  const int half = A.kv.head_dim / 2;
+  const double step = std::pow(A.rope_theta, -1.0 / half);
+  double f = 1.0 / (2.0 * 3.14159265358979323846);
+  for (int i = 0; i < half; ++i, f *= step) P.turns[i] = f;
+  // One token a block until the GPU has a few blocks an SM, then four.
+  if (A.T <= 8 * num_sms()) {
+    launch_kernel(kv_append_kernel<1>, dim3((unsigned)A.T), dim3(KV_THREADS), 0, st, 0u, P);
+  } else {
+    launch_kernel(kv_append_kernel<4>, dim3((unsigned)((A.T + 3) / 4)), dim3(KV_THREADS), 0, st, 0u, P);
+  }
+  return check_launch("kv_append_kernel");
+}
+
+}  // namespace hb

@@ -21,7 +21,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import DecodeArgs, LayerParams, PrefillArgs, StateView
+from ._lib import (DecodeArgs, KvAppendArgs, LayerParams, PagedAttentionArgs, PrefillArgs,
+                   StateView)
 
 BF16 = torch.bfloat16
 E4M3 = torch.float8_e4m3fn
@@ -480,3 +481,269 @@ def gemm_bf16(a, b, bias=None, out=None):
                                    C.c_size_t(0 if ws is None else ws.numel() * 4), _stream()),
                "hyena_gemm_bf16")
     return out
+
+
+# ---------------------------------------------------------------- attention cache, gated MLP
+ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2}
+
+
+def _operands(**tensors):
+    """Checks that the given tensors (None: absent) are on one CUDA device and
+    need no gradient; returns the device.  These operators have no backward pass."""
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires grad: this operator has no backward pass "
+                             "(call it under torch.no_grad())")
+    return device
+
+
+def _launch_on(device, launch):
+    """launch(stream) with `device` current, on its current stream."""
+    if device.index == torch.cuda.current_device():
+        return launch(_stream())
+    with torch.cuda.device(device):
+        return launch(_stream())
+
+
+def _rows3(t, name, heads=None, dim=None):
+    if t.dim() != 3 or t.dtype != BF16 or t.stride(2) != 1:
+        raise ValueError(f"{name} must be (tokens, heads, head_dim) bf16 with unit last stride, "
+                         f"got {tuple(t.shape)} {t.dtype}")
+    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{name} must have {heads} heads of {dim}, got {tuple(t.shape)}")
+
+
+def _ints(t, name, at_least):
+    """A 1-D contiguous int32 view (converted if need be) of at least `at_least` elements."""
+    if t.dim() != 1 or t.shape[0] < at_least:
+        raise ValueError(f"{name} must be 1-D with at least {at_least} elements, got {tuple(t.shape)}")
+    if t.is_floating_point() or t.dtype == torch.bool:
+        raise ValueError(f"{name} must hold integers, got {t.dtype}")
+    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+
+
+def _paged_kv(kv, k_cache, v_cache, page_table, requests):
+    """Fills the hyena_paged_kv `kv`; returns the page table it points to."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dim() != 4 or t.dtype != BF16 or t.stride(3) != 1:
+            raise ValueError(f"{name} must be (pages, page size, kv heads, head_dim) bf16 with unit "
+                             f"last stride, got {tuple(t.shape)} {t.dtype}")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
+    if page_table.dim() != 2 or page_table.shape[0] < requests or page_table.is_floating_point():
+        raise ValueError(f"page_table must be (>= {requests} requests, pages) int, "
+                         f"got {tuple(page_table.shape)} {page_table.dtype}")
+    if page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        page_table = page_table.to(torch.int32).contiguous()
+    kv.k, kv.v = k_cache.data_ptr(), v_cache.data_ptr()
+    kv.k_page_stride, kv.k_token_stride, kv.k_head_stride, _ = k_cache.stride()
+    kv.v_page_stride, kv.v_token_stride, kv.v_head_stride, _ = v_cache.stride()
+    kv.page_table, kv.page_table_stride = page_table.data_ptr(), page_table.stride(0)
+    kv.num_pages, kv.page_size, kv.kv_heads, kv.head_dim = k_cache.shape
+    kv.pages_per_request = page_table.shape[1]
+    return page_table
+
+
+def _flags_ptr(error_flags):
+    if error_flags is None:
+        return None
+    _require(error_flags.dtype == torch.int32 and error_flags.numel() >= 1,
+             "error_flags must be an int32 tensor")
+    return error_flags.data_ptr()
+
+
+def kv_append(q, k, v, positions, k_cache, v_cache, page_table, query_start_loc=None, *,
+              rope_theta=10000.0, q_out=None, error_flags=None):
+    """Rotary embedding of a step's queries and keys, with the rotated keys and the
+    values written into the paged cache on the way (hyena_kv_append; the rotation
+    of Evo2Attention, model.py:104-152).
+
+    q (T, heads, D) or None; k, v (T, kv_heads, D): bf16, any token and head
+    strides (views of the fused projection's output will do), D 64 or 128.
+    positions (T,): the token's position, which is its rotation and its row of
+    the cache; a negative one marks a token to leave alone.  Caches (pages, page
+    size, kv_heads, D) with any strides, written in place; position p of request
+    r lies in page page_table[r, p // page size], page size a multiple of 16.
+    Request r owns the tokens [query_start_loc[r], query_start_loc[r + 1])
+    (default: token r alone); tokens that no request owns are left alone.  A page
+    outside the cache is not written and sets HYENA_FLAG_BLOCK_RANGE in
+    error_flags.  No two tokens of a step may name the same row.
+
+    Returns the rotated queries: q_out (may be q) or a new tensor; None for q None."""
+    device = _operands(k=k, q=q, v=v, positions=positions, k_cache=k_cache, v_cache=v_cache,
+                       page_table=page_table, query_start_loc=query_start_loc, q_out=q_out,
+                       error_flags=error_flags)
+    T, dim = k.shape[0], k_cache.shape[-1]
+    kv_heads = k_cache.shape[2] if k_cache.dim() == 4 else None
+    _rows3(k, "k", kv_heads, dim)
+    _rows3(v, "v", kv_heads, dim)
+    _require(v.shape[0] == T, f"v has {v.shape[0]} tokens, k {T}")
+    if q is not None:
+        _rows3(q, "q", None, dim)
+        _require(q.shape[0] == T, f"q has {q.shape[0]} tokens, k {T}")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=BF16, device=device)
+        else:
+            _rows3(q_out, "q_out", q.shape[1], dim)
+            _require(q_out.shape[0] == T, f"q_out has {q_out.shape[0]} tokens, q {T}")
+    else:
+        _require(q_out is None, "q_out without q")
+    positions = _ints(positions, "positions", T)
+    if query_start_loc is not None:
+        query_start_loc = _ints(query_start_loc, "query_start_loc", 1)
+        requests = query_start_loc.shape[0] - 1
+    else:
+        requests = page_table.shape[0]
+    a = KvAppendArgs()
+    table = _paged_kv(a.kv, k_cache, v_cache, page_table, requests)
+    if T == 0 or requests == 0:
+        return q_out
+    if q is not None:
+        a.q, (a.q_token_stride, a.q_head_stride, _) = q.data_ptr(), q.stride()
+        a.q_out, (a.q_out_token_stride, a.q_out_head_stride, _) = q_out.data_ptr(), q_out.stride()
+        a.heads = q.shape[1]
+    a.k, (a.k_token_stride, a.k_head_stride, _) = k.data_ptr(), k.stride()
+    a.v, (a.v_token_stride, a.v_head_stride, _) = v.data_ptr(), v.stride()
+    a.positions = positions.data_ptr()
+    a.query_start_loc = None if query_start_loc is None else query_start_loc.data_ptr()
+    a.T, a.num_requests = T, requests
+    a.rope_theta = rope_theta
+    a.error_flags = _flags_ptr(error_flags)
+    _lib.check(_launch_on(device, lambda st: _lib.load().hyena_kv_append(C.byref(a), st)),
+               "hyena_kv_append")
+    del table  # alive until the launch returned
+    return q_out
+
+
+def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=None, *,
+                    shared_lens=None, group_start=None, scale=None, out=None, error_flags=None):
+    """Causal attention of a step's queries over the paged cache, the leading keys
+    that the requests of a group share read once for the group
+    (hyena_paged_attention; Evo2Attention's softmax attention, model.py:104-152).
+
+    q (T, heads, D) bf16, heads a multiple of kv_heads; caches and page_table as
+    for kv_append.  seq_lens (B,): keys of request r, the step's own tokens
+    (appended before) included; its n queries sit at the last n positions and see
+    the keys up to their own.  A request with seq_lens 0 (padding) gets zeros;
+    rows that no request owns are left alone (uninitialised in a new `out`).
+    shared_lens (G,): requests group_start[g] .. group_start[g + 1] - 1 (default:
+    one group of all) name the same rows for their first shared_lens[g] keys; a
+    run longer than what all of the group's queries see is cut, so the result
+    never depends on it.  scale defaults to D ** -0.5.  B + G is at most 2048.
+
+    One launch, and one that joins the pieces of split rows; lengths and tables
+    are read on the device, so a captured graph serves growing contexts.  The
+    workspace comes from torch's caching allocator.  Returns (T, heads, D) bf16."""
+    device = _operands(q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+                       seq_lens=seq_lens, query_start_loc=query_start_loc, shared_lens=shared_lens,
+                       group_start=group_start, out=out, error_flags=error_flags)
+    _rows3(q, "q", None, k_cache.shape[-1])
+    T, heads, dim = q.shape
+    seq_lens = _ints(seq_lens, "seq_lens", 0)
+    requests = seq_lens.shape[0]
+    if query_start_loc is not None:
+        query_start_loc = _ints(query_start_loc, "query_start_loc", requests + 1)
+    groups = 0
+    if shared_lens is not None:
+        shared_lens = _ints(shared_lens, "shared_lens", 1)
+        groups = shared_lens.shape[0]
+        if group_start is not None:
+            group_start = _ints(group_start, "group_start", groups + 1)
+        _require(group_start is not None or groups == 1, "several groups need group_start")
+    else:
+        _require(group_start is None, "group_start without shared_lens")
+    if out is None:
+        out = torch.empty(q.shape, dtype=BF16, device=device)
+    else:
+        _rows3(out, "out", heads, dim)
+        _require(out.shape[0] == T, f"out has {out.shape[0]} tokens, q {T}")
+    a = PagedAttentionArgs()
+    table = _paged_kv(a.kv, k_cache, v_cache, page_table, requests)
+    if T == 0 or requests == 0:
+        return out
+    a.q, (a.q_token_stride, a.q_head_stride, _) = q.data_ptr(), q.stride()
+    a.out, (a.out_token_stride, a.out_head_stride, _) = out.data_ptr(), out.stride()
+    a.seq_lens = seq_lens.data_ptr()
+    a.query_start_loc = None if query_start_loc is None else query_start_loc.data_ptr()
+    a.shared_lens = None if shared_lens is None else shared_lens.data_ptr()
+    a.group_start = None if group_start is None else group_start.data_ptr()
+    a.T, a.num_requests, a.num_groups, a.heads = T, requests, groups, heads
+    a.scale = dim ** -0.5 if scale is None else scale
+    a.error_flags = _flags_ptr(error_flags)
+    lib = _lib.load()
+
+    def launch(st):
+        n = lib.hyena_paged_attention_workspace_size(C.byref(a))
+        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        return lib.hyena_paged_attention(C.byref(a), None if ws is None else ws.data_ptr(), n, st)
+
+    _lib.check(_launch_on(device, launch), "hyena_paged_attention")
+    del table  # alive until the launch returned
+    return out
+
+
+def _matrix(t, name, cols=None):
+    if t.dim() != 2 or t.dtype != BF16 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} must be a 2-D bf16 tensor with unit column stride, "
+                         f"got {tuple(t.shape)} {t.dtype}")
+    if cols is not None and t.shape[1] != cols:
+        raise ValueError(f"{name} must have {cols} columns, got {tuple(t.shape)}")
+
+
+def gemm_gated_bf16(a, b1, b2, activation="none", out=None):
+    """out (M, N) bf16 = act(a . b1^T) * (a . b2^T): a (M, K), b1 and b2 (N, K)
+    bf16, activation "none", "gelu" (erf) or "silu", fp32 up to the one rounding
+    (hyena_gemm_gated_bf16, tcgen05).  K % 64 == 0, N % 8 == 0."""
+    device = _operands(a=a, b1=b1, b2=b2, out=out)
+    _matrix(a, "a")
+    M, K = a.shape
+    _matrix(b1, "b1", K)
+    _matrix(b2, "b2", K)
+    N = b1.shape[0]
+    _require(b2.shape[0] == N, f"b1 has {N} rows, b2 {b2.shape[0]}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if out is None:
+        out = torch.empty(M, N, dtype=BF16, device=device)
+    else:
+        _matrix(out, "out", N)
+        _require(out.shape[0] == M, f"out must have {M} rows, got {out.shape[0]}")
+    # a one-row tensor may carry any row stride: its length is what counts
+    ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1]  # noqa: E731
+    _lib.check(_launch_on(device, lambda st: _lib.load().hyena_gemm_gated_bf16(
+        a.data_ptr(), ld(a), b1.data_ptr(), ld(b1), b2.data_ptr(), ld(b2), out.data_ptr(), ld(out),
+        M, N, K, ACTIVATIONS[activation], st)), "hyena_gemm_gated_bf16")
+    return out
+
+
+def gated_mlp(x, w1, w2, w3, activation="none", out=None):
+    """The gated feed-forward block of Evo2MLP (model.py:77-101):
+    out (M, H) bf16 = (act(x . w1^T) * (x . w2^T)) . w3^T, x (M, H), w1 and w2
+    (I, H), w3 (H_out, I) bf16; H and I multiples of 64.  Two launches: both
+    projections with the activation and the product (gemm_gated_bf16, whose
+    result is the one bf16 intermediate), then gemm_bf16."""
+    _operands(x=x, w1=w1, w2=w2, w3=w3, out=out)
+    _matrix(w1, "w1")
+    _matrix(w3, "w3", w1.shape[0])
+    _require(w1.shape[0] % 64 == 0, f"the inner width must be a multiple of 64, got {w1.shape[0]}")
+    if out is not None:
+        _matrix(out, "out", w3.shape[0])
+        _require(out.shape[0] == x.shape[0], f"out must have {x.shape[0]} rows, got {out.shape[0]}")
+    h = gemm_gated_bf16(x, w1, w2, activation)
+    if out is None:
+        out = torch.empty(h.shape[0], w3.shape[0], dtype=BF16, device=h.device)
+    if h.shape[0] == 0:
+        return out
+    if h.device.index == torch.cuda.current_device():
+        return gemm_bf16(h, w3, out=out)
+    with torch.cuda.device(h.device):
+        return gemm_bf16(h, w3, out=out)

@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define HYENA_ABI_VERSION 8
+#define HYENA_ABI_VERSION 9
 
 #if defined(__GNUC__)
 #define HYENA_API __attribute__((visibility("default")))
@@ -341,6 +341,100 @@ HYENA_API void hyena_set_gemm_max_ctas(int32_t n);
  * work on other streams and want SMs released between kernels.  Process-wide.
  * No counterpart in the reference. */
 HYENA_API void hyena_set_launch_chaining(int32_t enable);
+
+/* ---------------------------------------------------------------- paged attention
+ * The attention layers' key/value cache.  Row `at` of page p, head h:
+ * k + p * k_page_stride + at * k_token_stride + h * k_head_stride (elements;
+ * head_dim contiguous bf16), v alike.  Position j of request r lies in page
+ * page_table[r * page_table_stride + j / page_size], row j % page_size; requests
+ * may name the same pages.  page_size is a multiple of 16, head_dim 64 or 128,
+ * strides multiples of 8 elements, bases 16-byte aligned.  A page outside
+ * [0, num_pages), or a position beyond the table, sets HYENA_FLAG_BLOCK_RANGE
+ * and is neither read nor written. */
+typedef struct hyena_paged_kv {
+  void* k;
+  void* v;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  int32_t pages_per_request; /* columns of page_table */
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+} hyena_paged_kv;
+
+/* Rotary embedding (neox halves, Evo2Attention, model.py:104-152) of a step's
+ * queries and keys, the keys and values written into the paged cache on the way:
+ * for token t of request r at position p = positions[t],
+ *   q_out[t] = rot(q[t], p);  cache.k[p] = rot(k[t], p);  cache.v[p] = v[t],
+ * rot pairs element i with i + head_dim / 2 at angle p * theta^(-2i/head_dim),
+ * formed in fp64, applied in fp32, rounded once.  Request r owns tokens
+ * [query_start_loc[r], query_start_loc[r+1]) (NULL: token r only); tokens that no
+ * request owns and tokens with a negative position are left alone, in q_out too.
+ * q may be q_out (in place); q == q_out == NULL appends only.  No two tokens of a
+ * step may name the same cache row. */
+typedef struct hyena_kv_append_args {
+  const void* q; int64_t q_token_stride, q_head_stride;          /* (T, heads, head_dim) bf16 */
+  void* q_out; int64_t q_out_token_stride, q_out_head_stride;
+  const void* k; int64_t k_token_stride, k_head_stride;          /* (T, kv_heads, head_dim) bf16 */
+  const void* v; int64_t v_token_stride, v_head_stride;
+  const int32_t* positions;        /* (T) */
+  const int32_t* query_start_loc;  /* (num_requests + 1) or NULL */
+  int32_t T;
+  int32_t num_requests;
+  int32_t heads;
+  hyena_paged_kv kv;
+  double rope_theta;
+  int32_t* error_flags;            /* optional device int */
+} hyena_kv_append_args;
+
+HYENA_API int hyena_kv_append(const hyena_kv_append_args* a, void* stream);
+
+/* Causal softmax attention of a step's queries over the paged cache: query i of
+ * the n of request r sits at position seq_lens[r] - n + i and sees the keys
+ * j <= that position (seq_lens counts the step's own tokens, appended before).
+ * A query that sees no key (seq_lens[r] = 0: a padded request) gives zeros;
+ * output rows that no request owns are left alone; keys that a query does not see
+ * do not touch its result, whatever they hold.
+ * Sharing: the requests [group_start[g], group_start[g+1]) (NULL: all, one group)
+ * name the same key and value rows for their first shared_lens[g] positions,
+ * which are then read once for the group.  What a query sees is not changed by
+ * it: a run longer than what every query of the group sees is cut.
+ * heads is a multiple of kv_heads (query head h reads head h / (heads / kv_heads)).
+ * The lengths are read on the device: one captured launch serves growing contexts. */
+typedef struct hyena_paged_attention_args {
+  const void* q; int64_t q_token_stride, q_head_stride;          /* (T, heads, head_dim) bf16 */
+  void* out; int64_t out_token_stride, out_head_stride;
+  const int32_t* seq_lens;         /* (num_requests) */
+  const int32_t* query_start_loc;  /* (num_requests + 1) or NULL: token r only */
+  const int32_t* shared_lens;      /* (num_groups) or NULL: nothing shared */
+  const int32_t* group_start;      /* (num_groups + 1) or NULL */
+  int32_t T;
+  int32_t num_requests;            /* with num_groups at most 2048 */
+  int32_t num_groups;              /* 0 with shared_lens NULL */
+  int32_t heads;
+  float scale;
+  hyena_paged_kv kv;
+  int32_t* error_flags;
+} hyena_paged_attention_args;
+
+/* Bytes of 16-byte aligned device memory the call needs (0 for invalid arguments). */
+HYENA_API size_t hyena_paged_attention_workspace_size(const hyena_paged_attention_args* a);
+HYENA_API int hyena_paged_attention(const hyena_paged_attention_args* a, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- gated projections
+ * out(M,N) bf16 = act(A(M,K) . B1(N,K)^T) * (A . B2(N,K)^T), all bf16 with fp32
+ * accumulators and one rounding: the first half of Evo2MLP (model.py:77-101);
+ * hyena_gemm_bf16 with l3 is the second.  Same requirements as hyena_gemm_bf16. */
+#define HYENA_ACT_NONE 0
+#define HYENA_ACT_GELU 1  /* x Phi(x), with erf */
+#define HYENA_ACT_SILU 2  /* x / (1 + exp(-x)) */
+HYENA_API int hyena_gemm_gated_bf16(const void* A, int64_t lda, const void* B1, int64_t ldb1,
+                                    const void* B2, int64_t ldb2, void* out, int64_t ldo, int32_t M,
+                                    int32_t N, int32_t K, int32_t act, void* stream);
 
 /* ---------------------------------------------------------------- misc */
 HYENA_API int hyena_abi_version(void);
