@@ -28,23 +28,12 @@ namespace attn {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int KT = 16;          // keys of a warp's tile
 constexpr int ROWS = 16;        // rows of an item
 constexpr int STAGES = 3;       // tiles in flight per warp
 constexpr int MIN_CHUNK = 128;  // keys
 constexpr int MAX_SEGMENTS = 2048;
 constexpr int ITEMS_PER_CTA = 8;
-
-struct Params {
-  hyena_paged_attention_args a;
-  int groups;      // 0: nothing shared
-  int per;         // query heads of one key/value head
-  float scale;     // scale * log2(e)
-  int slots_s, slots_o;  // pieces a row may have: of the shared run, of its own keys
-  int32_t* plan;   // {chunk_s, chunk_o}, then each group's shared run
-  float2* ml;      // [T * heads][slots]: (m, l)
-  float* o;        // [T * heads][slots][D]
-};
+constexpr int TC_MIN_ROWS = 16;  // mean rows of a group and key/value head
 
 struct Plan {
   int chunk_s, chunk_o, items;
@@ -53,40 +42,6 @@ struct Plan {
   int* leader; // [groups] the request whose pages stand for it
 };
 
-__device__ __forceinline__ int query_begin(const Params& P, int r) {
-  return P.a.query_start_loc != nullptr ? __ldg(P.a.query_start_loc + r) : r;
-}
-// Queries of request r and their first row.  Rows beyond T do not exist.
-__device__ __forceinline__ int queries(const Params& P, int r, int& begin) {
-  begin = query_begin(P, r);
-  int end = query_begin(P, r + 1);
-  end = end < P.a.T ? end : P.a.T;
-  return begin >= 0 && end > begin ? end - begin : 0;
-}
-__device__ __forceinline__ int length(const Params& P, int r) {
-  const int cap = P.a.kv.pages_per_request * P.a.kv.page_size;
-  const int n = __ldg(P.a.seq_lens + r);
-  return n < 0 ? 0 : n < cap ? n : cap;
-}
-// Group of request r, or -1.
-__device__ __forceinline__ int group_of(const Params& P, int r) {
-  if (P.groups == 0) return -1;
-  if (P.a.group_start == nullptr) return 0;
-  const int g = find_segment(P.a.group_start, P.groups, r);
-  return __ldg(P.a.group_start + g) <= r && r < __ldg(P.a.group_start + g + 1) ? g : -1;
-}
-__device__ __forceinline__ int group_begin(const Params& P, int g) {
-  int r = P.a.group_start != nullptr ? __ldg(P.a.group_start + g) : g == 0 ? 0 : P.a.num_requests;
-  r = r < 0 ? 0 : r;
-  return r < P.a.num_requests ? r : P.a.num_requests;
-}
-// Query rows of group g (tokens) and the first of them, inside [0, T).
-__device__ __forceinline__ int group_queries(const Params& P, int g, int& begin) {
-  begin = min(max(query_begin(P, group_begin(P, g)), 0), P.a.T);
-  const int end = min(query_begin(P, group_begin(P, g + 1)), P.a.T);
-  return end > begin ? end - begin : 0;
-}
-__host__ __device__ __forceinline__ int ceil_div(int a, int b) { return a / b + (a % b != 0); }
 __device__ __forceinline__ int row_tiles(const Params& P, int nq) {
   return (int)(((long long)nq * P.per + ROWS - 1) / ROWS);
 }
@@ -106,27 +61,7 @@ __device__ __forceinline__ int chunk_keys(long long work, int longest, int slots
 __device__ void make_plan(const Params& P, Plan& L, long long* red) {
   const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int B = P.a.num_requests, G = P.groups, hkv = P.a.kv.kv_heads;
-  const int cap = P.a.kv.pages_per_request * P.a.kv.page_size;
-  for (int g = tid; g < G; g += THREADS) {
-    const int n = __ldg(P.a.shared_lens + g);
-    L.shared[g] = n < 0 ? 0 : n < cap ? n : cap;
-    L.leader[g] = 0x7fffffff;
-  }
-  __syncthreads();
-  if (G > 0) {
-    for (int r = tid; r < B; r += THREADS) {
-      int begin;
-      const int n = queries(P, r, begin), len = length(P, r), g = group_of(P, r);
-      if (n > 0 && len > 0 && g >= 0) {  // a padded request (no keys) does not count
-        atomicMin(&L.shared[g], max(len - n + 1, 0));
-        atomicMin(&L.leader[g], r);
-      }
-    }
-    __syncthreads();
-    for (int g = tid; g < G; g += THREADS)
-      L.shared[g] = L.leader[g] < B ? L.shared[g] & ~(KT - 1) : 0;
-    __syncthreads();
-  }
+  shared_runs<THREADS>(P, L.shared, L.leader);
   long long v[4] = {0, 0, 0, 0};  // work and longest, shared and own
   for (int s = tid; s < G + B; s += THREADS) {
     if (s < G) {
@@ -173,7 +108,7 @@ __device__ void make_plan(const Params& P, Plan& L, long long* red) {
     int items;
     if (s < G) {
       int begin;
-      items = ceil_div(L.shared[s], L.chunk_s) * row_tiles(P, group_queries(P, s, begin)) * hkv;
+      items = P.tc ? 0 : ceil_div(L.shared[s], L.chunk_s) * row_tiles(P, group_queries(P, s, begin)) * hkv;
     } else {
       int begin;
       const int n = queries(P, s - G, begin), g = group_of(P, s - G);
@@ -238,11 +173,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // Byte offset of 16-byte chunk c of row `row` in a tile of D-element rows, the
 // chunks permuted within groups of eight so that eight rows' same chunk (an
 // ldmatrix phase) lies in distinct banks.
@@ -286,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, 2) stream_kernel(const __grid_constan
   make_plan(P, L, red);
   if (blockIdx.x == 0 && P.plan != nullptr) {
     if (tid == 0) {
-      P.plan[0] = L.chunk_s;
+      if (!P.tc) P.plan[0] = L.chunk_s;
       P.plan[1] = L.chunk_o;
     }
     for (int g = tid; g < G; g += THREADS) P.plan[2 + g] = L.shared[g];
@@ -724,6 +654,9 @@ static int launch(const hyena_paged_attention_args& A, const Slots& S, void* ws,
   P.scale = A.scale * 1.4426950408889634f;
   P.slots_s = S.s;
   P.slots_o = S.o;
+  // Shared runs of more rows than one 16-row tile go to the tcgen05 kernel.
+  P.tc = S.s > 0 && A.num_groups <= MAX_TC_GROUPS &&
+         (long long)A.T * P.per > (long long)TC_MIN_ROWS * A.num_groups;
   P.plan = nullptr;
   P.ml = nullptr;
   P.o = nullptr;
@@ -743,6 +676,10 @@ static int launch(const hyena_paged_attention_args& A, const Slots& S, void* ws,
   const long long bound = (rows / A.kv.kv_heads / ROWS + segments) * A.kv.kv_heads * (S.s + S.o);
   const long long ctas = std::min<long long>(2ll * num_sms(), bound);
   launch_kernel(stream_kernel<D>, dim3((unsigned)ctas), dim3(THREADS), smem, st, 0u, P);
+  if (P.tc) {
+    const int rc = shared_launch(P, st);
+    if (rc) return rc;
+  }
   if (S.join) {
     // a block a row while those fill one wave of 16 blocks an SM
     if (rows <= 16ll * num_sms())

@@ -1,4 +1,6 @@
-// The paged attention cache, shared by kvcache.cu and attention.cu.
+// The paged attention cache and the pieces of attention over it, shared by
+// kvcache.cu, attention.cu (segments of few rows; joining) and
+// attention_shared.cu (shared runs of many rows).
 #pragma once
 
 #include "common.cuh"
@@ -7,4 +9,94 @@ namespace hb {
 
 int check_paged_kv(const hyena_paged_kv& kv);
 
+namespace attn {
+
+constexpr int KT = 16;  // a shared run is cut to whole tiles of this many keys
+
+struct Params {
+  hyena_paged_attention_args a;
+  int groups;      // 0: nothing shared
+  int per;         // query heads of one key/value head
+  float scale;     // scale * log2(e)
+  int slots_s, slots_o;  // pieces a row may have: of the shared run, of its own keys
+  int32_t* plan;   // {chunk_s, chunk_o}, then each group's shared run
+  int tc;          // the shared runs go to attention_shared.cu
+  float2* ml;      // [T * heads][slots]: (m, l)
+  float* o;        // [T * heads][slots][D]
+};
+
+__device__ __forceinline__ int query_begin(const Params& P, int r) {
+  return P.a.query_start_loc != nullptr ? __ldg(P.a.query_start_loc + r) : r;
+}
+// Queries of request r and their first row.  Rows beyond T do not exist.
+__device__ __forceinline__ int queries(const Params& P, int r, int& begin) {
+  begin = query_begin(P, r);
+  int end = query_begin(P, r + 1);
+  end = end < P.a.T ? end : P.a.T;
+  return begin >= 0 && end > begin ? end - begin : 0;
+}
+__device__ __forceinline__ int length(const Params& P, int r) {
+  const int cap = P.a.kv.pages_per_request * P.a.kv.page_size;
+  const int n = __ldg(P.a.seq_lens + r);
+  return n < 0 ? 0 : n < cap ? n : cap;
+}
+// Group of request r, or -1.
+__device__ __forceinline__ int group_of(const Params& P, int r) {
+  if (P.groups == 0) return -1;
+  if (P.a.group_start == nullptr) return 0;
+  const int g = find_segment(P.a.group_start, P.groups, r);
+  return __ldg(P.a.group_start + g) <= r && r < __ldg(P.a.group_start + g + 1) ? g : -1;
+}
+__device__ __forceinline__ int group_begin(const Params& P, int g) {
+  int r = P.a.group_start != nullptr ? __ldg(P.a.group_start + g) : g == 0 ? 0 : P.a.num_requests;
+  r = r < 0 ? 0 : r;
+  return r < P.a.num_requests ? r : P.a.num_requests;
+}
+// Query rows of group g (tokens) and the first of them, inside [0, T).
+__device__ __forceinline__ int group_queries(const Params& P, int g, int& begin) {
+  begin = min(max(query_begin(P, group_begin(P, g)), 0), P.a.T);
+  const int end = min(query_begin(P, group_begin(P, g + 1)), P.a.T);
+  return end > begin ? end - begin : 0;
+}
+__host__ __device__ __forceinline__ int ceil_div(int a, int b) { return a / b + (a % b != 0); }
+
+// The groups' shared runs and the requests whose page tables stand for them
+// (leader), in shared memory: shared_lens cut to what every query of the group
+// sees, then to whole KT-key tiles.  Padded requests (no keys) do not count.
+template <int NTHREADS>
+__device__ __forceinline__ void shared_runs(const Params& P, int* shared, int* leader) {
+  const int G = P.groups, B = P.a.num_requests, tid = (int)threadIdx.x;
+  const int cap = P.a.kv.pages_per_request * P.a.kv.page_size;
+  if (G == 0) return;
+  for (int g = tid; g < G; g += NTHREADS) {
+    const int n = __ldg(P.a.shared_lens + g);
+    shared[g] = n < 0 ? 0 : n < cap ? n : cap;
+    leader[g] = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int r = tid; r < B; r += NTHREADS) {
+    int begin;
+    const int n = queries(P, r, begin), len = length(P, r), g = group_of(P, r);
+    if (n > 0 && len > 0 && g >= 0) {
+      atomicMin(&shared[g], max(len - n + 1, 0));
+      atomicMin(&leader[g], r);
+    }
+  }
+  __syncthreads();
+  for (int g = tid; g < G; g += NTHREADS) shared[g] = leader[g] < B ? shared[g] & ~(KT - 1) : 0;
+  __syncthreads();
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Groups the tensor-core kernel of the shared runs takes (its plan's room).
+constexpr int MAX_TC_GROUPS = 64;
+int shared_launch(const Params& P, cudaStream_t st);
+int shared_wait_timeouts(int32_t* count, int reset);
+
+}  // namespace attn
 }  // namespace hb

@@ -1,0 +1,566 @@
+// Attention over the keys that the requests of a group share: one tcgen05 pass
+// for the queries of the whole group (see attention.cu for the decomposition
+// into pieces and for the join).
+//
+// An item is NT x 128 query rows (queries x heads of one key/value head) against
+// a chunk of the shared run; one CTA per SM walks its items:
+//   warps 0 .. 4 NT - 1  softmax: a thread owns one row; its 128 scores of a key
+//                tile come from TMEM, 2^(s - m) goes back as bf16 over the same
+//                columns, ready to be the A operand of the value product
+//   next warp    tcgen05.mma issue (one thread): S_t = Q_t K^T (K-major operands),
+//                O_t += P_t V with P_t in TMEM and V read MN-major as it lies in
+//                the cache; O stays in TMEM for the whole item
+//   last warp    TMA: tiles of 128 keys (256 B rows, SWIZZLE_128B, two 64-column
+//                halves) by the largest box that a page holds whole; keys and
+//                values take turns in one ring
+// Every row sees every key of the run, so only the run's last tile has a mask.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the m
+// it is scaled by: the weights then stay below 2^8, where bf16 and fp32 round as
+// well as at 1, and the pass over O's columns (TMEM -> registers -> TMEM) is rare
+// instead of once a tile.  m and l leave with the piece, so nothing is lost.
+//
+// NT = 1 keeps two score buffers (S of the next tile is computed under the
+// softmax); NT = 2 (256 rows) reads each key and value once for two row tiles,
+// whose softmax and matrix products alternate.  Bound by the keys' bytes up to
+// about 128 rows, beyond by the exponentials and the tensor pipe.
+//
+// Launched after the stream kernel as its programmatic dependent, it does not
+// wait for it at entry: that kernel's CTAs trigger only after their own wait, so
+// the kernels before it have completed, and the two share no data.  Every
+// thread waits at its end instead, so that the join kernel, which waits for this
+// one, finds both complete.
+#include <algorithm>
+
+#include "attention.cuh"
+#include "tcgen05.cuh"
+
+namespace hb {
+namespace attn {
+
+using namespace tc;
+
+constexpr int TILE_KEYS = 128;
+constexpr int BOX_MIN = 16;
+constexpr unsigned long long WAIT_NS = 4000000000ull;  // 4 s
+constexpr float RESCALE_LOG2 = 8.0f;
+constexpr int ITEM_OVERHEAD = 3;  // tiles that an item's start and end cost
+
+__device__ int g_shared_wait_timeouts;
+
+template <int D, int NT>
+struct Tc {
+  static constexpr int HALVES = D / 64;              // 64-column swizzled halves of a row
+  static constexpr int HALF_BYTES = TILE_KEYS * 128;
+  static constexpr int TILE_BYTES = HALVES * HALF_BYTES;  // 128 rows x D
+  static constexpr int FIT = (224 * 1024 - NT * TILE_BYTES) / TILE_BYTES;
+  static constexpr int SLOTS = FIT < 8 ? FIT : 8;
+  static constexpr int NBUF = NT == 1 ? 2 : 1;       // score buffers of a row tile
+  static constexpr int THREADS = NT * 128 + 64;
+  static constexpr uint32_t S_COL = 0, O_COL = 256;  // TMEM columns
+  static constexpr uint32_t TMEM_COLS = 512;
+};
+
+template <int D, int NT>
+struct __align__(1024) TcSmem {
+  uint8_t q[NT][Tc<D, NT>::TILE_BYTES];
+  uint8_t ring[Tc<D, NT>::SLOTS][Tc<D, NT>::TILE_BYTES];
+  uint64_t full[Tc<D, NT>::SLOTS], empty[Tc<D, NT>::SLOTS];
+  uint64_t q_full;
+  uint64_t s_full[NT][2], p_full[NT], pv_done[NT];
+  uint32_t bad[8];  // 16-key blocks of a tile whose page is out of range
+  uint32_t tmem;
+  unsigned long long best[16];
+  int chunk_tiles, items;
+  int first[MAX_TC_GROUPS + 1], shared[MAX_TC_GROUPS], leader[MAX_TC_GROUPS];
+};
+
+// Waits (bounded) for a phase; counts and flags an expired wait.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int32_t* flags) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = now_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (now_ns() - t0 > WAIT_NS) {
+      atomicAdd(&g_shared_wait_timeouts, 1);
+      flag_error(flags, HYENA_FLAG_WAIT);
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* bar, void* dst, int x,
+                                            int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(su32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(su32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+// D[128 x N] (+)= A[128 x 16] B[N x 16]^T, A in shared memory / in TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u));
+}
+// SWIZZLE_128B descriptor of an operand whose N (or M) index runs along the
+// 128-byte rows: 64-element atoms `lead` bytes apart along N, eight rows (K)
+// 1024 bytes.
+__device__ __forceinline__ uint64_t sw128_mn_desc(const void* p, uint32_t lead) {
+  const uint64_t addr = su32(p);
+  return ((addr & 0x3FFFFull) >> 4) | (uint64_t(lead >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// bf16 operands, fp32 accumulator, M = 128, N = n; b_mn: B is MN-major.
+__host__ __device__ constexpr uint32_t attn_idesc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(128 >> 4) << 24);
+}
+
+struct Item {
+  int group, leader, row0, rows, begin, head, chunk, k0, k1, tiles;
+};
+
+template <int D, int NT>
+__device__ __forceinline__ Item item_of(const Params& P, const TcSmem<D, NT>& S, int item) {
+  Item I;
+  int g = 0;
+  while (item >= S.first[g + 1]) ++g;
+  I.group = g;
+  I.leader = S.leader[g];
+  I.rows = group_queries(P, g, I.begin) * P.per;
+  const int row_tiles = ceil_div(I.rows, NT * 128), hkv = P.a.kv.kv_heads;
+  int rem = item - S.first[g];
+  I.row0 = rem % row_tiles * (NT * 128);
+  rem /= row_tiles;
+  I.head = rem % hkv;
+  I.chunk = rem / hkv;
+  I.k0 = I.chunk * S.chunk_tiles * TILE_KEYS;
+  const int end = S.shared[g];
+  I.k1 = end - I.k0 > S.chunk_tiles * TILE_KEYS ? I.k0 + S.chunk_tiles * TILE_KEYS : end;
+  I.tiles = ceil_div(I.k1 - I.k0, TILE_KEYS);
+  return I;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(Tc<D, NT>::THREADS, 1)
+shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensorMap map_k,
+              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k16,
+              const __grid_constant__ CUtensorMap map_v16, int box) {
+  using T = Tc<D, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  TcSmem<D, NT>& S = *reinterpret_cast<TcSmem<D, NT>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const hyena_paged_attention_args& A = P.a;
+  const int tid = (int)threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int G = P.groups, hkv = A.kv.kv_heads;
+
+  if (tid == 0) {
+    for (int s = 0; s < T::SLOTS; ++s) {
+      mbar_init(&S.full[s], 1);
+      mbar_init(&S.empty[s], 1);
+    }
+    mbar_init(&S.q_full, NT * 128);
+    for (int t = 0; t < NT; ++t) {
+      for (int b = 0; b < 2; ++b) mbar_init(&S.s_full[t][b], 2);
+      mbar_init(&S.p_full[t], 128);
+      mbar_init(&S.pv_done[t], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4 * NT) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     su32(&S.tmem)),
+                 "r"(T::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+
+  // ---- plan: the chunk length (in tiles) that lets the CTAs finish soonest,
+  // waves x (tiles of an item + its overhead), over the chunk counts of the
+  // longest run; then the groups' first items
+  shared_runs<T::THREADS>(P, S.shared, S.leader);
+  {
+    int longest = 0;
+    for (int g = 0; g < G; ++g) longest = max(longest, S.shared[g]);
+    const int most = ceil_div(longest, TILE_KEYS);
+    unsigned long long best = ~0ull;
+    for (int c = tid + 1; c <= P.slots_s && c <= max(most, 1); c += T::THREADS) {
+      const int n = max(ceil_div(most, c), 1);
+      long long items = 0;
+      for (int g = 0; g < G; ++g) {
+        int begin;
+        const int rows = group_queries(P, g, begin) * P.per;
+        items += (long long)ceil_div(rows, NT * 128) * hkv *
+                 ceil_div(ceil_div(S.shared[g], TILE_KEYS), n);
+      }
+      const unsigned long long cost = (unsigned long long)((items + gridDim.x - 1) / gridDim.x) *
+                                      (unsigned long long)(n + ITEM_OVERHEAD);
+      best = min(best, (cost << 24) | (unsigned long long)min(n, (1 << 24) - 1));
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, d));
+    if (lane == 0) S.best[warp] = best;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < T::THREADS / 32; ++w) best = min(best, S.best[w]);
+      const int n = (int)(best & 0xFFFFFFull);
+      int at = 0;
+      for (int g = 0; g < G; ++g) {
+        int begin;
+        const int rows = group_queries(P, g, begin) * P.per;
+        S.first[g] = at;
+        at += ceil_div(rows, NT * 128) * hkv * ceil_div(ceil_div(S.shared[g], TILE_KEYS), n);
+      }
+      S.first[G] = at;
+      S.items = at;
+      S.chunk_tiles = n;
+      if (blockIdx.x == 0) P.plan[0] = n * TILE_KEYS;
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = S.tmem;
+  const int items = S.items;
+
+  if (warp == 4 * NT + 1) {
+    // ---------------------------------------------------------------- loads
+    uint32_t u = 0, tile_no = 0;
+    bool ok = true;
+    for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x) {
+      const Item I = item_of<D, NT>(P, S, item);
+      const int32_t* table = A.kv.page_table + (long long)I.leader * A.kv.page_table_stride;
+      for (int i = 0; i < I.tiles && ok; ++i, ++tile_no) {
+        const int kpos = I.k0 + i * TILE_KEYS;
+        const int keys = min(TILE_KEYS, I.k1 - kpos);
+        // lane j: 16-key block j of the tile (its page), and whether it leads a
+        // whole box or stands alone in the tail
+        int page = 0, at = 0;
+        bool mine = lane < TILE_KEYS / BOX_MIN && lane * BOX_MIN < keys, good = true;
+        const bool whole = (lane * BOX_MIN / box + 1) * box <= keys;
+        if (mine) {
+          const int pos = kpos + lane * BOX_MIN;
+          page = __ldg(table + pos / A.kv.page_size);
+          at = pos % A.kv.page_size;
+          good = page >= 0 && page < A.kv.num_pages;
+          if (!good) flag_error(A.error_flags, HYENA_FLAG_BLOCK_RANGE);
+        }
+        const uint32_t bad = __ballot_sync(0xffffffffu, !good);
+        const uint32_t have = __ballot_sync(0xffffffffu, mine && good);
+        if (lane == 0) S.bad[tile_no & 7] = bad;
+        const bool leads = mine && good && (whole ? lane * BOX_MIN % box == 0 : true);
+        const uint32_t bytes = uint32_t(__popc(have)) * BOX_MIN * D * 2;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++u) {  // keys, then values
+          const int s = u % T::SLOTS;
+          ok = __all_sync(0xffffffffu, wait(&S.empty[s], ((u / T::SLOTS) & 1) ^ 1, A.error_flags));
+          if (!ok) break;
+          uint8_t* slot = S.ring[s];
+          if (kv == 1 && have != 0xFFu) {
+            // weights of absent keys are zero, but so must their values be
+            for (int r = lane; r < TILE_KEYS * T::HALVES * 8; r += 32) {
+              const int row = r / 8 % TILE_KEYS;
+              if (!((have >> (row / BOX_MIN)) & 1u))
+                *reinterpret_cast<uint4*>(slot + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          if (lane == 0) mbar_expect_tx(&S.full[s], bytes);
+          __syncwarp();
+          if (leads) {
+            const CUtensorMap* map = kv == 0 ? (whole ? &map_k : &map_k16) : (whole ? &map_v : &map_v16);
+#pragma unroll
+            for (int h = 0; h < T::HALVES; ++h)
+              tma_load_4d(map, &S.full[s], slot + h * T::HALF_BYTES + lane * BOX_MIN * 128, h * 64, at,
+                          I.head, page);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    // Drain: every issued copy has landed, and every slot's release has arrived,
+    // before the CTA can exit.
+    for (uint32_t i = u > (uint32_t)T::SLOTS ? u - T::SLOTS : 0; i < u; ++i) {
+      wait(&S.full[i % T::SLOTS], (i / T::SLOTS) & 1, A.error_flags);
+      if (ok) wait(&S.empty[i % T::SLOTS], (i / T::SLOTS) & 1, A.error_flags);
+    }
+  } else if (warp == 4 * NT) {
+    // ---------------------------------------------------------------- products
+    if (lane == 0) {
+      constexpr uint32_t ID_S = attn_idesc(TILE_KEYS, false), ID_O = attn_idesc(D, true);
+      uint32_t u = 0, gi = 0, n_item = 0;
+      bool ok = true;
+      auto score = [&](int t, uint32_t no, uint32_t slot_u) {  // S_t of tile `no`
+        const int b = T::NBUF == 2 ? (no & 1) : 0;
+        const uint32_t d = tmem + T::S_COL + uint32_t((T::NBUF == 2 ? b : t) * TILE_KEYS);
+        const uint8_t* k = S.ring[slot_u % T::SLOTS];
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const int off = (ks / 4) * T::HALF_BYTES + (ks % 4) * 32;
+          mma_ss(d, sw128_desc(S.q[t] + off), sw128_desc(k + off), ID_S, ks != 0);
+        }
+        mma_commit(&S.s_full[t][b]);
+        mbar_arrive(&S.s_full[t][b]);  // passes on what the loading warp wrote for the tile
+      };
+      auto values = [&](int t, uint32_t no, uint32_t slot_u, bool acc) {  // O_t += P_t V
+        const int b = T::NBUF == 2 ? (no & 1) : 0;
+        const uint32_t p = tmem + T::S_COL + uint32_t((T::NBUF == 2 ? b : t) * TILE_KEYS);
+        const uint32_t d = tmem + T::O_COL + uint32_t(t * D);
+        const uint8_t* v = S.ring[slot_u % T::SLOTS];
+#pragma unroll
+        for (int ks = 0; ks < TILE_KEYS / 16; ++ks)
+          mma_ts(d, p + ks * 8, sw128_mn_desc(v + ks * 2048, T::HALF_BYTES), ID_O, acc || ks != 0);
+        mma_commit(&S.pv_done[t]);
+      };
+      auto slot_full = [&](uint32_t slot_u) {
+        ok = ok && wait(&S.full[slot_u % T::SLOTS], (slot_u / T::SLOTS) & 1, A.error_flags);
+        fence_after();
+      };
+      for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x, ++n_item) {
+        const Item I = item_of<D, NT>(P, S, item);
+        ok = ok && wait(&S.q_full, n_item & 1, A.error_flags);
+        slot_full(u);
+        if (!ok) break;
+        for (int t = 0; t < NT; ++t) score(t, gi, u);
+        mma_commit(&S.empty[u % T::SLOTS]);
+        for (int i = 0; i < I.tiles && ok; ++i, ++gi, u += 2) {
+          const bool more = i + 1 < I.tiles;
+          if constexpr (NT == 1) {
+            if (more) {
+              slot_full(u + 2);
+              if (!ok) break;
+              score(0, gi + 1, u + 2);
+              mma_commit(&S.empty[(u + 2) % T::SLOTS]);
+            }
+          }
+          for (int t = 0; t < NT && ok; ++t) {
+            ok = ok && wait(&S.p_full[t], gi & 1, A.error_flags);
+            if (t == 0) slot_full(u + 1);
+            if (!ok) break;
+            fence_after();
+            values(t, gi, u + 1, i != 0);
+            if (t == NT - 1) mma_commit(&S.empty[(u + 1) % T::SLOTS]);
+            if constexpr (NT > 1) {
+              if (more) {
+                if (t == 0) slot_full(u + 2);
+                if (!ok) break;
+                score(t, gi + 1, u + 2);
+                if (t == NT - 1) mma_commit(&S.empty[(u + 2) % T::SLOTS]);
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int t = warp / 4, row_in = tid % 128;
+    const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
+    const float scale = fabsf(P.scale);
+    const uint32_t flip = P.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes to the query
+    const int slots = P.slots_s + P.slots_o;
+    uint32_t gi = 0;
+    bool ok = true;
+    for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x) {
+      const Item I = item_of<D, NT>(P, S, item);
+      const int row = I.row0 + t * 128 + row_in;
+      const int qi = row / P.per;
+      const long long token = I.begin + qi;
+      const int head = I.head * P.per + row - qi * P.per;
+      {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            static_cast<const bf16*>(A.q) + token * A.q_token_stride + (long long)head * A.q_head_stride);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (row < I.rows) x = src[c];
+          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+          *reinterpret_cast<uint4*>(S.q[t] + (c / 8) * T::HALF_BYTES + row_in * 128 +
+                                    (((c & 7) ^ (row_in & 7)) << 4)) = x;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&S.q_full);
+      }
+      const bool active = I.row0 + t * 128 + 32 * (warp % 4) < I.rows;  // some row of the warp exists
+      float m = -INFINITY, l = 0.0f;  // m: what O and l are scaled by (log2)
+      for (int i = 0; i < I.tiles && ok; ++i, ++gi) {
+        const int b = T::NBUF == 2 ? (gi & 1) : 0;
+        const uint32_t parity = T::NBUF == 2 ? (gi >> 1) & 1 : gi & 1;
+        ok = __all_sync(0xffffffffu, wait(&S.s_full[t][b], parity, A.error_flags));
+        if (!ok) break;
+        fence_after();
+        if (active) {
+          const uint32_t scol = tmem + lanes + T::S_COL + uint32_t((T::NBUF == 2 ? b : t) * TILE_KEYS);
+          uint32_t x[TILE_KEYS];
+#pragma unroll
+          for (int c = 0; c < TILE_KEYS / 32; ++c)
+            tmem_ld32_async(scol + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
+          tmem_wait_ld();
+          const int keys = I.k1 - (I.k0 + i * TILE_KEYS);
+          const uint32_t bad = S.bad[gi & 7];
+          if (keys < TILE_KEYS || bad != 0) {
+#pragma unroll
+            for (int j = 0; j < TILE_KEYS; ++j)
+              if (j >= keys || ((bad >> (j / BOX_MIN)) & 1u)) x[j] = 0xff800000u;  // -inf
+          }
+          float top[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top[k] = __uint_as_float(x[k]);
+#pragma unroll
+          for (int j = 4; j < TILE_KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(x[j]));
+          float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+          if (mx != mx) mx = -INFINITY;  // 0 * inf: the row's NaN comes from its weights
+          const bool grow = mx > m + RESCALE_LOG2 || (m == -INFINITY && mx > m);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? mx : m;
+            const float keep = grow ? exp2_approx(m - mn) : 1.0f;
+            m = mn;
+            l *= keep;
+            if (i > 0) {
+              ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
+              if (!ok) break;
+              fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                const uint32_t col = tmem + lanes + T::O_COL + uint32_t(t * D + c * 32);
+                tmem_ld32(col, o);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                tmem_st32(col, o);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.0f : m;
+          const f2 sc2 = f2_make(scale, scale), nb2 = f2_make(-base, -base);
+          f2 sum[2] = {f2_make(0.0f, 0.0f), f2_make(0.0f, 0.0f)};
+#pragma unroll
+          for (int h = 0; h < TILE_KEYS; h += 64) {
+            uint32_t p[32];
+#pragma unroll
+            for (int j = h; j < h + 64; j += 2) {
+              const float2 y = f2_split(
+                  f2_fma(f2_make(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), sc2, nb2));
+              const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+              sum[(j >> 1) & 1] = f2_add(sum[(j >> 1) & 1], f2_make(w.x, w.y));
+              p[(j - h) / 2] = as_u32(pack2_rn(w));
+            }
+            tmem_st32(scol + h / 2, p);
+          }
+          const float2 a = f2_split(f2_add(sum[0], sum[1]));
+          l += a.x + a.y;
+          tmem_wait_st();
+        }
+        fence_before();
+        mbar_arrive(&S.p_full[t]);
+      }
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
+      if (!ok) break;
+      fence_after();
+      if (active) {
+        const long long slot = (token * A.heads + head) * slots + I.chunk;
+        if (row < I.rows) P.ml[slot] = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tmem + lanes + T::O_COL + uint32_t(t * D + c * 32), o);
+          if (row < I.rows) {
+            float4* dst = reinterpret_cast<float4*>(P.o + slot * D + c * 32);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                   __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+          }
+        }
+      }
+      fence_before();
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 4 * NT) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(T::TMEM_COLS)
+                 : "memory");
+  }
+  pdl_trigger();
+  pdl_wait();  // the stream kernel: see above
+}
+
+// ---------------------------------------------------------------- host side
+// (head_dim, token in page, head, page) over a cache; box: `rows` tokens of one
+// page and head, 64 columns.
+static int cache_map(CUtensorMap* m, const hyena_paged_kv& kv, const void* base, int64_t page_stride,
+                     int64_t token_stride, int64_t head_stride, int rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return fail(HYENA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  // the stride of a dimension of one is never used; give it a valid one
+  cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.kv_heads,
+                        (cuuint64_t)kv.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)token_stride * 2,
+                           (cuuint64_t)(kv.kv_heads > 1 ? head_stride : 8) * 2,
+                           (cuuint64_t)(kv.num_pages > 1 ? page_stride : 8) * 2};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
+                        boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HYENA_ERR_CUDA, "cuTensorMapEncodeTiled(cache) failed");
+  return HYENA_OK;
+}
+
+template <int D, int NT>
+static int launch_tc(const Params& P, cudaStream_t st) {
+  const hyena_paged_kv& kv = P.a.kv;
+  int box = BOX_MIN;
+  while (box < TILE_KEYS && kv.page_size % (2 * box) == 0) box *= 2;
+  CUtensorMap k, v, k16, v16;
+  int rc = cache_map(&k, kv, kv.k, kv.k_page_stride, kv.k_token_stride, kv.k_head_stride, box);
+  if (!rc) rc = cache_map(&v, kv, kv.v, kv.v_page_stride, kv.v_token_stride, kv.v_head_stride, box);
+  if (!rc) rc = cache_map(&k16, kv, kv.k, kv.k_page_stride, kv.k_token_stride, kv.k_head_stride, BOX_MIN);
+  if (!rc) rc = cache_map(&v16, kv, kv.v, kv.v_page_stride, kv.v_token_stride, kv.v_head_stride, BOX_MIN);
+  if (rc) return rc;
+  const size_t smem = sizeof(TcSmem<D, NT>) + 1024;
+  static_assert(sizeof(TcSmem<D, NT>) + 1024 <= 232448, "shared memory of a CTA");
+  if (!smem_attr<shared_kernel<D, NT>>((int)smem))
+    return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(paged_attention shared) failed");
+  const long long row_tiles = (long long)P.a.T * P.per / (NT * 128) + P.groups;
+  const long long ctas = std::min<long long>(num_sms(), row_tiles * kv.kv_heads * P.slots_s);
+  launch_kernel(shared_kernel<D, NT>, dim3((unsigned)ctas), dim3(Tc<D, NT>::THREADS), smem, st, 0u, P,
+                k, v, k16, v16, box);
+  return check_launch("paged_attention shared");
+}
+
+int shared_launch(const Params& P, cudaStream_t st) {
+  const bool two = (long long)P.a.T * P.per > 128ll * P.groups;  // mean rows of a group
+  if (P.a.kv.head_dim == 128) return two ? launch_tc<128, 2>(P, st) : launch_tc<128, 1>(P, st);
+  return two ? launch_tc<64, 2>(P, st) : launch_tc<64, 1>(P, st);
+}
+
+int shared_wait_timeouts(int32_t* count, int reset) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_shared_wait_timeouts, sizeof(int));
+  if (e == cudaSuccess && reset && v != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_shared_wait_timeouts, &zero, sizeof(int));
+  }
+  if (e != cudaSuccess)
+    return fail(HYENA_ERR_CUDA, std::string("attention wait counter: ") + cudaGetErrorString(e));
+  *count = v;
+  return HYENA_OK;
+}
+
+}  // namespace attn
+}  // namespace hb

@@ -48,6 +48,7 @@ extern "C" {
 #define HYENA_FLAG_SEGMENT 2     /* query_start_loc was not non-decreasing / exceeded T */
 #define HYENA_FLAG_STAMP 4       /* a position stamp did not match the request position */
 #define HYENA_FLAG_COLLECTIVE 8  /* a cross-rank wait of a collective kernel expired */
+#define HYENA_FLAG_WAIT 16       /* a shared-memory barrier wait of a kernel expired */
 
 typedef struct hyena_state_view {
   void* data;            /* element (block 0, column 0, channel 0) */
@@ -282,7 +283,8 @@ HYENA_API int hyena_spec_record(const int32_t* out_slots, int64_t s0, int64_t s1
                                 float* stamps, int64_t stamp_stride, int32_t num_blocks,
                                 int32_t* error_flags, void* stream);
 
-/* Every shared-memory barrier wait inside the GEMMs is bounded (4 s); a wait
+/* Every shared-memory barrier wait inside the GEMMs and hyena_paged_attention
+ * (which also sets HYENA_FLAG_WAIT) is bounded (4 s); a wait
  * that expires is counted in a per-device counter and the kernel finishes
  * without its tile being complete, so its output must not be trusted.  This
  * copies the current device's counter into *count (a synchronous read: call it
