@@ -186,10 +186,10 @@ SIGNATURES = {
     "hyena_gemm_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                   C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                   C.c_void_p, C.c_size_t, C.c_void_p]),
-    "hyena_kv_append": (C.c_int, [C.POINTER(KvAppendArgs), C.c_void_p]),
-    "hyena_paged_attention_workspace_size": (C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
-    "hyena_paged_attention": (C.c_int, [C.POINTER(PagedAttentionArgs), C.c_void_p, C.c_size_t,
-                                        C.c_void_p]),
+    # argument structs by byref, or as bytes packed in their layout (ops.py)
+    "hyena_kv_append": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "hyena_paged_attention_workspace_size": (C.c_size_t, [C.c_void_p]),
+    "hyena_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "hyena_gemm_gated_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                         C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
                                         C.c_int32, C.c_int32, C.c_void_p]),

@@ -10,34 +10,46 @@
 //   M = max m_i,  o = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i   (m in log2).
 //
 // Work.  A segment is either the shared keys of a group, seen by every query of
-// its requests, or the own keys of one request.  Segment x 16-row tile (rows =
-// queries x heads of one key/value head) x key/value head x chunk of keys is an
-// item; persistent CTAs walk the items.  Every length is read on the device
-// (one captured graph serves growing contexts), so each CTA first derives the
-// same plan from them: the chunk lengths, a prefix sum of the segments' items.
+// its requests, or the own keys of one request; a unit is a segment x key/value
+// head x 16-row tile (rows = queries x heads of one key/value head), and an item
+// is `chunk` 16-key tiles of a unit.  Warps take items in turn, those of a
+// segment ordered by position, then head: the warps of the GPU sweep through the
+// cache together, a page's heads at about the same time.  (Giving each warp one
+// long run of tiles instead evens the work out exactly, but spreads the warps
+// over the whole cache: 343 us instead of 3XX for 32 requests of up to 8000
+// keys, the memory's pages and translations being hit at random.)  A warp's
+// loads run on across its items.  Every length is read on the device (one
+// captured graph serves growing contexts), so each CTA first derives the same
+// list from them, a prefix sum over segments.
 //
 // `shared_lens` says what may be read once, never what is seen: a group's
 // shared run is cut to what every query of the group sees and to whole 16-key
-// tiles, and the rest of it counts as own keys.
+// tiles, and the rest of it counts as own keys.  Runs of more than 16 rows a
+// key/value head go to attention_shared.cu.
 #include <algorithm>
+#include <cmath>
 
 #include "attention.cuh"
 
 namespace hb {
 namespace attn {
 
+using namespace tc;
+
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int ROWS = 16;        // rows of an item
+constexpr int ROWS = 16;        // rows of a unit
 constexpr int STAGES = 3;       // tiles in flight per warp
-constexpr int MIN_CHUNK = 128;  // keys
+constexpr int MIN_TILES = 4;    // tiles of an item, and how many items a warp should get
+constexpr int ITEMS_PER_WARP = 8;
 constexpr int MAX_SEGMENTS = 2048;
-constexpr int ITEMS_PER_CTA = 8;
 constexpr int TC_MIN_ROWS = 16;  // mean rows of a group and key/value head
 
 struct Plan {
-  int chunk_s, chunk_o, items;
+  int chunk;   // tiles of an item
+  int items;
   int* first;  // [groups + requests + 1] first item of a segment
+  int4* info;  // [groups + requests]: first query, queries, keys, {leader | first own key}
   int* shared; // [groups] the shared run
   int* leader; // [groups] the request whose pages stand for it
 };
@@ -45,78 +57,65 @@ struct Plan {
 __device__ __forceinline__ int row_tiles(const Params& P, int nq) {
   return (int)(((long long)nq * P.per + ROWS - 1) / ROWS);
 }
-
-// Chunk of a kind of segment: the work spread over ITEMS_PER_CTA items a CTA,
-// at most `slots` chunks a segment, whole rounds of the four warps.
-__device__ __forceinline__ int chunk_keys(long long work, int longest, int slots, int ctas) {
-  long long c = (work + (long long)ctas * ITEMS_PER_CTA - 1) / ((long long)ctas * ITEMS_PER_CTA);
-  const int floor_slots = ceil_div(longest, slots > 0 ? slots : 1);
-  if (c < floor_slots) c = floor_slots;
-  if (c < MIN_CHUNK) c = MIN_CHUNK;
-  c = (c + WARPS * KT - 1) / (WARPS * KT) * (WARPS * KT);
-  return (int)(c < (1ll << 30) ? c : (1ll << 30));
+// Tiles of a unit of an own segment.  A request with queries has a tile even
+// without keys: its rows are written there.
+__device__ __forceinline__ int own_tiles(int len, int k_begin) {
+  return max(ceil_div(max(len - k_begin, 0), KT), 1);
 }
 
-// Every thread of the CTA; red: 4 x 4 long longs of scratch.
-__device__ void make_plan(const Params& P, Plan& L, long long* red) {
+// Every thread of the CTA.
+__device__ void make_plan(const Params& P, Plan& L) {
+  __shared__ long long wsum[WARPS];
+  __shared__ int wlong[WARPS], wfirst[WARPS];
   const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int B = P.a.num_requests, G = P.groups, hkv = P.a.kv.kv_heads;
+  const int G = P.groups, n = G + P.a.num_requests;
   shared_runs<THREADS>(P, L.shared, L.leader);
-  long long v[4] = {0, 0, 0, 0};  // work and longest, shared and own
-  for (int s = tid; s < G + B; s += THREADS) {
+  // a thread takes a run of consecutive segments
+  const int per = ceil_div(n, THREADS);
+  const int s0 = min(tid * per, n), s1 = min(s0 + per, n);
+  auto tiles_of = [&](int s, const int4& x) { return s < G ? x.z / KT : own_tiles(x.z, x.w); };
+  long long work = 0;
+  int longest = 0;
+  for (int s = s0; s < s1; ++s) {
+    int4 x;
     if (s < G) {
-      int begin;
-      const long long w = (long long)L.shared[s] * row_tiles(P, group_queries(P, s, begin)) * hkv;
-      v[0] += w;
-      if (w > 0 && L.shared[s] > v[1]) v[1] = L.shared[s];
+      x.y = P.tc ? 0 : group_queries(P, s, x.x);
+      x.z = L.shared[s];
+      x.w = L.leader[s];
     } else {
-      int begin;
-      const int n = queries(P, s - G, begin), g = group_of(P, s - G);
-      int own = length(P, s - G) - (g >= 0 ? L.shared[g] : 0);
-      own = own > 0 && n > 0 ? own : 0;
-      v[2] += (long long)own * row_tiles(P, n) * hkv;
-      if (own > v[3]) v[3] = own;
+      const int r = s - G, g = group_of(P, r);
+      x.y = queries(P, r, x.x);
+      x.z = length(P, r);
+      x.w = g >= 0 && x.z > 0 ? L.shared[g] : 0;
     }
+    L.info[s] = x;
+    const int units = row_tiles(P, x.y) * P.a.kv.kv_heads, tiles = tiles_of(s, x);
+    work += (long long)tiles * units;
+    if (units > 0) longest = max(longest, tiles);
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const long long x = __shfl_xor_sync(0xffffffffu, v[k], d);
-      v[k] = (k & 1) ? (x > v[k] ? x : v[k]) : v[k] + x;
-    }
-  }
+  for (int d = 16; d > 0; d >>= 1) work += __shfl_xor_sync(0xffffffffu, work, d);
+  longest = __reduce_max_sync(0xffffffffu, longest);
   if (lane == 0) {
-    for (int k = 0; k < 4; ++k) red[warp * 4 + k] = v[k];
+    wsum[warp] = work;
+    wlong[warp] = longest;
   }
   __syncthreads();
-  for (int k = 0; k < 4; ++k) {
-    v[k] = 0;
-    for (int w = 0; w < WARPS; ++w) {
-      const long long x = red[w * 4 + k];
-      v[k] = (k & 1) ? (x > v[k] ? x : v[k]) : v[k] + x;
-    }
+  work = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    work += wsum[w];
+    longest = max(longest, wlong[w]);
   }
-  L.chunk_s = chunk_keys(v[0], (int)v[1], P.slots_s, (int)gridDim.x);
-  L.chunk_o = chunk_keys(v[2], (int)v[3], P.slots_o, (int)gridDim.x);
-  // Items of the segments, then their exclusive prefix sum: a thread sums a run
-  // of consecutive segments, the threads' sums are scanned.
-  const int per = ceil_div(G + B, THREADS);
-  const int s0 = tid * per, s1 = s0 + per < G + B ? s0 + per : G + B;
+  // at most P.slots items a unit
+  const long long want = (long long)gridDim.x * (WARPS * ITEMS_PER_WARP);
+  const long long even = (work + want - 1) / want;
+  L.chunk = (int)max(max(even, (long long)ceil_div(longest, P.slots)), (long long)MIN_TILES);
   int sum = 0;
   for (int s = s0; s < s1; ++s) {
-    int items;
-    if (s < G) {
-      int begin;
-      items = P.tc ? 0 : ceil_div(L.shared[s], L.chunk_s) * row_tiles(P, group_queries(P, s, begin)) * hkv;
-    } else {
-      int begin;
-      const int n = queries(P, s - G, begin), g = group_of(P, s - G);
-      const int own = length(P, s - G) - (g >= 0 ? L.shared[g] : 0);
-      items = (own > 0 ? ceil_div(own, L.chunk_o) : 1) * row_tiles(P, n) * hkv;
-    }
-    L.first[s] = items;
-    sum += items;
+    const int4 x = L.info[s];
+    L.first[s] = sum;
+    sum += ceil_div(tiles_of(s, x), L.chunk) * row_tiles(P, x.y) * P.a.kv.kv_heads;
   }
   int scan = sum;
 #pragma unroll
@@ -124,35 +123,21 @@ __device__ void make_plan(const Params& P, Plan& L, long long* red) {
     const int x = __shfl_up_sync(0xffffffffu, scan, d);
     if (lane >= d) scan += x;
   }
-  __syncthreads();
-  int* wsum = reinterpret_cast<int*>(red);
-  if (lane == 31) wsum[warp] = scan;
+  if (lane == 31) wfirst[warp] = scan;
   __syncthreads();
   int at = scan - sum, total = 0;
+#pragma unroll
   for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) at += wsum[w];
-    total += wsum[w];
+    if (w < warp) at += wfirst[w];
+    total += wfirst[w];
   }
-  for (int s = s0; s < s1; ++s) {
-    const int items = L.first[s];
-    L.first[s] = at;
-    at += items;
-  }
-  if (tid == 0) L.first[G + B] = total;
+  for (int s = s0; s < s1; ++s) L.first[s] += at;
+  if (tid == 0) L.first[n] = total;
   L.items = total;
   __syncthreads();
 }
 
 // ---------------------------------------------------------------- fragments
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-// 16 bytes global -> shared, zeros instead where !valid.
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(valid ? 16 : 0)
-               : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -173,342 +158,377 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Byte offset of 16-byte chunk c of row `row` in a tile of D-element rows, the
-// chunks permuted within groups of eight so that eight rows' same chunk (an
-// ldmatrix phase) lies in distinct banks.
-template <int D>
-__device__ __forceinline__ uint32_t tile_at(int row, int c) {
-  if constexpr (D == 128) return uint32_t(row * 256 + ((c ^ (row & 7)) << 4));
-  return uint32_t(row * 128 + ((c ^ (row & 7)) << 4));
-}
-
 template <int D>
 struct Layout {
-  static constexpr int TILE = KT * D * 2;          // bytes of one operand's tile
-  static constexpr int STAGE = 2 * TILE;           // keys, then values
-  static constexpr int RING = STAGES * STAGE;      // a warp's ring
-  static constexpr int PITCH = D + 4;              // floats of a parked row of O
-  static_assert(RING >= ROWS * PITCH * 4, "the ring holds a warp's parked O");
-  static constexpr int PLAN = WARPS * RING;        // ints of the plan follow
+  static constexpr int HALVES = D / 64;         // 64-column swizzled halves of a row
+  static constexpr int HALF = KT * 128;         // bytes of a half's tile
+  static constexpr int TILE = HALVES * HALF;    // one operand's tile
+  static constexpr int STAGE = 2 * TILE;        // keys, then values
+  static constexpr int RING = STAGES * STAGE;   // a warp's ring
+  static constexpr int PLAN = WARPS * RING;     // the plan follows
 };
+// Byte offset of 16-byte chunk c of row `row` in a tile as TMA leaves it
+// (SWIZZLE_128B halves): eight rows' same chunk, an ldmatrix phase, lies in
+// distinct banks.
+__device__ __forceinline__ uint32_t tile_at(int row, int c) {
+  return uint32_t((c >> 3) * (KT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+}
 
-// One CTA walks its items; within an item warp w owns tiles w, w + 4, ... of the
-// chunk, with its own ring, maximum, sum and O, and no barrier until the four
-// warps' pieces are joined through shared memory.  The 16 rows of a tensor-core
-// tile are mostly padding for one token and ungrouped heads; the item is bound
-// by its keys' bytes all the same (128 mma for 32 KB of keys and values).
-template <int D>
-__global__ void __launch_bounds__(THREADS, 2) stream_kernel(const __grid_constant__ Params P) {
-  using LT = Layout<D>;
-  constexpr int CPR = D / 8;  // 16-byte chunks of a row
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long red[WARPS * 4];
-  __shared__ float2 ml_s[WARPS][ROWS];
-  pdl_entry();
-  const hyena_paged_attention_args& A = P.a;
-  const hyena_paged_kv& kv = A.kv;
-  const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int G = P.groups, B = A.num_requests, hkv = kv.kv_heads;
-  Plan L;
-  L.first = reinterpret_cast<int*>(smem + LT::PLAN);
-  L.shared = L.first + (G + B + 1);
-  L.leader = L.shared + G;
-  make_plan(P, L, red);
-  if (blockIdx.x == 0 && P.plan != nullptr) {
-    if (tid == 0) {
-      if (!P.tc) P.plan[0] = L.chunk_s;
-      P.plan[1] = L.chunk_o;
-    }
-    for (int g = tid; g < G; g += THREADS) P.plan[2 + g] = L.shared[g];
-  }
-  const int slots = P.slots_s + P.slots_o;
-  uint8_t* ring = smem + warp * LT::RING;
-  const uint32_t ring_u = smem_u32(ring);
-  const int g8 = lane >> 2, t4 = lane & 3;
+__device__ __forceinline__ uint32_t query_word(const bf16* p, uint2 sign) {
+  return (*reinterpret_cast<const uint32_t*>(p) ^ sign.x) & sign.y;
+}
 
-  for (int item = (int)blockIdx.x; item < L.items; item += (int)gridDim.x) {
-    // ---- which keys and rows
-    int lo = 0, hi = G + B;
+// An item as a warp meets it (all warp-uniform).
+struct Item {
+  int seg, index;    // its segment; which chunk of its unit it is
+  int n;             // its tiles
+  int request, head, begin, rows, row0, nq, len;
+  int k0, k1;        // its keys [k0, k1): those some row sees
+  int all_see;       // keys below it are seen by every row
+  bool only;         // the only piece of its rows
+};
+__device__ __forceinline__ Item item_at(const Params& P, const Plan& L, int item, int seg) {
+  Item I;
+  const int G = P.groups;
+  if (seg < 0 || item >= L.first[seg + 1]) {
+    int lo = seg < 0 ? 0 : seg + 1, hi = G + P.a.num_requests;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (L.first[mid] <= item) lo = mid; else hi = mid;
     }
-    const int seg = lo;
-    const bool own_seg = seg >= G;
-    int request, begin, rows, nq = 0, len = 0, k_begin, k_end, chunk, chunks;
-    if (own_seg) {
-      request = seg - G;
-      nq = queries(P, request, begin);
-      len = length(P, request);
-      rows = nq * P.per;
-      const int g = group_of(P, request);
-      k_begin = g >= 0 ? L.shared[g] : 0;
-      k_end = len > k_begin ? len : k_begin;
-      if (len == 0) k_begin = k_end = 0;
-      chunk = L.chunk_o;
-    } else {
-      request = L.leader[seg];
-      rows = group_queries(P, seg, begin) * P.per;
-      k_begin = 0;
-      k_end = L.shared[seg];
-      chunk = L.chunk_s;
-    }
-    chunks = k_end > k_begin ? ceil_div(k_end - k_begin, chunk) : 1;
-    const int tiles_r = ceil_div(rows, ROWS);
-    int rem = item - L.first[seg];
-    const int rt = rem % tiles_r;
-    rem /= tiles_r;
-    const int h = rem % hkv, c = rem / hkv;
-    const int row0 = rt * ROWS;
-    int k0 = k_begin + c * chunk;
-    int k1 = k_end - k0 > chunk ? k0 + chunk : k_end;
-    int all_see = k1;  // keys below it are seen by every row of the tile
-    if (own_seg) {
-      const int last = min(nq - 1, (row0 + ROWS - 1) / P.per);
-      k1 = min(k1, len - nq + last + 1);
-      all_see = min(k1, len - nq + row0 / P.per + 1);
-    }
-    const int tiles = k1 > k0 ? ceil_div(k1 - k0, KT) : 0;
+    seg = lo;
+  }
+  I.seg = seg;
+  const int4 x = L.info[seg];
+  const bool own = seg >= G;
+  I.begin = x.x;
+  I.nq = x.y;
+  I.len = x.z;
+  I.rows = x.y * P.per;
+  I.request = own ? seg - G : x.w;
+  const int first_key = own ? x.w : 0, tiles = own ? own_tiles(x.z, x.w) : x.z / KT;
+  const int tiles_r = ceil_div(I.rows, ROWS), units = tiles_r * P.a.kv.kv_heads;
+  const int rem = item - L.first[seg];
+  I.index = rem / units;
+  const int v = rem - I.index * units;
+  I.head = v / tiles_r;
+  I.row0 = (v - I.head * tiles_r) * ROWS;
+  I.n = min(L.chunk, tiles - I.index * L.chunk);
+  I.only = own && x.w == 0 && tiles <= L.chunk;
+  I.k0 = first_key + I.index * L.chunk * KT;
+  I.k1 = I.all_see = min(x.z, I.k0 + I.n * KT);
+  if (own) {
+    const int last = min(I.nq - 1, (I.row0 + ROWS - 1) / P.per);
+    I.k1 = min(I.k1, I.len - I.nq + last + 1);
+    I.all_see = min(I.k1, I.len - I.nq + I.row0 / P.per + 1);
+  }
+  return I;
+}
 
+// A warp walks its tiles with its own ring, maximum, sum and O; no barrier after
+// the plan.  The 16 rows of a tensor-core tile are mostly padding for one token
+// and ungrouped heads (rows 8-15 are skipped in the softmax where a unit has
+// none); the kernel is bound by the keys' bytes as long as the some 130
+// instructions of an 8 KB tile stay well under the 2850 cycles that an SM's share
+// of HBM gives each of its eight warps for it.  Hence TMA (four instructions a
+// tile), masks only in the tiles that need them, and a maximum that is compared
+// by one vote: m moves, and O is rescaled, only when a score exceeds it by 2^8
+// (the weights stay below 2^8, where bf16 and fp32 round as well as at 1).
+template <int D>
+__global__ void __launch_bounds__(THREADS, 2)
+stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensorMap map_k,
+              const __grid_constant__ CUtensorMap map_v) {
+  using LT = Layout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_s[WARPS][STAGES];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  const hyena_paged_attention_args& A = P.a;
+  const hyena_paged_kv& kv = A.kv;
+  const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = P.groups, B = A.num_requests;
+  uint64_t* full = full_s[warp];
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_entry();
+  Plan L;
+  L.info = reinterpret_cast<int4*>(smem + LT::PLAN);
+  L.first = reinterpret_cast<int*>(L.info + (G + B));
+  L.shared = reinterpret_cast<int*>(L.first + (G + B + 1));
+  L.leader = L.shared + G;
+  make_plan(P, L);
+  if (blockIdx.x == 0) {  // for the join
+    if (tid == 0) {
+      if (!P.tc) P.plan[0] = L.chunk * KT;
+      P.plan[1] = L.chunk;
+    }
+    for (int g = tid; g < G; g += THREADS) P.plan[2 + g] = L.shared[g];
+  }
+  uint8_t* ring = smem + warp * LT::RING;
+  const uint32_t ring_u = su32(ring);
+  const int g8 = lane >> 2, t4 = lane & 3;
+  const int warps = (int)gridDim.x * WARPS, first = warp * (int)gridDim.x + (int)blockIdx.x;
+  if (first >= L.items) return;
+
+  // ---- loads, STAGES - 1 tiles ahead; a lane holds the page of one of 32
+  // consecutive page-table entries
+  int next = first;                       // the item being loaded
+  Item N = item_at(P, L, next, -1);
+  int tile = 0, page_at = 0, page_index = 0, window = -64, window_of = -1, pages = 0;
+  uint32_t bad = 0;  // stages whose page is out of range
+  int load_stage = 0;
+  page_index = N.k0 / kv.page_size;
+  page_at = N.k0 - page_index * kv.page_size;
+  auto load = [&]() {
+    if (next >= L.items) return;
+    const int s = load_stage;
+    load_stage = s + 1 == STAGES ? 0 : s + 1;
+    if (N.k0 + tile * KT < N.k1) {
+      if (window_of != N.request || page_index < window || page_index >= window + 32) {
+        window = page_index;
+        window_of = N.request;
+        pages = __ldg(kv.page_table + (long long)N.request * kv.page_table_stride +
+                      min(page_index + lane, kv.pages_per_request - 1));
+      }
+      const int page = __shfl_sync(0xffffffffu, pages, page_index - window);
+      const bool ok = page >= 0 && page < kv.num_pages;
+      bad = ok ? bad & ~(1u << s) : bad | (1u << s);
+      if (lane == 0) {
+        if (ok) {
+          uint8_t* dst = ring + s * LT::STAGE;
+          mbar_expect_tx(&full[s], LT::STAGE);
+#pragma unroll
+          for (int h = 0; h < LT::HALVES; ++h) {
+            tma_load_4d(&map_k, &full[s], dst + h * LT::HALF, h * 64, page_at, N.head, page);
+            tma_load_4d(&map_v, &full[s], dst + LT::TILE + h * LT::HALF, h * 64, page_at, N.head, page);
+          }
+        } else {
+          flag_error(A.error_flags, HYENA_FLAG_BLOCK_RANGE);
+          mbar_arrive(&full[s]);
+        }
+      }
+      page_at += KT;
+      if (page_at == kv.page_size) {
+        page_at = 0;
+        ++page_index;
+      }
+    } else if (lane == 0) {
+      mbar_arrive(&full[s]);  // nothing to load: the phase completes by itself
+    }
+    if (++tile == N.n) {
+      tile = 0;
+      next += warps;
+      if (next < L.items) {
+        N = item_at(P, L, next, N.seg);
+        page_index = N.k0 / kv.page_size;
+        page_at = N.k0 - page_index * kv.page_size;
+      }
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; ++i) load();
+
+  const float scale = P.scale == 0.0f ? 1.0f : fabsf(P.scale);
+  const uint2 sign = query_sign(P.scale);
+  uint32_t qf[D / 16][4];
+  float o[D / 8][4], m[2], l[2];
+  int s = 0, seg = -1;
+  uint32_t parity = 0;
+#pragma unroll 1
+  for (int item = first; item < L.items; item += warps) {
+    const Item U = item_at(P, L, item, seg);
+    seg = U.seg;
+    const bool two = U.rows - U.row0 > 8;  // rows 8-15 exist
     // ---- this lane's two rows (g8, g8 + 8) as mma A fragments
-    uint32_t qf[D / 16][4];
-    int limit[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = row0 + g8 + 8 * i;
-      limit[i] = 0;
+      const int row = U.row0 + g8 + 8 * i;
       const bf16* src = nullptr;
-      if (row < rows) {
+      if (row < U.rows) {
         const int qi = row / P.per;
-        limit[i] = own_seg ? len - nq + qi + 1 : 0x7fffffff;
-        src = static_cast<const bf16*>(A.q) + (long long)(begin + qi) * A.q_token_stride +
-              (long long)(h * P.per + row - qi * P.per) * A.q_head_stride;
+        src = static_cast<const bf16*>(A.q) + (long long)(U.begin + qi) * A.q_token_stride +
+              (long long)(U.head * P.per + row - qi * P.per) * A.q_head_stride;
       }
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        qf[ks][i] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + t4 * 2) : 0u;
-        qf[ks][2 + i] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + t4 * 2) : 0u;
+        qf[ks][i] =
+            src != nullptr ? query_word(src + ks * 16 + t4 * 2, sign) : 0u;
+        qf[ks][2 + i] =
+            src != nullptr ? query_word(src + ks * 16 + 8 + t4 * 2, sign) : 0u;
       }
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
     }
-
-    // ---- loads
-    const int32_t* table = kv.page_table + (long long)request * kv.page_table_stride;
-    const int mine = tiles > warp ? (tiles - warp + WARPS - 1) / WARPS : 0;
-    auto page_for = [&](int i) {  // page of this warp's tile i
-      return i < mine ? __ldg(table + (k0 + (warp + i * WARPS) * KT) / kv.page_size) : 0;
-    };
-    uint32_t bad = 0;  // stages whose page is out of range
-    auto load = [&](int i, int page) {
-      if (i < mine) {
-        const int kpos = k0 + (warp + i * WARPS) * KT, s = i % STAGES;
-        const bool ok = page >= 0 && page < kv.num_pages;
-        bad = ok ? bad & ~(1u << s) : bad | (1u << s);
-        if (!ok) {
-          if (lane == 0) flag_error(A.error_flags, HYENA_FLAG_BLOCK_RANGE);
-          page = 0;
-        }
-        const int at = kpos % kv.page_size;
-        const int ch = lane % CPR, r0 = lane / CPR;
-        const bf16* ks = static_cast<const bf16*>(kv.k) + page * kv.k_page_stride +
-                         (at + r0) * kv.k_token_stride + h * kv.k_head_stride + ch * 8;
-        const bf16* vs = static_cast<const bf16*>(kv.v) + page * kv.v_page_stride +
-                         (at + r0) * kv.v_token_stride + h * kv.v_head_stride + ch * 8;
-        const uint32_t dst = ring_u + uint32_t(s * LT::STAGE);
-        const int nvalid = ok ? k1 - kpos : 0;  // rows behind the last key are zeros
-#pragma unroll
-        for (int r = 0; r < KT; r += 32 / CPR) {
-          const uint32_t d = dst + tile_at<D>(r0 + r, ch);
-          cp_async16_or_zero(d, ks + r * kv.k_token_stride, r0 + r < nvalid);
-          cp_async16_or_zero(d + LT::TILE, vs + r * kv.v_token_stride, r0 + r < nvalid);
-        }
-      }
-      cp_async_commit();
-    };
-    int page_next = page_for(0);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      const int page = page_next;
-      page_next = page_for(i + 1);
-      load(i, page);
-    }
-
-    float o[D / 8][4];
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-    for (int i = 0; i < mine; ++i) {
-      {
-        const int page = page_next;
-        page_next = page_for(i + STAGES);
-        load(i + STAGES - 1, page);
+#pragma unroll 1
+    for (int i_tile = 0; i_tile < U.n; ++i_tile) {
+    load();
+    const int kpos = U.k0 + i_tile * KT;
+    if (!__all_sync(0xffffffffu, wait(&full[s], parity, A.error_flags))) {
+      // gave up: what else was issued lands (waits bounded too) before the warp leaves
+      for (int k = 1; k < STAGES; ++k) {
+        if (++s == STAGES) {
+          s = 0;
+          parity ^= 1u;
+        }
+        if (s != load_stage) wait(&full[s], parity, A.error_flags);
       }
-      cp_async_wait<STAGES - 1>();
-      __syncwarp();
-      const int s = i % STAGES;
-      const int kpos = k0 + (warp + i * WARPS) * KT;
+      return;
+    }
+    if (kpos < U.k1 && !((bad >> s) & 1u)) {
       const uint32_t ks_u = ring_u + uint32_t(s * LT::STAGE), vs_u = ks_u + LT::TILE;
-      const bool is_bad = (bad >> s) & 1u;
-
       // scores of 16 rows x 16 keys
       float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         uint32_t b[4];  // keys 0-7 (k 0-7, 8-15), keys 8-15 (k 0-7, 8-15)
-        ldsm4(ks_u + tile_at<D>((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), b);
+        ldsm4(ks_u + tile_at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), b);
         mma_bf16(sc[0], qf[ks], b[0], b[1]);
         mma_bf16(sc[1], qf[ks], b[2], b[3]);
       }
-      float p[2][4];
+      const bool partial = kpos + KT > U.all_see;  // some row does not see some key of the tile
+      if (partial) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int end = is_bad ? 0 : min(limit[r], k1) - kpos;  // keys of the tile this row sees
-        float x[4];
+        for (int i = 0; i < 2; ++i) {
+          const int row = U.row0 + g8 + 8 * i;
+          int end = U.k1 - kpos;  // keys of the tile this row sees
+          if (U.seg >= G && row < U.rows) end = min(end, U.len - U.nq + row / P.per + 1 - kpos);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
-          x[e] = key < end ? sc[e >> 1][r * 2 + (e & 1)] * P.scale : -INFINITY;
-        }
-        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(m[r], top);
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float keep = exp2_approx(m[r] - base);
-        m[r] = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float w = exp2_approx(x[e] - base);
-          sum += w;
-          p[e >> 1][r * 2 + (e & 1)] = w;
-        }
-        l[r] = l[r] * keep + sum;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[n][r * 2] *= keep;
-          o[n][r * 2 + 1] *= keep;
+          for (int e = 0; e < 4; ++e) {
+            const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
+            if (key >= end) sc[e >> 1][i * 2 + (e & 1)] = -INFINITY;
+          }
         }
       }
-      // Keys that some row of the tile does not see (a later token of the same
-      // step): added row by row, so that a masked value, whatever it holds,
-      // meets no product; the mma below gets zeros for them.
-      if (all_see < kpos + KT && all_see < k1) {
-        const int j0 = max(all_see - kpos, 0), j1 = min(k1 - kpos, KT);
-        for (int j = j0; j < j1; ++j) {
-          const int src = (lane & ~3) | ((j & 7) >> 1);
-          const float w00 = __shfl_sync(0xffffffffu, p[0][0], src), w01 = __shfl_sync(0xffffffffu, p[0][1], src);
-          const float w02 = __shfl_sync(0xffffffffu, p[0][2], src), w03 = __shfl_sync(0xffffffffu, p[0][3], src);
-          const float w10 = __shfl_sync(0xffffffffu, p[1][0], src), w11 = __shfl_sync(0xffffffffu, p[1][1], src);
-          const float w12 = __shfl_sync(0xffffffffu, p[1][2], src), w13 = __shfl_sync(0xffffffffu, p[1][3], src);
-          const bool upper = j >= 8, odd = j & 1;
-          const float wa = upper ? (odd ? w11 : w10) : (odd ? w01 : w00);
-          const float wb = upper ? (odd ? w13 : w12) : (odd ? w03 : w02);
-          const bool sa = !is_bad && kpos + j < limit[0], sb = !is_bad && kpos + j < limit[1];
+      float top[2];
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            const float2 v = unpack2(*reinterpret_cast<const bf162*>(
-                ring + s * LT::STAGE + LT::TILE + tile_at<D>(j, n) + t4 * 4));
-            if (sa) {
-              o[n][0] = fmaf(wa, v.x, o[n][0]);
-              o[n][1] = fmaf(wa, v.y, o[n][1]);
-            }
-            if (sb) {
-              o[n][2] = fmaf(wb, v.x, o[n][2]);
-              o[n][3] = fmaf(wb, v.y, o[n][3]);
+      for (int i = 0; i < 2; ++i)
+        top[i] = fmaxf(fmaxf(sc[0][i * 2], sc[0][i * 2 + 1]), fmaxf(sc[1][i * 2], sc[1][i * 2 + 1])) * scale;
+      bool grow = top[0] > m[0] + RESCALE_LOG2;
+      if (two) grow = grow || top[1] > m[1] + RESCALE_LOG2;
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = top[i] == top[i] ? top[i] : -INFINITY;
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          if (x > m[i] + RESCALE_LOG2) {  // by the row alone
+            const float keep = exp2_approx(m[i] - x);
+            m[i] = x;
+            l[i] *= keep;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+              o[n][i * 2] *= keep;
+              o[n][i * 2 + 1] *= keep;
             }
           }
-          __syncwarp();
-          if (lane < CPR)
-            *reinterpret_cast<uint4*>(ring + s * LT::STAGE + LT::TILE + tile_at<D>(j, lane)) =
-                make_uint4(0u, 0u, 0u, 0u);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
-          if (key >= j0) p[e >> 1][e & 1] = p[e >> 1][2 + (e & 1)] = 0.0f;
         }
       }
       // The weights are rounded to bf16 for the product, as the values are; l
       // sums them before that rounding, which is unbiased.
-      uint32_t pa[4];
-      pa[0] = as_u32(pack2_rn(make_float2(p[0][0], p[0][1])));
-      pa[1] = as_u32(pack2_rn(make_float2(p[0][2], p[0][3])));
-      pa[2] = as_u32(pack2_rn(make_float2(p[1][0], p[1][1])));
-      pa[3] = as_u32(pack2_rn(make_float2(p[1][2], p[1][3])));
+      float p[2][4];
+      uint32_t pa[4] = {0u, 0u, 0u, 0u};
+      auto weights = [&](int i) {
+        const float base = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          p[e >> 1][i * 2 + (e & 1)] = exp2_approx(fmaf(sc[e >> 1][i * 2 + (e & 1)], scale, -base));
+        l[i] += (p[0][i * 2] + p[0][i * 2 + 1]) + (p[1][i * 2] + p[1][i * 2 + 1]);
+        pa[i] = as_u32(pack2_rn(make_float2(p[0][i * 2], p[0][i * 2 + 1])));
+        pa[2 + i] = as_u32(pack2_rn(make_float2(p[1][i * 2], p[1][i * 2 + 1])));
+      };
+      weights(0);
+      if (two) weights(1);
+      if (partial) {
+        // Keys that some row of the tile does not see (a later token of the same
+        // step, or beyond the last): those that another row sees are added row by
+        // row, so that a masked value, whatever it holds, meets no product; then
+        // zeros take their place for the mma.
+        const int j0 = max(U.all_see - kpos, 0), j1 = min(U.k1 - kpos, KT);
+        uint8_t* vt = ring + s * LT::STAGE + LT::TILE;
+        for (int j = j0; j < j1; ++j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (i == 1 && !two) continue;
+            const uint32_t pw0 = __shfl_sync(0xffffffffu, __float_as_uint(j < 8 ? p[0][i * 2] : p[1][i * 2]),
+                                             (lane & ~3) | ((j & 7) >> 1));
+            const uint32_t pw1 = __shfl_sync(
+                0xffffffffu, __float_as_uint(j < 8 ? p[0][i * 2 + 1] : p[1][i * 2 + 1]),
+                (lane & ~3) | ((j & 7) >> 1));
+            const float w = __uint_as_float(j & 1 ? pw1 : pw0);
+            const int row = U.row0 + g8 + 8 * i;
+            if (row < U.rows && kpos + j < U.len - U.nq + row / P.per + 1) {
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) {
+                const float2 v = unpack2(*reinterpret_cast<const bf162*>(vt + tile_at(j, n) + t4 * 4));
+                o[n][i * 2] = fmaf(w, v.x, o[n][i * 2]);
+                o[n][i * 2 + 1] = fmaf(w, v.y, o[n][i * 2 + 1]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        for (int c = lane; c < (KT - j0) * (D / 8); c += 32)
+          *reinterpret_cast<uint4*>(vt + tile_at(j0 + c / (D / 8), c % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA fills the stage again
+        __syncwarp();
+        const int key = t4 * 2;
+        const uint32_t lo0 = key < j0 ? 0xFFFFu : 0u, hi0 = key + 1 < j0 ? 0xFFFF0000u : 0u;
+        const uint32_t lo1 = key + 8 < j0 ? 0xFFFFu : 0u, hi1 = key + 9 < j0 ? 0xFFFF0000u : 0u;
+        pa[0] &= lo0 | hi0;
+        pa[1] &= lo0 | hi0;
+        pa[2] &= lo1 | hi1;
+        pa[3] &= lo1 | hi1;
+      }
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
         uint32_t b[4];  // values of keys 0-7 and 8-15, columns 16n + 0-7 then 16n + 8-15
-        ldsm4_trans(vs_u + tile_at<D>(lane & 15, n * 2 + (lane >> 4)), b);
+        ldsm4_trans(vs_u + tile_at(lane & 15, n * 2 + (lane >> 4)), b);
         mma_bf16(o[2 * n], pa, b[0], b[1]);
         mma_bf16(o[2 * n + 1], pa, b[2], b[3]);
       }
-      __syncwarp();  // the stage is read before it is filled again
     }
-    cp_async_wait<0>();
+    __syncwarp();  // the stage is read before it is filled again
+    if (++s == STAGES) {
+      s = 0;
+      parity ^= 1u;
+    }
 
-    // ---- join the warps' pieces
-    float* parked = reinterpret_cast<float*>(ring);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t4 == 0) ml_s[warp][g8 + 8 * r] = make_float2(m[r], l[r]);
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(parked + (g8 + 8 * r) * LT::PITCH + n * 8 + t4 * 2) =
-            make_float2(o[n][r * 2], o[n][r * 2 + 1]);
     }
-    __syncthreads();
+    // ---- the piece is complete
     {
-      const int row = tid / 8, col = (tid % 8) * (D / 8);
-      if (row0 + row < rows) {
-        float mx = -INFINITY, lsum = 0.0f, w[WARPS];
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) mx = fmaxf(mx, ml_s[k][row].x);
-        const float base = mx == -INFINITY ? 0.0f : mx;
-#pragma unroll
-        for (int k = 0; k < WARPS; ++k) {
-          w[k] = exp2_approx(ml_s[k][row].x - base);
-          lsum += w[k] * ml_s[k][row].y;
-        }
-        float acc[D / 8];
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j) acc[j] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < WARPS; ++k) {
-          const float* src = reinterpret_cast<const float*>(smem + k * LT::RING) + row * LT::PITCH + col;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) acc[j] = fmaf(w[k], src[j], acc[j]);
-        }
-        const int qi = (row0 + row) / P.per;
-        const long long token = begin + qi;
-        const int head = h * P.per + row0 + row - qi * P.per;
-        if (own_seg && chunks == 1 && k_begin == 0) {  // the row's only piece
-          const float inv = lsum > 0.0f || lsum != lsum ? 1.0f / lsum : 0.0f;
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const int row = U.row0 + g8 + 8 * i;
+        if (row >= U.rows) continue;
+        const int qi = row / P.per;
+        const long long token = U.begin + qi;
+        const int head = U.head * P.per + row - qi * P.per;
+        if (U.only) {
+          const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
           bf16* dst = static_cast<bf16*>(A.out) + token * A.out_token_stride +
-                      (long long)head * A.out_head_stride + col;
+                      (long long)head * A.out_head_stride + t4 * 2;
 #pragma unroll
-          for (int j = 0; j < D / 8; j += 8) {
-            uint4 pk;
-            uint32_t* pw = reinterpret_cast<uint32_t*>(&pk);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              pw[e] = as_u32(pack2_rn(make_float2(acc[j + 2 * e] * inv, acc[j + 2 * e + 1] * inv)));
-            *reinterpret_cast<uint4*>(dst + j) = pk;
-          }
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<uint32_t*>(dst + n * 8) =
+                as_u32(pack2_rn(make_float2(o[n][i * 2] * inv, o[n][i * 2 + 1] * inv)));
         } else {
-          const long long slot = (token * A.heads + head) * slots + (own_seg ? P.slots_s + c : c);
-          if (col == 0) P.ml[slot] = make_float2(mx, lsum);
-          float* dst = P.o + slot * D + col;
+          const long long slot = (token * A.heads + head) * (P.slots_s + P.slots) +
+                                 (U.seg >= G ? P.slots_s : 0) + U.index;
+          if (t4 == 0) P.ml[slot] = make_float2(m[i], l[i]);
+          float* dst = P.o + slot * D + t4 * 2;
 #pragma unroll
-          for (int j = 0; j < D / 8; j += 4)
-            *reinterpret_cast<float4*>(dst + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][i * 2], o[n][i * 2 + 1]);
         }
       }
     }
-    __syncthreads();  // the rings are free again
   }
 }
 
@@ -532,12 +552,12 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
   } else if (r >= A.num_requests) {
     return;
   }
-  const int chunk_s = P.plan[0], chunk_o = P.plan[1];
   const int g = group_of(P, r), len = length(P, r);
   const int sh = g >= 0 && len > 0 ? P.plan[2 + g] : 0;
-  const int ns = ceil_div(sh, chunk_s), no = len > sh ? ceil_div(len - sh, chunk_o) : 1;
+  const int ns = sh > 0 ? ceil_div(sh, P.plan[0]) : 0;
+  const int no = ceil_div(own_tiles(len, sh), P.plan[1]);
   if (ns == 0 && no == 1) return;  // written already
-  const long long base = row * (P.slots_s + P.slots_o);
+  const long long base = row * (P.slots_s + P.slots);
   float m = -INFINITY, l = 0.0f, acc[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) acc[j] = 0.0f;
@@ -595,13 +615,40 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
 }
 
 // ---------------------------------------------------------------- host side
+int wait_timeouts(int32_t* count, int reset) {
+  int n = 0;
+  const int rc = read_wait_timeouts(&n, reset);
+  return rc ? rc : shared_wait_timeouts(count, reset) ? HYENA_ERR_CUDA : (*count += n, HYENA_OK);
+}
+
+// (head_dim, token in page, head, page) over a cache; box: `rows` tokens of one
+// page and head, 64 columns.
+int cache_map(CUtensorMap* m, const hyena_paged_kv& kv, bool keys, int rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return fail(HYENA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int64_t page = keys ? kv.k_page_stride : kv.v_page_stride;
+  const int64_t token = keys ? kv.k_token_stride : kv.v_token_stride;
+  const int64_t head = keys ? kv.k_head_stride : kv.v_head_stride;
+  // the stride of a dimension of one is never used; give it a valid one
+  cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.kv_heads,
+                        (cuuint64_t)kv.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)token * 2, (cuuint64_t)(kv.kv_heads > 1 ? head : 8) * 2,
+                           (cuuint64_t)(kv.num_pages > 1 ? page : 8) * 2};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, keys ? kv.k : kv.v, dims, strides, boxes,
+                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HYENA_ERR_CUDA, "cuTensorMapEncodeTiled(cache) failed");
+  return HYENA_OK;
+}
+
 // Pieces a row may have, from sizes the host knows: enough that one segment
-// alone spreads over the GPU, bounded by the chunks its pages can hold and by
-// the workspace.
+// alone spreads over the GPU (8 pieces an SM over the key/value heads), bounded
+// by what its pages can hold and by the workspace.
 struct Slots {
   int s, o;
-  bool join;
-  size_t bytes;
+  size_t header, bytes;
 };
 constexpr size_t WORKSPACE_BYTES = size_t(256) << 20;
 
@@ -611,15 +658,14 @@ static Slots slots_of(const hyena_paged_attention_args& A) {
   const long long row_bytes = (A.kv.head_dim + 2) * 4;
   const long long keys = (long long)A.kv.pages_per_request * A.kv.page_size;
   long long n = (8ll * num_sms() + A.kv.kv_heads - 1) / A.kv.kv_heads;
-  n = std::min(n, (keys + MIN_CHUNK - 1) / MIN_CHUNK);
+  n = std::min(n, (keys + MIN_TILES * KT - 1) / (MIN_TILES * KT));
   n = std::min(n, (long long)WORKSPACE_BYTES / (rows * row_bytes * (shared ? 2 : 1)));
   n = std::max(n, 1ll);
   Slots S;
   S.o = (int)n;
   S.s = shared ? (int)n : 0;
-  S.join = shared || n > 1;
-  const size_t head = 8 + 4 * (size_t)A.num_groups;
-  S.bytes = S.join ? ((head + 255) & ~size_t(255)) + (size_t)(rows * (S.s + S.o)) * row_bytes : 0;
+  S.header = (8 + 4 * (size_t)A.num_groups + 255) & ~size_t(255);  // the plan
+  S.bytes = S.header + (size_t)(rows * (S.s + S.o)) * row_bytes;
   return S;
 }
 
@@ -635,6 +681,7 @@ static int check(const hyena_paged_attention_args& A) {
   HB_REQUIRE(A.q_token_stride % 8 == 0 && A.q_head_stride % 8 == 0 && A.out_token_stride % 8 == 0 &&
                  A.out_head_stride % 8 == 0,
              "paged_attention: strides must be multiples of 8 elements");
+  HB_REQUIRE(std::isfinite(A.scale), "paged_attention: scale must be finite");
   HB_REQUIRE((A.shared_lens != nullptr) == (A.num_groups > 0),
              "paged_attention: shared_lens and num_groups go together");
   HB_REQUIRE(A.group_start != nullptr || A.num_groups <= 1,
@@ -653,41 +700,33 @@ static int launch(const hyena_paged_attention_args& A, const Slots& S, void* ws,
   P.per = A.heads / A.kv.kv_heads;
   P.scale = A.scale * 1.4426950408889634f;
   P.slots_s = S.s;
-  P.slots_o = S.o;
+  P.slots = S.o;
   // Shared runs of more rows than one 16-row tile go to the tcgen05 kernel.
   P.tc = S.s > 0 && A.num_groups <= MAX_TC_GROUPS &&
          (long long)A.T * P.per > (long long)TC_MIN_ROWS * A.num_groups;
-  P.plan = nullptr;
-  P.ml = nullptr;
-  P.o = nullptr;
   const long long rows = (long long)A.T * A.heads;
-  if (S.join) {
-    uint8_t* w = static_cast<uint8_t*>(ws);
-    P.plan = reinterpret_cast<int32_t*>(w);
-    w += (8 + 4 * (size_t)A.num_groups + 255) & ~size_t(255);
-    P.o = reinterpret_cast<float*>(w);  // 16-byte pieces first
-    P.ml = reinterpret_cast<float2*>(w + (size_t)(rows * (S.s + S.o)) * D * 4);
-  }
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  P.plan = reinterpret_cast<int32_t*>(w);
+  P.o = reinterpret_cast<float*>(w + S.header);  // 16-byte pieces first
+  P.ml = reinterpret_cast<float2*>(w + S.header + (size_t)(rows * (S.s + S.o)) * D * 4);
   const int segments = A.num_requests + A.num_groups;
-  const size_t smem = Layout<D>::PLAN + (size_t)(segments + 1 + 2 * A.num_groups) * 4;
-  constexpr int smem_max = Layout<D>::PLAN + (MAX_SEGMENTS + 1 + 2 * MAX_SEGMENTS) * 4;
+  const size_t smem = 1024 + Layout<D>::PLAN + (size_t)segments * 20 + 4 + (size_t)A.num_groups * 8;
+  constexpr int smem_max = 1024 + Layout<D>::PLAN + MAX_SEGMENTS * 28 + 4;
   if (!smem_attr<stream_kernel<D>>(smem_max))
     return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(paged_attention) failed");
-  const long long bound = (rows / A.kv.kv_heads / ROWS + segments) * A.kv.kv_heads * (S.s + S.o);
-  const long long ctas = std::min<long long>(2ll * num_sms(), bound);
-  launch_kernel(stream_kernel<D>, dim3((unsigned)ctas), dim3(THREADS), smem, st, 0u, P);
-  if (P.tc) {
-    const int rc = shared_launch(P, st);
-    if (rc) return rc;
-  }
-  if (S.join) {
-    // a block a row while those fill one wave of 16 blocks an SM
-    if (rows <= 16ll * num_sms())
-      launch_kernel(join_kernel<D, WARPS>, dim3((unsigned)rows), dim3(THREADS), 0, st, 0u, P);
-    else
-      launch_kernel(join_kernel<D, 1>, dim3((unsigned)((rows + WARPS - 1) / WARPS)), dim3(THREADS), 0,
-                    st, 0u, P);
-  }
+  CUtensorMap map_k, map_v;
+  int rc = cache_map(&map_k, A.kv, true, KT);
+  if (!rc) rc = cache_map(&map_v, A.kv, false, KT);
+  if (rc) return rc;
+  launch_kernel(stream_kernel<D>, dim3((unsigned)(2 * num_sms())), dim3(THREADS), smem, st, 0u, P, map_k,
+                map_v);
+  if (P.tc && (rc = shared_launch(P, map_k, map_v, st))) return rc;
+  // a block a row while those fill one wave of 16 blocks an SM
+  if (rows <= 16ll * num_sms())
+    launch_kernel(join_kernel<D, WARPS>, dim3((unsigned)rows), dim3(THREADS), 0, st, 0u, P);
+  else
+    launch_kernel(join_kernel<D, 1>, dim3((unsigned)((rows + WARPS - 1) / WARPS)), dim3(THREADS), 0, st,
+                  0u, P);
   return check_launch("paged_attention");
 }
 
@@ -704,7 +743,7 @@ int paged_attention_launch(const hyena_paged_attention_args& A, void* ws, size_t
   if (rc) return rc;
   if (A.T == 0 || A.num_requests == 0) return HYENA_OK;
   const attn::Slots S = attn::slots_of(A);
-  HB_REQUIRE(S.bytes == 0 || (ws != nullptr && aligned16(ws) && ws_bytes >= S.bytes),
+  HB_REQUIRE(ws != nullptr && aligned16(ws) && ws_bytes >= S.bytes,
              "paged_attention: workspace missing, misaligned or too small");
   if (A.kv.head_dim == 128) return attn::launch<128>(A, S, ws, st);
   return attn::launch<64>(A, S, ws, st);

@@ -3,7 +3,7 @@
 // attention_shared.cu (shared runs of many rows).
 #pragma once
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace hb {
 
@@ -18,8 +18,8 @@ struct Params {
   int groups;      // 0: nothing shared
   int per;         // query heads of one key/value head
   float scale;     // scale * log2(e)
-  int slots_s, slots_o;  // pieces a row may have: of the shared run, of its own keys
-  int32_t* plan;   // {chunk_s, chunk_o}, then each group's shared run
+  int slots_s, slots;  // pieces a row may have: of the shared run, of its own keys
+  int32_t* plan;   // {keys of a piece of a shared run, tiles of an own piece}, each group's shared run
   int tc;          // the shared runs go to attention_shared.cu
   float2* ml;      // [T * heads][slots]: (m, l)
   float* o;        // [T * heads][slots][D]
@@ -93,9 +93,59 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// The kernels scale scores by a positive number after the maximum, where masked
+// ones are -inf already: a negative scale's sign, or a zero scale, goes to the
+// query (bf16 pairs: xor .x, and .y).
+__device__ __forceinline__ uint2 query_sign(float scale) {
+  return make_uint2(scale < 0.0f ? 0x80008000u : 0u, scale == 0.0f ? 0u : 0xffffffffu);
+}
+// O is rescaled when a score exceeds the m it is scaled by by more than this.
+constexpr float RESCALE_LOG2 = 8.0f;
+constexpr unsigned long long WAIT_NS = 4000000000ull;  // 4 s
+
+static __device__ int g_wait_timeouts;  // one a source file
+
+// Waits (bounded) for a phase; counts and flags an expired wait.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int32_t* flags) {
+  if (tc::mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = tc::now_ns();
+  while (!tc::mbar_try_wait(bar, parity)) {
+    if (tc::now_ns() - t0 > WAIT_NS) {
+      atomicAdd(&g_wait_timeouts, 1);
+      flag_error(flags, HYENA_FLAG_WAIT);
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* bar, void* dst, int x,
+                                            int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(tc::su32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::su32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+static int read_wait_timeouts(int32_t* count, int reset) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_wait_timeouts, sizeof(int));
+  if (e == cudaSuccess && reset && v != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_wait_timeouts, &zero, sizeof(int));
+  }
+  if (e != cudaSuccess)
+    return fail(HYENA_ERR_CUDA, std::string("attention wait counter: ") + cudaGetErrorString(e));
+  *count = v;
+  return HYENA_OK;
+}
+
+int cache_map(CUtensorMap* m, const hyena_paged_kv& kv, bool keys, int rows);
+
 // Groups the tensor-core kernel of the shared runs takes (its plan's room).
 constexpr int MAX_TC_GROUPS = 64;
-int shared_launch(const Params& P, cudaStream_t st);
+int shared_launch(const Params& P, const CUtensorMap& k16, const CUtensorMap& v16, cudaStream_t st);
 int shared_wait_timeouts(int32_t* count, int reset);
 
 }  // namespace attn

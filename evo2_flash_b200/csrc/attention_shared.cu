@@ -33,7 +33,6 @@
 #include <algorithm>
 
 #include "attention.cuh"
-#include "tcgen05.cuh"
 
 namespace hb {
 namespace attn {
@@ -42,11 +41,7 @@ using namespace tc;
 
 constexpr int TILE_KEYS = 128;
 constexpr int BOX_MIN = 16;
-constexpr unsigned long long WAIT_NS = 4000000000ull;  // 4 s
-constexpr float RESCALE_LOG2 = 8.0f;
 constexpr int ITEM_OVERHEAD = 3;  // tiles that an item's start and end cost
-
-__device__ int g_shared_wait_timeouts;
 
 template <int D, int NT>
 struct Tc {
@@ -75,28 +70,6 @@ struct __align__(1024) TcSmem {
   int first[MAX_TC_GROUPS + 1], shared[MAX_TC_GROUPS], leader[MAX_TC_GROUPS];
 };
 
-// Waits (bounded) for a phase; counts and flags an expired wait.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int32_t* flags) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = now_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (now_ns() - t0 > WAIT_NS) {
-      atomicAdd(&g_shared_wait_timeouts, 1);
-      flag_error(flags, HYENA_FLAG_WAIT);
-      return false;
-    }
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* bar, void* dst, int x,
-                                            int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(su32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(su32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 // D[128 x N] (+)= A[128 x 16] B[N x 16]^T, A in shared memory / in TMEM.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
   asm volatile(
@@ -366,9 +339,9 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     // ---------------------------------------------------------------- softmax
     const int t = warp / 4, row_in = tid % 128;
     const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
-    const float scale = fabsf(P.scale);
-    const uint32_t flip = P.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes to the query
-    const int slots = P.slots_s + P.slots_o;
+    const float scale = P.scale == 0.0f ? 1.0f : fabsf(P.scale);
+    const uint2 sign = query_sign(P.scale);
+    const int slots = P.slots_s + P.slots;
     uint32_t gi = 0;
     bool ok = true;
     for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x) {
@@ -384,7 +357,10 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
         for (int c = 0; c < D / 8; ++c) {
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
           if (row < I.rows) x = src[c];
-          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+          x.x = (x.x ^ sign.x) & sign.y;
+          x.y = (x.y ^ sign.x) & sign.y;
+          x.z = (x.z ^ sign.x) & sign.y;
+          x.w = (x.w ^ sign.x) & sign.y;
           *reinterpret_cast<uint4*>(S.q[t] + (c / 8) * T::HALF_BYTES + row_in * 128 +
                                     (((c & 7) ^ (row_in & 7)) << 4)) = x;
         }
@@ -500,37 +476,14 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
 }
 
 // ---------------------------------------------------------------- host side
-// (head_dim, token in page, head, page) over a cache; box: `rows` tokens of one
-// page and head, 64 columns.
-static int cache_map(CUtensorMap* m, const hyena_paged_kv& kv, const void* base, int64_t page_stride,
-                     int64_t token_stride, int64_t head_stride, int rows) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return fail(HYENA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  // the stride of a dimension of one is never used; give it a valid one
-  cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.kv_heads,
-                        (cuuint64_t)kv.num_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)token_stride * 2,
-                           (cuuint64_t)(kv.kv_heads > 1 ? head_stride : 8) * 2,
-                           (cuuint64_t)(kv.num_pages > 1 ? page_stride : 8) * 2};
-  cuuint32_t boxes[4] = {64, (cuuint32_t)rows, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
-                        boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(HYENA_ERR_CUDA, "cuTensorMapEncodeTiled(cache) failed");
-  return HYENA_OK;
-}
-
 template <int D, int NT>
-static int launch_tc(const Params& P, cudaStream_t st) {
+static int launch_tc(const Params& P, const CUtensorMap& k16, const CUtensorMap& v16, cudaStream_t st) {
   const hyena_paged_kv& kv = P.a.kv;
   int box = BOX_MIN;
   while (box < TILE_KEYS && kv.page_size % (2 * box) == 0) box *= 2;
-  CUtensorMap k, v, k16, v16;
-  int rc = cache_map(&k, kv, kv.k, kv.k_page_stride, kv.k_token_stride, kv.k_head_stride, box);
-  if (!rc) rc = cache_map(&v, kv, kv.v, kv.v_page_stride, kv.v_token_stride, kv.v_head_stride, box);
-  if (!rc) rc = cache_map(&k16, kv, kv.k, kv.k_page_stride, kv.k_token_stride, kv.k_head_stride, BOX_MIN);
-  if (!rc) rc = cache_map(&v16, kv, kv.v, kv.v_page_stride, kv.v_token_stride, kv.v_head_stride, BOX_MIN);
+  CUtensorMap k, v;
+  int rc = cache_map(&k, kv, true, box);
+  if (!rc) rc = cache_map(&v, kv, false, box);
   if (rc) return rc;
   const size_t smem = sizeof(TcSmem<D, NT>) + 1024;
   static_assert(sizeof(TcSmem<D, NT>) + 1024 <= 232448, "shared memory of a CTA");
@@ -543,24 +496,14 @@ static int launch_tc(const Params& P, cudaStream_t st) {
   return check_launch("paged_attention shared");
 }
 
-int shared_launch(const Params& P, cudaStream_t st) {
+int shared_launch(const Params& P, const CUtensorMap& k16, const CUtensorMap& v16, cudaStream_t st) {
   const bool two = (long long)P.a.T * P.per > 128ll * P.groups;  // mean rows of a group
-  if (P.a.kv.head_dim == 128) return two ? launch_tc<128, 2>(P, st) : launch_tc<128, 1>(P, st);
-  return two ? launch_tc<64, 2>(P, st) : launch_tc<64, 1>(P, st);
+  if (P.a.kv.head_dim == 128)
+    return two ? launch_tc<128, 2>(P, k16, v16, st) : launch_tc<128, 1>(P, k16, v16, st);
+  return two ? launch_tc<64, 2>(P, k16, v16, st) : launch_tc<64, 1>(P, k16, v16, st);
 }
 
-int shared_wait_timeouts(int32_t* count, int reset) {
-  int v = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_shared_wait_timeouts, sizeof(int));
-  if (e == cudaSuccess && reset && v != 0) {
-    const int zero = 0;
-    e = cudaMemcpyToSymbol(g_shared_wait_timeouts, &zero, sizeof(int));
-  }
-  if (e != cudaSuccess)
-    return fail(HYENA_ERR_CUDA, std::string("attention wait counter: ") + cudaGetErrorString(e));
-  *count = v;
-  return HYENA_OK;
-}
+int shared_wait_timeouts(int32_t* count, int reset) { return read_wait_timeouts(count, reset); }
 
 }  // namespace attn
 }  // namespace hb

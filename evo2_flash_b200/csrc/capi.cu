@@ -66,7 +66,7 @@ size_t paged_attention_workspace_size(const hyena_paged_attention_args& A);
 int paged_attention_launch(const hyena_paged_attention_args& A, void* ws, size_t ws_bytes,
                            cudaStream_t st);
 namespace attn {
-int shared_wait_timeouts(int32_t* count, int reset);
+int wait_timeouts(int32_t* count, int reset);
 }
 int gemm_gated_bf16_launch(const void* A, int64_t lda, const void* B1, int64_t ldb1, const void* B2,
                            int64_t ldb2, void* out, int64_t ldo, int M, int N, int K, int act,
@@ -263,7 +263,7 @@ int hyena_gemm_gated_bf16(const void* A, int64_t lda, const void* B1, int64_t ld
 int hyena_gemm_wait_timeouts(int32_t* count, int32_t reset) {
   HB_REQUIRE(count != nullptr, "hyena_gemm_wait_timeouts: null count");
   int32_t attention = 0;
-  int rc = attn::shared_wait_timeouts(&attention, reset);
+  int rc = attn::wait_timeouts(&attention, reset);
   if (rc == HYENA_OK) rc = gemm_wait_timeouts(count, reset);
   if (rc == HYENA_OK) *count += attention;
   return rc;

@@ -90,61 +90,64 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
   }
   __syncthreads();
 
-  const int octs = half / 8;
+  const int oct_bits = half == 64 ? 3 : 2;  // 8-element pieces of a half
   const int hq = A.q != nullptr ? A.heads : 0, hkv = A.kv.kv_heads;
-  const int items = (hq + 2 * hkv) * octs;
-  constexpr int U = 3;
-  for (int tok = 0; tok < TB; ++tok) {
-    if (!live[tok]) continue;
-    const long long t = t0 + tok;
-    for (int i0 = tid; i0 < items; i0 += U * KV_THREADS) {
-      uint4 a[U], b[U];
-      bf16* dst[U];
-      int oct[U];
-      bool turned[U];
+  const int items = (hq + 2 * hkv) << oct_bits;
+  constexpr int U = 4;
+  for (int i0 = tid; i0 < TB * items; i0 += U * KV_THREADS) {
+    uint4 a[U], b[U];
+    bf16* dst[U];
+    int oct[U], token[U];
+    bool turned[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * KV_THREADS;
-        dst[u] = nullptr;
-        if (i >= items) continue;
-        int h = i / octs;
-        oct[u] = i - h * octs;
-        const bf16* src;
-        turned[u] = h < hq + hkv;
-        if (h < hq) {
-          src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
-          dst[u] = static_cast<bf16*>(A.q_out) + t * A.q_out_token_stride + h * A.q_out_head_stride;
-        } else if (turned[u]) {
-          h -= hq;
-          src = static_cast<const bf16*>(A.k) + t * A.k_token_stride + h * A.k_head_stride;
-          if (koff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.k) + koff[tok] + h * A.kv.k_head_stride;
-        } else {
-          h -= hq + hkv;
-          src = static_cast<const bf16*>(A.v) + t * A.v_token_stride + h * A.v_head_stride;
-          if (voff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.v) + voff[tok] + h * A.kv.v_head_stride;
-        }
-        if (dst[u] == nullptr) continue;
-        a[u] = *reinterpret_cast<const uint4*>(src + oct[u] * 8);
-        b[u] = *reinterpret_cast<const uint4*>(src + half + oct[u] * 8);
+    for (int u = 0; u < U; ++u) {
+      int i = i0 + u * KV_THREADS;
+      dst[u] = nullptr;
+      if (i >= TB * items) continue;
+      int tok = 0;
+#pragma unroll
+      for (int k = 1; k < TB; ++k) tok += i >= k * items;
+      if (!live[tok]) continue;
+      i -= tok * items;
+      token[u] = tok;
+      const long long t = t0 + tok;
+      int h = i >> oct_bits;
+      oct[u] = i - (h << oct_bits);
+      const bf16* src;
+      turned[u] = h < hq + hkv;
+      if (h < hq) {
+        src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
+        dst[u] = static_cast<bf16*>(A.q_out) + t * A.q_out_token_stride + h * A.q_out_head_stride;
+      } else if (turned[u]) {
+        h -= hq;
+        src = static_cast<const bf16*>(A.k) + t * A.k_token_stride + h * A.k_head_stride;
+        if (koff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.k) + koff[tok] + h * A.kv.k_head_stride;
+      } else {
+        h -= hq + hkv;
+        src = static_cast<const bf16*>(A.v) + t * A.v_token_stride + h * A.v_head_stride;
+        if (voff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.v) + voff[tok] + h * A.kv.v_head_stride;
       }
+      if (dst[u] == nullptr) continue;
+      a[u] = *reinterpret_cast<const uint4*>(src + oct[u] * 8);
+      b[u] = *reinterpret_cast<const uint4*>(src + half + oct[u] * 8);
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (dst[u] == nullptr) continue;
-        if (turned[u]) {
-          uint32_t* aw = reinterpret_cast<uint32_t*>(&a[u]);
-          uint32_t* bw = reinterpret_cast<uint32_t*>(&b[u]);
-          const float4* tab = reinterpret_cast<const float4*>(&cs[tok][oct[u] * 8]);
+    for (int u = 0; u < U; ++u) {
+      if (dst[u] == nullptr) continue;
+      if (turned[u]) {
+        uint32_t* aw = reinterpret_cast<uint32_t*>(&a[u]);
+        uint32_t* bw = reinterpret_cast<uint32_t*>(&b[u]);
+        const float4* tab = reinterpret_cast<const float4*>(&cs[token[u]][oct[u] * 8]);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float4 r = tab[w];  // cos, sin of two pairs
-            const float2 x = unpack2(as_bf162(aw[w])), y = unpack2(as_bf162(bw[w]));
-            aw[w] = as_u32(pack2_rn(make_float2(x.x * r.x - y.x * r.y, x.y * r.z - y.y * r.w)));
-            bw[w] = as_u32(pack2_rn(make_float2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w)));
-          }
+        for (int w = 0; w < 4; ++w) {
+          const float4 r = tab[w];  // cos, sin of two pairs
+          const float2 x = unpack2(as_bf162(aw[w])), y = unpack2(as_bf162(bw[w]));
+          aw[w] = as_u32(pack2_rn(make_float2(x.x * r.x - y.x * r.y, x.y * r.z - y.y * r.w)));
+          bw[w] = as_u32(pack2_rn(make_float2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w)));
         }
-        *reinterpret_cast<uint4*>(dst[u] + oct[u] * 8) = a[u];
-        *reinterpret_cast<uint4*>(dst[u] + half + oct[u] * 8) = b[u];
       }
+      *reinterpret_cast<uint4*>(dst[u] + oct[u] * 8) = a[u];
+      *reinterpret_cast<uint4*>(dst[u] + half + oct[u] * 8) = b[u];
     }
   }
 }

@@ -105,7 +105,7 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  inline PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   if (fn == nullptr) {
     cudaDriverEntryPointQueryResult q;
     void* p = nullptr;

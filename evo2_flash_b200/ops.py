@@ -16,13 +16,13 @@ Kernel-side layouts:
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import (DecodeArgs, KvAppendArgs, LayerParams, PagedAttentionArgs, PrefillArgs,
-                   StateView)
+from ._lib import DecodeArgs, LayerParams, PrefillArgs, StateView
 
 BF16 = torch.bfloat16
 E4M3 = torch.float8_e4m3fn
@@ -484,78 +484,117 @@ def gemm_bf16(a, b, bias=None, out=None):
 
 
 # ---------------------------------------------------------------- attention cache, gated MLP
+# These are called once a layer and decode step, so their host side counts: the
+# argument structs are packed in one go (layouts as in include/hyena_b200.h,
+# native alignment) and the stream is read without building a torch.cuda.Stream.
 ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2}
+_PAGED_KV = "PP6qPq5i"  # hyena_paged_kv
+_KV_APPEND = struct.Struct("@PqqPqqPqqPqqPP3i" + _PAGED_KV + "dP")          # hyena_kv_append_args
+_PAGED_ATTENTION = struct.Struct("@PqqPqqPPPP4if" + _PAGED_KV + "P")        # hyena_paged_attention_args
 
 
-def _operands(**tensors):
-    """Checks that the given tensors (None: absent) are on one CUDA device and
-    need no gradient; returns the device.  These operators have no backward pass."""
+def _same_device(names, *tensors):
+    """The index of the one CUDA device that the given tensors (None: absent) are
+    on; refuses others, and tensors that need a gradient: these operators have no
+    backward pass."""
     device = None
-    for name, t in tensors.items():
+    grad = torch.is_grad_enabled()
+    for i, t in enumerate(tensors):
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
+        d = t.get_device()
+        if d < 0:
+            raise ValueError(f"{names.split()[i]} must be a CUDA tensor")
         if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires grad: this operator has no backward pass "
+            device = d
+        elif d != device:
+            raise ValueError(f"{names.split()[i]} is on cuda:{d}, not on cuda:{device}")
+        if grad and t.requires_grad:
+            raise ValueError(f"{names.split()[i]} requires grad: this operator has no backward pass "
                              "(call it under torch.no_grad())")
     return device
 
 
-def _launch_on(device, launch):
-    """launch(stream) with `device` current, on its current stream."""
-    if device.index == torch.cuda.current_device():
-        return launch(_stream())
-    with torch.cuda.device(device):
-        return launch(_stream())
+class _On:
+    """`with _On(device) as stream:` makes the device current if it is not, and
+    gives its current stream's handle."""
+
+    __slots__ = ("device", "guard")
+
+    def __init__(self, device):
+        self.device, self.guard = device, None
+
+    def __enter__(self):
+        if torch._C._cuda_getDevice() != self.device:
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.device)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
-def _rows3(t, name, heads=None, dim=None):
-    if t.dim() != 3 or t.dtype != BF16 or t.stride(2) != 1:
-        raise ValueError(f"{name} must be (tokens, heads, head_dim) bf16 with unit last stride, "
-                         f"got {tuple(t.shape)} {t.dtype}")
-    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
-        raise ValueError(f"{name} must have {heads} heads of {dim}, got {tuple(t.shape)}")
+def _rows3(t, name, heads, dim):
+    """(tokens, token stride, head stride) of a (tokens, heads, dim) bf16 tensor."""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype is not BF16:
+        raise ValueError(f"{name} must be (tokens, heads, head_dim) bf16, got {tuple(shape)} {t.dtype}")
+    n, h, d = shape
+    if d != dim or (heads is not None and h != heads):
+        raise ValueError(f"{name} must have {'' if heads is None else str(heads) + ' '}heads of {dim}, "
+                         f"got {tuple(shape)}")
+    a, b, c = t.stride()
+    if c != 1:
+        raise ValueError(f"{name} must have a unit last stride, got {t.stride()}")
+    return n, a if n > 1 else 0, b if h > 1 else 0
 
 
 def _ints(t, name, at_least):
-    """A 1-D contiguous int32 view (converted if need be) of at least `at_least` elements."""
+    """A 1-D contiguous int32 tensor (converted if need be) of at least `at_least` elements."""
     if t.dim() != 1 or t.shape[0] < at_least:
         raise ValueError(f"{name} must be 1-D with at least {at_least} elements, got {tuple(t.shape)}")
-    if t.is_floating_point() or t.dtype == torch.bool:
-        raise ValueError(f"{name} must hold integers, got {t.dtype}")
-    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+    if t.dtype is not torch.int32:
+        if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+            raise ValueError(f"{name} must hold integers, got {t.dtype}")
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _paged_kv(kv, k_cache, v_cache, page_table, requests):
-    """Fills the hyena_paged_kv `kv`; returns the page table it points to."""
+def _cache_shape(k_cache, v_cache):
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.dim() != 4 or t.dtype != BF16 or t.stride(3) != 1:
+        if t.dim() != 4 or t.dtype is not BF16 or t.stride(3) != 1:
             raise ValueError(f"{name} must be (pages, page size, kv heads, head_dim) bf16 with unit "
                              f"last stride, got {tuple(t.shape)} {t.dtype}")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
+    shape = k_cache.shape
+    if shape != v_cache.shape:
+        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)} differ")
+    return shape
+
+
+def _paged_kv(k_cache, v_cache, shape, page_table, requests):
+    """The fields of hyena_paged_kv, and the page table they point to."""
     if page_table.dim() != 2 or page_table.shape[0] < requests or page_table.is_floating_point():
         raise ValueError(f"page_table must be (>= {requests} requests, pages) int, "
                          f"got {tuple(page_table.shape)} {page_table.dtype}")
-    if page_table.dtype != torch.int32 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+    row, one = page_table.stride()
+    if page_table.dtype is not torch.int32 or (one != 1 and page_table.shape[1] > 1):
         page_table = page_table.to(torch.int32).contiguous()
-    kv.k, kv.v = k_cache.data_ptr(), v_cache.data_ptr()
-    kv.k_page_stride, kv.k_token_stride, kv.k_head_stride, _ = k_cache.stride()
-    kv.v_page_stride, kv.v_token_stride, kv.v_head_stride, _ = v_cache.stride()
-    kv.page_table, kv.page_table_stride = page_table.data_ptr(), page_table.stride(0)
-    kv.num_pages, kv.page_size, kv.kv_heads, kv.head_dim = k_cache.shape
-    kv.pages_per_request = page_table.shape[1]
-    return page_table
+        row = page_table.stride(0)
+    kp, kt, kh, _ = k_cache.stride()
+    vp, vt, vh, _ = v_cache.stride()
+    pages, _, heads, _ = shape
+    if pages == 1:
+        kp = vp = 0
+    if heads == 1:
+        kh = vh = 0
+    return (k_cache.data_ptr(), v_cache.data_ptr(), kp, kt, kh, vp, vt, vh, page_table.data_ptr(), row,
+            page_table.shape[1], *shape), page_table
 
 
 def _flags_ptr(error_flags):
     if error_flags is None:
-        return None
+        return 0
     _require(error_flags.dtype == torch.int32 and error_flags.numel() >= 1,
              "error_flags must be an int32 tensor")
     return error_flags.data_ptr()
@@ -579,48 +618,50 @@ def kv_append(q, k, v, positions, k_cache, v_cache, page_table, query_start_loc=
     error_flags.  No two tokens of a step may name the same row.
 
     Returns the rotated queries: q_out (may be q) or a new tensor; None for q None."""
-    device = _operands(k=k, q=q, v=v, positions=positions, k_cache=k_cache, v_cache=v_cache,
-                       page_table=page_table, query_start_loc=query_start_loc, q_out=q_out,
-                       error_flags=error_flags)
-    T, dim = k.shape[0], k_cache.shape[-1]
-    kv_heads = k_cache.shape[2] if k_cache.dim() == 4 else None
-    _rows3(k, "k", kv_heads, dim)
-    _rows3(v, "v", kv_heads, dim)
-    _require(v.shape[0] == T, f"v has {v.shape[0]} tokens, k {T}")
+    device = _same_device("k v positions k_cache v_cache page_table q query_start_loc q_out error_flags",
+                          k, v, positions, k_cache, v_cache, page_table, q, query_start_loc, q_out,
+                          error_flags)
+    shape = _cache_shape(k_cache, v_cache)
+    kv_heads, dim = shape[2], shape[3]
+    T, k_token, k_head = _rows3(k, "k", kv_heads, dim)
+    n, v_token, v_head = _rows3(v, "v", kv_heads, dim)
+    if n != T:
+        raise ValueError(f"v has {n} tokens, k {T}")
+    heads = 0
+    q_ptr = q_token = q_head = out_ptr = out_token = out_head = 0
     if q is not None:
-        _rows3(q, "q", None, dim)
-        _require(q.shape[0] == T, f"q has {q.shape[0]} tokens, k {T}")
+        n, q_token, q_head = _rows3(q, "q", None, dim)
+        if n != T:
+            raise ValueError(f"q has {n} tokens, k {T}")
+        heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=BF16, device=device)
+            q_out = torch.empty((T, heads, dim), dtype=BF16, device=k.device)
+            out_token, out_head = heads * dim, dim
         else:
-            _rows3(q_out, "q_out", q.shape[1], dim)
-            _require(q_out.shape[0] == T, f"q_out has {q_out.shape[0]} tokens, q {T}")
-    else:
-        _require(q_out is None, "q_out without q")
+            n, out_token, out_head = _rows3(q_out, "q_out", heads, dim)
+            if n != T:
+                raise ValueError(f"q_out has {n} tokens, q {T}")
+        q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
     positions = _ints(positions, "positions", T)
+    requests = page_table.shape[0]
+    starts = 0
     if query_start_loc is not None:
         query_start_loc = _ints(query_start_loc, "query_start_loc", 1)
         requests = query_start_loc.shape[0] - 1
-    else:
-        requests = page_table.shape[0]
-    a = KvAppendArgs()
-    table = _paged_kv(a.kv, k_cache, v_cache, page_table, requests)
+        starts = query_start_loc.data_ptr()
+    kv, table = _paged_kv(k_cache, v_cache, shape, page_table, requests)
     if T == 0 or requests == 0:
         return q_out
-    if q is not None:
-        a.q, (a.q_token_stride, a.q_head_stride, _) = q.data_ptr(), q.stride()
-        a.q_out, (a.q_out_token_stride, a.q_out_head_stride, _) = q_out.data_ptr(), q_out.stride()
-        a.heads = q.shape[1]
-    a.k, (a.k_token_stride, a.k_head_stride, _) = k.data_ptr(), k.stride()
-    a.v, (a.v_token_stride, a.v_head_stride, _) = v.data_ptr(), v.stride()
-    a.positions = positions.data_ptr()
-    a.query_start_loc = None if query_start_loc is None else query_start_loc.data_ptr()
-    a.T, a.num_requests = T, requests
-    a.rope_theta = rope_theta
-    a.error_flags = _flags_ptr(error_flags)
-    _lib.check(_launch_on(device, lambda st: _lib.load().hyena_kv_append(C.byref(a), st)),
-               "hyena_kv_append")
+    args = _KV_APPEND.pack(q_ptr, q_token, q_head, out_ptr, out_token, out_head, k.data_ptr(), k_token,
+                           k_head, v.data_ptr(), v_token, v_head, positions.data_ptr(), starts, T,
+                           requests, heads, *kv, rope_theta, _flags_ptr(error_flags))
+    with _On(device) as stream:
+        rc = _lib.load().hyena_kv_append(args, stream)
     del table  # alive until the launch returned
+    if rc:
+        _lib.check(rc, "hyena_kv_append")
     return q_out
 
 
@@ -643,51 +684,51 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
     One launch, and one that joins the pieces of split rows; lengths and tables
     are read on the device, so a captured graph serves growing contexts.  The
     workspace comes from torch's caching allocator.  Returns (T, heads, D) bf16."""
-    device = _operands(q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
-                       seq_lens=seq_lens, query_start_loc=query_start_loc, shared_lens=shared_lens,
-                       group_start=group_start, out=out, error_flags=error_flags)
-    _rows3(q, "q", None, k_cache.shape[-1])
-    T, heads, dim = q.shape
+    device = _same_device("q k_cache v_cache page_table seq_lens query_start_loc shared_lens group_start "
+                          "out error_flags", q, k_cache, v_cache, page_table, seq_lens, query_start_loc,
+                          shared_lens, group_start, out, error_flags)
+    shape = _cache_shape(k_cache, v_cache)
+    dim = shape[3]
+    T, q_token, q_head = _rows3(q, "q", None, dim)
+    heads = q.shape[1]
     seq_lens = _ints(seq_lens, "seq_lens", 0)
     requests = seq_lens.shape[0]
+    starts = shared = group = groups = 0
     if query_start_loc is not None:
         query_start_loc = _ints(query_start_loc, "query_start_loc", requests + 1)
-    groups = 0
+        starts = query_start_loc.data_ptr()
     if shared_lens is not None:
         shared_lens = _ints(shared_lens, "shared_lens", 1)
-        groups = shared_lens.shape[0]
+        groups, shared = shared_lens.shape[0], shared_lens.data_ptr()
         if group_start is not None:
             group_start = _ints(group_start, "group_start", groups + 1)
-        _require(group_start is not None or groups == 1, "several groups need group_start")
-    else:
-        _require(group_start is None, "group_start without shared_lens")
+            group = group_start.data_ptr()
+        elif groups > 1:
+            raise ValueError("several groups need group_start")
+    elif group_start is not None:
+        raise ValueError("group_start without shared_lens")
     if out is None:
-        out = torch.empty(q.shape, dtype=BF16, device=device)
+        out = torch.empty((T, heads, dim), dtype=BF16, device=q.device)
+        out_token, out_head = heads * dim, dim
     else:
-        _rows3(out, "out", heads, dim)
-        _require(out.shape[0] == T, f"out has {out.shape[0]} tokens, q {T}")
-    a = PagedAttentionArgs()
-    table = _paged_kv(a.kv, k_cache, v_cache, page_table, requests)
+        n, out_token, out_head = _rows3(out, "out", heads, dim)
+        if n != T:
+            raise ValueError(f"out has {n} tokens, q {T}")
+    kv, table = _paged_kv(k_cache, v_cache, shape, page_table, requests)
     if T == 0 or requests == 0:
         return out
-    a.q, (a.q_token_stride, a.q_head_stride, _) = q.data_ptr(), q.stride()
-    a.out, (a.out_token_stride, a.out_head_stride, _) = out.data_ptr(), out.stride()
-    a.seq_lens = seq_lens.data_ptr()
-    a.query_start_loc = None if query_start_loc is None else query_start_loc.data_ptr()
-    a.shared_lens = None if shared_lens is None else shared_lens.data_ptr()
-    a.group_start = None if group_start is None else group_start.data_ptr()
-    a.T, a.num_requests, a.num_groups, a.heads = T, requests, groups, heads
-    a.scale = dim ** -0.5 if scale is None else scale
-    a.error_flags = _flags_ptr(error_flags)
+    args = _PAGED_ATTENTION.pack(
+        q.data_ptr(), q_token, q_head, out.data_ptr(), out_token, out_head, seq_lens.data_ptr(), starts,
+        shared, group, T, requests, groups, heads, dim ** -0.5 if scale is None else scale, *kv,
+        _flags_ptr(error_flags))
     lib = _lib.load()
-
-    def launch(st):
-        n = lib.hyena_paged_attention_workspace_size(C.byref(a))
-        ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        return lib.hyena_paged_attention(C.byref(a), None if ws is None else ws.data_ptr(), n, st)
-
-    _lib.check(_launch_on(device, launch), "hyena_paged_attention")
+    with _On(device) as stream:
+        n = lib.hyena_paged_attention_workspace_size(args)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        rc = lib.hyena_paged_attention(args, 0 if ws is None else ws.data_ptr(), n, stream)
     del table  # alive until the launch returned
+    if rc:
+        _lib.check(rc, "hyena_paged_attention")
     return out
 
 
@@ -703,7 +744,7 @@ def gemm_gated_bf16(a, b1, b2, activation="none", out=None):
     """out (M, N) bf16 = act(a . b1^T) * (a . b2^T): a (M, K), b1 and b2 (N, K)
     bf16, activation "none", "gelu" (erf) or "silu", fp32 up to the one rounding
     (hyena_gemm_gated_bf16, tcgen05).  K % 64 == 0, N % 8 == 0."""
-    device = _operands(a=a, b1=b1, b2=b2, out=out)
+    device = _same_device("a b1 b2 out", a, b1, b2, out)
     _matrix(a, "a")
     M, K = a.shape
     _matrix(b1, "b1", K)
@@ -713,15 +754,18 @@ def gemm_gated_bf16(a, b1, b2, activation="none", out=None):
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
     if out is None:
-        out = torch.empty(M, N, dtype=BF16, device=device)
+        out = torch.empty(M, N, dtype=BF16, device=a.device)
     else:
         _matrix(out, "out", N)
         _require(out.shape[0] == M, f"out must have {M} rows, got {out.shape[0]}")
     # a one-row tensor may carry any row stride: its length is what counts
     ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1]  # noqa: E731
-    _lib.check(_launch_on(device, lambda st: _lib.load().hyena_gemm_gated_bf16(
-        a.data_ptr(), ld(a), b1.data_ptr(), ld(b1), b2.data_ptr(), ld(b2), out.data_ptr(), ld(out),
-        M, N, K, ACTIVATIONS[activation], st)), "hyena_gemm_gated_bf16")
+    with _On(device) as stream:
+        rc = _lib.load().hyena_gemm_gated_bf16(a.data_ptr(), ld(a), b1.data_ptr(), ld(b1), b2.data_ptr(),
+                                               ld(b2), out.data_ptr(), ld(out), M, N, K,
+                                               ACTIVATIONS[activation], stream)
+    if rc:
+        _lib.check(rc, "hyena_gemm_gated_bf16")
     return out
 
 
@@ -731,7 +775,7 @@ def gated_mlp(x, w1, w2, w3, activation="none", out=None):
     (I, H), w3 (H_out, I) bf16; H and I multiples of 64.  Two launches: both
     projections with the activation and the product (gemm_gated_bf16, whose
     result is the one bf16 intermediate), then gemm_bf16."""
-    _operands(x=x, w1=w1, w2=w2, w3=w3, out=out)
+    device = _same_device("x w1 w2 w3 out", x, w1, w2, w3, out)
     _matrix(w1, "w1")
     _matrix(w3, "w3", w1.shape[0])
     _require(w1.shape[0] % 64 == 0, f"the inner width must be a multiple of 64, got {w1.shape[0]}")
@@ -743,7 +787,5 @@ def gated_mlp(x, w1, w2, w3, activation="none", out=None):
         out = torch.empty(h.shape[0], w3.shape[0], dtype=BF16, device=h.device)
     if h.shape[0] == 0:
         return out
-    if h.device.index == torch.cuda.current_device():
-        return gemm_bf16(h, w3, out=out)
-    with torch.cuda.device(h.device):
+    with _On(device):
         return gemm_bf16(h, w3, out=out)

@@ -83,6 +83,7 @@ def test_append_refuses(lib, change, text):
     ({"out_token_stride": 4}, b"multiples of 8"), ({"num_groups": 1}, b"go together"),
     ({"shared_lens": 4096}, b"go together"), ({"shared_lens": 4096, "num_groups": 2}, b"group_start"),
     ({"T": 2100, "num_requests": 2100}, b"2048"), ({"T": 1 << 30}, b"too many"),
+    ({"scale": float("nan")}, b"finite"), ({"scale": float("inf")}, b"finite"),
     ({}, b"workspace"),  # several chunks fit the table: a workspace is needed
 ])
 def test_attention_refuses(lib, change, text):
@@ -103,14 +104,14 @@ def test_null_arguments_and_empty_steps(lib):
 
 
 def test_workspace_is_bounded(lib):
-    """None for a table of one chunk with nothing shared; otherwise a few pieces a
-    row, at most 256 MB and a fixed part while the rows allow it."""
+    """The plan, and a few pieces a row: at most what the pages hold, and 256 MB
+    beyond the plan while one piece a row allows it."""
     size = lambda **kw: lib.hyena_paged_attention_workspace_size(C.byref(attention_args(**kw)))  # noqa: E731
-    assert size(kv_pages_per_request=8) == 0
-    one = size(kv_pages_per_request=8, shared_lens=4096, num_groups=1)
-    assert one == 256 + 3 * 4 * 2 * 130 * 4
+    assert size(kv_pages_per_request=8) == 256 + 3 * 4 * 2 * 130 * 4  # 128 keys: two pieces a row
+    assert size(kv_pages_per_request=1, shared_lens=4096, num_groups=1) == 256 + 3 * 4 * 2 * 130 * 4
+    assert size(kv_pages_per_request=1) == 256 + 3 * 4 * 130 * 4
     for T in (1, 64, 1024):
-        assert 0 < size(T=T, num_requests=T, heads=64, kv_pages_per_request=1 << 16) <= (256 << 20) + 4096
+        assert 0 < size(T=T, num_requests=T, heads=64, kv_pages_per_request=1 << 16) <= (256 << 20) + 16384
 
 
 @pytest.mark.parametrize("change,text", [
@@ -123,3 +124,35 @@ def test_gated_gemm_refuses(lib, change, text):
     a.update(change)
     assert lib.hyena_gemm_gated_bf16(*a.values(), None) == 1
     assert text in lib.hyena_last_error()
+
+
+def test_packed_arguments_have_the_structs_layout():
+    """ops.py packs the argument structs itself: every field lands where the C
+    struct (the ctypes declaration) has it."""
+    from evo2_flash_b200 import ops
+    from evo2_flash_b200._lib import KvAppendArgs, PagedAttentionArgs
+
+    def flat(s):
+        for name, kind in s._fields_:
+            v = getattr(s, name)
+            if isinstance(v, C.Structure):
+                yield from flat(v)
+            else:
+                yield v or 0
+
+    def fill(s, n=1):
+        for name, kind in s._fields_:
+            if issubclass(kind, C.Structure):
+                n = fill(getattr(s, name), n)
+            else:
+                setattr(s, name, n)
+                n += 1
+        return n
+
+    for kind, packed in ((KvAppendArgs, ops._KV_APPEND), (PagedAttentionArgs, ops._PAGED_ATTENTION)):
+        a = kind()
+        fill(a)
+        values = list(flat(a))
+        assert packed.size <= C.sizeof(kind)  # the struct may end in padding
+        b = kind.from_buffer_copy(packed.pack(*values).ljust(C.sizeof(kind), b"\0"))
+        assert list(flat(b)) == values
