@@ -62,7 +62,7 @@ struct __align__(1024) TcSmem {
   uint8_t ring[Tc<D, NT>::SLOTS][Tc<D, NT>::TILE_BYTES];
   uint64_t full[Tc<D, NT>::SLOTS], empty[Tc<D, NT>::SLOTS];
   uint64_t q_full;
-  uint64_t s_full[NT][2], p_full[NT], pv_done[NT];
+  uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT];  // [..][score buffer]
   uint32_t bad[8];  // 16-key blocks of a tile whose page is out of range
   uint32_t tmem;
   unsigned long long best[16];
@@ -142,8 +142,10 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     }
     mbar_init(&S.q_full, NT * 128);
     for (int t = 0; t < NT; ++t) {
-      for (int b = 0; b < 2; ++b) mbar_init(&S.s_full[t][b], 2);
-      mbar_init(&S.p_full[t], 128);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&S.s_full[t][b], 2);
+        mbar_init(&S.p_full[t][b], 128);
+      }
       mbar_init(&S.pv_done[t], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -316,7 +318,10 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
             }
           }
           for (int t = 0; t < NT && ok; ++t) {
-            ok = ok && wait(&S.p_full[t], gi & 1, A.error_flags);
+            // (a barrier a buffer: a warp without rows is done with the next tile's
+            // scores before the others are with this one's)
+            ok = ok && wait(&S.p_full[t][T::NBUF == 2 ? (gi & 1) : 0],
+                            T::NBUF == 2 ? (gi >> 1) & 1 : gi & 1, A.error_flags);
             if (t == 0) slot_full(u + 1);
             if (!ok) break;
             fence_after();
@@ -437,8 +442,13 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
           l += a.x + a.y;
           tmem_wait_st();
         }
+        // Every phase of pv_done is seen in turn, since a parity tells only
+        // neighbours apart: with two score buffers the product before last is known
+        // to be complete here, the last one need not be (it ran under this softmax).
+        if (gi > 0) ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
+        if (!ok) break;
         fence_before();
-        mbar_arrive(&S.p_full[t]);
+        mbar_arrive(&S.p_full[t][b]);
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));

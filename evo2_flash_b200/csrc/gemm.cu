@@ -29,6 +29,7 @@
 // records the event in a device counter and runs to completion (TMEM freed);
 // hyena_gemm_wait_timeouts reads the counter back, so a GEMM that gave up
 // (and wrote an incomplete tile) is reported instead of passing silently.
+#include <algorithm>
 #include <atomic>
 
 #include "tcgen05.cuh"
@@ -160,14 +161,22 @@ __device__ __forceinline__ void tile_mn(int tile, int m_tiles, int n_tiles, int&
   }
 }
 
+// The last row tile's activations come through a tensor map of their own (tmT),
+// whose box is as high as its rows (`tail_rows`): the rows behind M in a full box
+// are not read, but filling them in shared memory costs as much as reading them
+// would (one token of the 7B gated projections: 55 us a launch with the full
+// box).  What the rows behind the box hold reaches only accumulator rows that are
+// not stored.
+static int tail_box_rows(int M) { return M % BM == 0 ? BM : M % BM; }
+
 template <bool FP8, int BN, bool GATED>
 __device__ __forceinline__ void
-gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
+gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmT, const CUtensorMap& tmB, const CUtensorMap& tmB2,
           bf16* __restrict__ out, int64_t ldo, int M, int N, int K, const float* __restrict__ sa,
-          const float* __restrict__ sb, const bf16* __restrict__ bias, int act) {
+          const float* __restrict__ sb, const bf16* __restrict__ bias, int act, int tail_rows) {
   constexpr int HN = GATED ? BN / 2 : BN;  // output columns of a tile
+  constexpr int CW = HN % 32 == 0 ? 32 : 16;  // columns of an epilogue step
   constexpr int STAGES = Cfg<BN>::STAGES;
-  constexpr int STAGE_BYTES = Cfg<BN>::STAGE_BYTES;
   constexpr uint32_t TMEM_COLS = Cfg<BN>::TMEM_COLS;
   extern __shared__ uint8_t smem_raw[];
   Smem<BN>& S = *reinterpret_cast<Smem<BN>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -231,11 +240,14 @@ gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB
         int mt, nt;
         tile_mn<GATED>(tile, m_tiles, n_tiles, mt, nt);
         const int m0 = mt * BM, n0 = nt * HN;
+        const bool tail = M - m0 < BM;
+        const CUtensorMap* map_a = tail ? &tmT : &tmA;
+        const int a_rows = tail ? tail_rows : BM;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
-          mbar_expect_tx(&S.full[s], STAGE_BYTES);
-          tma_load_2d(&tmA, &S.full[s], S.a[s], kb * KE, m0, pol_a);
+          mbar_expect_tx(&S.full[s], uint32_t(Cfg<BN>::B_BYTES + a_rows * BKB));
+          tma_load_2d(map_a, &S.full[s], S.a[s], kb * KE, m0, pol_a);
           tma_load_2d(&tmB, &S.full[s], S.b[s], kb * KE, n0, pol_b);
           if constexpr (GATED)
             tma_load_2d(&tmB2, &S.full[s], S.b[s] + HN * BKB, kb * KE, n0, pol_b);
@@ -288,29 +300,35 @@ gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB
       fence_after();
       const int row = m0 + 32 * q + lane;
 #pragma unroll 1
-      for (int cb = 0; cb < HN / 32; ++cb) {
-        uint32_t r[32];
+      for (int cb = 0; cb < HN / CW; ++cb) {
+        uint32_t r[CW];
         if constexpr (GATED) {
-          uint32_t r2[32];
-          tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + cb * 32), r);
-          tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + HN + cb * 32), r2);
+          uint32_t r2[CW];
+          const uint32_t col = tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + cb * CW);
+          if constexpr (CW == 32) {
+            tmem_ld32_async(col, r);
+            tmem_ld32_async(col + HN, r2);
+          } else {
+            tmem_ld16_async(col, r);
+            tmem_ld16_async(col + HN, r2);
+          }
           tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
+          for (int j = 0; j < CW; ++j)
             r[j] = __float_as_uint(gate(__uint_as_float(r[j]), __uint_as_float(r2[j]), act));
         } else {
           tmem_ld32(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN + cb * 32), r);
         }
-        if (cb == HN / 32 - 1) {  // accumulator fully read: hand it back to the MMA warp
+        if (cb == HN / CW - 1) {  // accumulator fully read: hand it back to the MMA warp
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&S.acc_empty[b]);
         }
-        const int col0 = n0 + cb * 32;
+        const int col0 = n0 + cb * CW;
         if (row >= M || col0 >= N) continue;
         bf16* dst = out + (long long)row * ldo + col0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        for (int v = 0; v < CW / 8; ++v) {
           if (col0 + 8 * v >= N) break;
           uint4 pk;
           uint32_t* pw = reinterpret_cast<uint32_t*>(&pk);
@@ -348,18 +366,20 @@ gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB
 
 template <bool FP8, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-            bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
+gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmT,
+            const __grid_constant__ CUtensorMap tmB, bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
             const float* __restrict__ sa, const float* __restrict__ sb,
-            const bf16* __restrict__ bias) {
-  gemm_body<FP8, BN, false>(tmA, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0);
+            const bf16* __restrict__ bias, int tail_rows) {
+  gemm_body<FP8, BN, false>(tmA, tmT, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0, tail_rows);
 }
 template <int BN>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB1,
+gemm_gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmT,
+                  const __grid_constant__ CUtensorMap tmB1,
                   const __grid_constant__ CUtensorMap tmB2, bf16* __restrict__ out, int64_t ldo,
-                  int M, int N, int K, int act) {
-  gemm_body<false, BN, true>(tmA, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr, act);
+                  int M, int N, int K, int act, int tail_rows) {
+  gemm_body<false, BN, true>(tmA, tmT, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr, act,
+                             tail_rows);
 }
 
 // ---------------------------------------------------------------- small M
@@ -450,13 +470,13 @@ __host__ __device__ constexpr uint32_t pow2_cols() {
 // copies have landed.
 template <bool FP8, int BN, bool GATED>
 __device__ __forceinline__ void
-gemm_cluster_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
+gemm_cluster_body(const CUtensorMap& tmA, const CUtensorMap& tmT, const CUtensorMap& tmB,
+                  const CUtensorMap& tmB2,
                   bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
                   const float* __restrict__ sa, const float* __restrict__ sb,
-                  const bf16* __restrict__ bias, int act) {
+                  const bf16* __restrict__ bias, int act, int tail_rows) {
   constexpr int HN = GATED ? BN / 2 : BN;  // output columns of a tile
   constexpr int STAGES = Cfg<BN>::STAGES;
-  constexpr int STAGE_BYTES = Cfg<BN>::STAGE_BYTES;
   constexpr uint32_t TMEM_COLS = pow2_cols<BN>();
   constexpr int LD = SmemSK<BN>::RED_LD;
   static_assert(BN % 32 == 0, "epilogue reads 32 columns at a time");
@@ -520,6 +540,8 @@ gemm_cluster_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensor
 
   if (warp == 0) {
     if (lane == 0) {
+      const CUtensorMap* map_a = rows < BM ? &tmT : &tmA;
+      const int a_rows = rows < BM ? tail_rows : BM;
       // The activations are re-read by every tile's cluster, the weights once.
       const uint64_t pol_a = policy_evict_last();
       const uint64_t pol_b = policy_evict_first();
@@ -527,8 +549,8 @@ gemm_cluster_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensor
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % STAGES;
         if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1) ^ 1)) break;
-        mbar_expect_tx(&S.full[s], STAGE_BYTES);
-        tma_load_2d(&tmA, &S.full[s], S.u.ring.a[s], kb * KE, m0, pol_a);
+        mbar_expect_tx(&S.full[s], uint32_t(Cfg<BN>::B_BYTES + a_rows * BKB));
+        tma_load_2d(map_a, &S.full[s], S.u.ring.a[s], kb * KE, m0, pol_a);
         tma_load_2d(&tmB, &S.full[s], S.u.ring.b[s], kb * KE, n0, pol_b);
         if constexpr (GATED)
           tma_load_2d(&tmB2, &S.full[s], S.u.ring.b[s] + HN * BKB, kb * KE, n0, pol_b);
@@ -721,20 +743,21 @@ gemm_cluster_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensor
 
 template <bool FP8, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
+gemm_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmT,
                     const __grid_constant__ CUtensorMap tmB, bf16* __restrict__ out, int64_t ldo,
                     int M, int N, int K, const float* __restrict__ sa,
-                    const float* __restrict__ sb, const bf16* __restrict__ bias) {
-  gemm_cluster_body<FP8, BN, false>(tmA, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0);
+                    const float* __restrict__ sb, const bf16* __restrict__ bias, int tail_rows) {
+  gemm_cluster_body<FP8, BN, false>(tmA, tmT, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0, tail_rows);
 }
 template <int BN>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_gated_cluster_kernel(const __grid_constant__ CUtensorMap tmA,
+                          const __grid_constant__ CUtensorMap tmT,
                           const __grid_constant__ CUtensorMap tmB1,
                           const __grid_constant__ CUtensorMap tmB2, bf16* __restrict__ out,
-                          int64_t ldo, int M, int N, int K, int act) {
-  gemm_cluster_body<false, BN, true>(tmA, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr,
-                                     act);
+                          int64_t ldo, int M, int N, int K, int act, int tail_rows) {
+  gemm_cluster_body<false, BN, true>(tmA, tmT, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr,
+                                     act, tail_rows);
 }
 
 // ---------------------------------------------------------------- 2-SM tiles
@@ -819,10 +842,10 @@ __host__ __device__ constexpr uint32_t idesc_pair() {
 
 template <bool FP8, bool GATED>
 __device__ __forceinline__ void
-gemm_pair_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
+gemm_pair_body(const CUtensorMap& tmA, const CUtensorMap& tmT, const CUtensorMap& tmB, const CUtensorMap& tmB2,
                bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
                const float* __restrict__ sa, const float* __restrict__ sb,
-               const bf16* __restrict__ bias, int act) {
+               const bf16* __restrict__ bias, int act, int tail_rows) {
   // Gated: the even CTA's B rows are B1's, the odd CTA's the same rows of B2.
   constexpr int HN = GATED ? BN2 / 2 : BN2;  // output columns of a tile
   pdl_trigger();
@@ -883,12 +906,16 @@ gemm_pair_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap
         tile_mn<GATED>(tile, m_tiles, n_tiles, mt, nt);
         const int m0 = mt * 2 * BM + (int)rank * BM;
         const int n0 = nt * HN + (GATED ? 0 : (int)rank * (BN2 / 2));
+        const CUtensorMap* map_a = M - m0 < BM ? &tmT : &tmA;
+        // operand bytes of the two CTAs, which the even one expects
+        const int pair_rows = M - m0 >= 2 * BM ? 2 * BM : M - m0 >= BM ? BM + tail_rows : 2 * tail_rows;
+        const uint32_t bytes = uint32_t(2 * Cfg2::B_BYTES + pair_rows * BKB);
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&S.empty[s], ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(&S.full[s], 2 * Cfg2::STAGE_BYTES);
+          if (rank == 0) mbar_expect_tx(&S.full[s], bytes);
           const uint32_t bar = full0 + uint32_t(s * sizeof(uint64_t));
-          tma_load_2d_pair(&tmA, bar, S.a[s], kb * KE, m0, pol_a);
+          tma_load_2d_pair(map_a, bar, S.a[s], kb * KE, m0, pol_a);
           tma_load_2d_pair(map_b, bar, S.b[s], kb * KE, n0, pol_b);
         }
       }
@@ -1009,18 +1036,19 @@ gemm_pair_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap
 
 template <bool FP8>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
+gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmT,
+                 const __grid_constant__ CUtensorMap tmB, bf16* __restrict__ out, int64_t ldo, int M, int N, int K,
                  const float* __restrict__ sa, const float* __restrict__ sb,
-                 const bf16* __restrict__ bias) {
-  gemm_pair_body<FP8, false>(tmA, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0);
+                 const bf16* __restrict__ bias, int tail_rows) {
+  gemm_pair_body<FP8, false>(tmA, tmT, tmB, tmB, out, ldo, M, N, K, sa, sb, bias, 0, tail_rows);
 }
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_gated_pair_kernel(const __grid_constant__ CUtensorMap tmA,
+gemm_gated_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmT,
                        const __grid_constant__ CUtensorMap tmB1,
                        const __grid_constant__ CUtensorMap tmB2, bf16* __restrict__ out, int64_t ldo,
-                       int M, int N, int K, int act) {
-  gemm_pair_body<false, true>(tmA, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr, act);
+                       int M, int N, int K, int act, int tail_rows) {
+  gemm_pair_body<false, true>(tmA, tmT, tmB1, tmB2, out, ldo, M, N, K, nullptr, nullptr, nullptr, act,
+                              tail_rows);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1048,7 +1076,7 @@ static int make_map(CUtensorMap* m, const void* base, bool fp8, uint64_t inner, 
 static std::atomic<int> g_max_ctas{0};
 
 template <bool FP8, int BN>
-static int launch_bn(const CUtensorMap& ta, const void* B, int64_t ldb, void* out, int64_t ldo,
+static int launch_bn(const CUtensorMap& ta, const CUtensorMap& tt, const void* B, int64_t ldb, void* out, int64_t ldo,
                      int M, int N, int K, const float* sa, const float* sb, const void* bias,
                      cudaStream_t st) {
   CUtensorMap tb;
@@ -1061,8 +1089,9 @@ static int launch_bn(const CUtensorMap& ta, const void* B, int64_t ldb, void* ou
   const int lim = g_max_ctas.load(std::memory_order_relaxed);
   if (lim > 0 && lim < cap) cap = lim;
   dim3 grid((unsigned)(tiles < cap ? tiles : cap));
-  launch_kernel(gemm_kernel<FP8, BN>, dim3(grid), dim3(THREADS), smem, st, 0u, ta, tb, static_cast<bf16*>(out), ldo, M, N,
-                                                    K, sa, sb, static_cast<const bf16*>(bias));
+  launch_kernel(gemm_kernel<FP8, BN>, dim3(grid), dim3(THREADS), smem, st, 0u, ta, tt, tb,
+                static_cast<bf16*>(out), ldo, M, N, K, sa, sb, static_cast<const bf16*>(bias),
+                tail_box_rows(M));
   return check_launch(FP8 ? "gemm_kernel<e4m3>" : "gemm_kernel<bf16>");
 }
 
@@ -1106,7 +1135,7 @@ static int resident_clusters(int splits) {
 }
 
 template <bool FP8, int BN>
-static int launch_cluster(const CUtensorMap& ta, const void* B, int64_t ldb, void* out,
+static int launch_cluster(const CUtensorMap& ta, const CUtensorMap& tt, const void* B, int64_t ldb, void* out,
                           int64_t ldo, int M, int N, int K, const float* sa, const float* sb,
                           const void* bias, int splits, cudaStream_t st) {
   CUtensorMap tb;
@@ -1115,13 +1144,14 @@ static int launch_cluster(const CUtensorMap& ta, const void* B, int64_t ldb, voi
   if (!cluster_attr<FP8, BN>()) return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_cluster) failed");
   const int tiles = ((N + BN - 1) / BN) * ((M + BM - 1) / BM);
   launch_kernel(gemm_cluster_kernel<FP8, BN>, dim3((unsigned)splits, (unsigned)tiles, 1),
-                dim3(THREADS), cluster_smem<FP8, BN>(), st, (unsigned)splits, ta, tb,
-                static_cast<bf16*>(out), ldo, M, N, K, sa, sb, static_cast<const bf16*>(bias));
+                dim3(THREADS), cluster_smem<FP8, BN>(), st, (unsigned)splits, ta, tt, tb,
+                static_cast<bf16*>(out), ldo, M, N, K, sa, sb, static_cast<const bf16*>(bias),
+                tail_box_rows(M));
   return check_launch(FP8 ? "gemm_cluster_kernel<e4m3>" : "gemm_cluster_kernel<bf16>");
 }
 
 template <bool FP8>
-static int launch_pair(const CUtensorMap& ta, const void* B, int64_t ldb, void* out, int64_t ldo,
+static int launch_pair(const CUtensorMap& ta, const CUtensorMap& tt, const void* B, int64_t ldb, void* out, int64_t ldo,
                        int M, int N, int K, const float* sa, const float* sb, const void* bias,
                        cudaStream_t st) {
   CUtensorMap tb;
@@ -1177,8 +1207,8 @@ static int launch_pair(const CUtensorMap& ta, const void* B, int64_t ldb, void* 
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, gemm_pair_kernel<FP8>, ta, tb, static_cast<bf16*>(out), ldo, M, N, K,
-                     sa, sb, static_cast<const bf16*>(bias));
+  cudaLaunchKernelEx(&cfg, gemm_pair_kernel<FP8>, ta, tt, tb, static_cast<bf16*>(out), ldo, M, N, K,
+                     sa, sb, static_cast<const bf16*>(bias), tail_box_rows(M));
   return check_launch(FP8 ? "gemm_pair_kernel<e4m3>" : "gemm_pair_kernel<bf16>");
 }
 
@@ -1209,6 +1239,22 @@ static int resident(int bn, int splits) {
 // (BN, splits) that, in one resident wave of at most one CTA per SM, puts the
 // fewest operand bytes through any one SM ((BM + BN) x its K slice; ties: fewer
 // splits), each K slice at least two stages long.
+// Cycles that `tiles` tiles of 128 x bn (pair: 256 x 256 on an SM pair) take for a
+// step of 16 bf16 (32 e4m3) of K on `slots` SMs or pairs.  A tile's step: the
+// tensor pipe's 128 x bn products at 4096 a cycle, or its (128 + bn) 32-byte
+// operand rows at the some 72 bytes a cycle that an SM takes in, whichever is
+// longer (256 columns: 171, the 74% of the tensor rate seen there); a pair 141
+// (91%).  The power cap holds long runs at 1 / 1.36 of the clock, so a last wave
+// that is mostly empty costs less than it would at full clock.
+static long long tile_step(int bn) { return std::max(bn / 2, (BM + bn) * 32 / 72); }
+static long long steps(long long tiles, long long slots, int bn, bool pair) {
+  const long long step = pair ? 141 : tile_step(bn);
+  return std::max((tiles + slots - 1) / slots * step, tiles * step * 136 / (100 * slots));
+}
+static long long pair_steps(int M, int n_tiles) {
+  return steps((M + 2 * BM - 1) / (2 * BM) * (long long)n_tiles, num_sms() / 2, BN2, true);
+}
+
 template <bool FP8>
 static Plan plan(int M, int N, int K) {
   const long long mt = (M + BM - 1) / BM;
@@ -1228,6 +1274,12 @@ static Plan plan(int M, int N, int K) {
       }
     }
     if (pick != 0 && cost256 >= 0 && pick != 256 && 10 * pick_cost > 9 * cost256) pick = 256;
+    // Between the persistent kernels (same sums in the same order, so the same
+    // bits): the SM pairs where their waves are a tenth shorter.  M = 777 x 4096
+    // x 11008: 107 us with 128-column tiles, 65 us with pairs.
+    if (!FP8 && pick != 0 && M > BM && N >= BN2 &&
+        10 * pair_steps(M, (N + BN2 - 1) / BN2) <= 9 * steps(mt * ((N + pick - 1) / pick), sms, pick, false))
+      return {BN2, 0, true};
     if (pick != 0) return {pick, 0};
   }
   const int kblocks = K / (BKB / (FP8 ? 1 : 2));
@@ -1263,36 +1315,37 @@ static int launch(const void* A, int64_t lda, const void* B, int64_t ldb, void* 
   HB_REQUIRE((lda * (FP8 ? 1 : 2)) % 16 == 0 && (ldb * (FP8 ? 1 : 2)) % 16 == 0,
              "GEMM row strides must be multiples of 16 bytes");
   HB_REQUIRE(lda >= K && ldb >= K && ldo >= N, "GEMM leading dimensions too small");
-  CUtensorMap ta;
-  int rc = make_map(&ta, A, FP8, (uint64_t)K, (uint64_t)M, (uint64_t)lda, BM);
-  if (rc) return rc;
   const Plan pl = plan<FP8>(M, N, K);
-  if (pl.pair) return launch_pair<FP8>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
+  CUtensorMap ta, tt;
+  int rc = make_map(&ta, A, FP8, (uint64_t)K, (uint64_t)M, (uint64_t)lda, BM);
+  if (!rc) rc = make_map(&tt, A, FP8, (uint64_t)K, (uint64_t)M, (uint64_t)lda, (uint32_t)tail_box_rows(M));
+  if (rc) return rc;
+  if (pl.pair) return launch_pair<FP8>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
   if (pl.splits > 0) {
     switch (pl.bn) {
       case 256:
-        return launch_cluster<FP8, 256>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
+        return launch_cluster<FP8, 256>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
       case 192:
-        return launch_cluster<FP8, 192>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
+        return launch_cluster<FP8, 192>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
       case 128:
-        return launch_cluster<FP8, 128>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
+        return launch_cluster<FP8, 128>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
       default:
-        return launch_cluster<FP8, 64>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
+        return launch_cluster<FP8, 64>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, pl.splits, st);
     }
   }
   switch (pl.bn) {
-    case 256: return launch_bn<FP8, 256>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
-    case 192: return launch_bn<FP8, 192>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
-    case 128: return launch_bn<FP8, 128>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
-    case 64: return launch_bn<FP8, 64>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
-    default: return launch_bn<FP8, 32>(ta, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
+    case 256: return launch_bn<FP8, 256>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
+    case 192: return launch_bn<FP8, 192>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
+    case 128: return launch_bn<FP8, 128>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
+    case 64: return launch_bn<FP8, 64>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
+    default: return launch_bn<FP8, 32>(ta, tt, B, ldb, out, ldo, M, N, K, sa, sb, bias, st);
   }
 }
 
 // ---------------------------------------------------------------- gated launch
 template <int BN>
-static int launch_gated_bn(const CUtensorMap& ta, const CUtensorMap& t1, const CUtensorMap& t2,
-                           bf16* out, int64_t ldo, int M, int N, int K, int act, cudaStream_t st) {
+static int launch_gated_bn(const CUtensorMap& ta, const CUtensorMap& tt, const CUtensorMap& t1,
+                           const CUtensorMap& t2, bf16* out, int64_t ldo, int M, int N, int K, int act, cudaStream_t st) {
   const size_t smem = sizeof(Smem<BN>) + 1024;
   if (!smem_attr<gemm_gated_kernel<BN>>((int)smem))
     return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_gated) failed");
@@ -1301,26 +1354,27 @@ static int launch_gated_bn(const CUtensorMap& ta, const CUtensorMap& t1, const C
   const int lim = g_max_ctas.load(std::memory_order_relaxed);
   if (lim > 0 && lim < cap) cap = lim;
   launch_kernel(gemm_gated_kernel<BN>, dim3((unsigned)(tiles < cap ? tiles : cap)), dim3(THREADS),
-                smem, st, 0u, ta, t1, t2, out, ldo, M, N, K, act);
+                smem, st, 0u, ta, tt, t1, t2, out, ldo, M, N, K, act, tail_box_rows(M));
   return check_launch("gemm_gated_kernel");
 }
 
 template <int BN>
-static int launch_gated_cluster(const CUtensorMap& ta, const CUtensorMap& t1, const CUtensorMap& t2,
-                                bf16* out, int64_t ldo, int M, int N, int K, int act, int splits,
+static int launch_gated_cluster(const CUtensorMap& ta, const CUtensorMap& tt, const CUtensorMap& t1,
+                                const CUtensorMap& t2, bf16* out, int64_t ldo, int M, int N, int K, int act, int splits,
                                 cudaStream_t st) {
   const size_t smem = sizeof(SmemSK<BN>) + 1024;
   if (!smem_attr<gemm_gated_cluster_kernel<BN>>((int)smem))
     return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_gated_cluster) failed");
   const int tiles = ((N + BN / 2 - 1) / (BN / 2)) * ((M + BM - 1) / BM);
   launch_kernel(gemm_gated_cluster_kernel<BN>, dim3((unsigned)splits, (unsigned)tiles, 1),
-                dim3(THREADS), smem, st, (unsigned)splits, ta, t1, t2, out, ldo, M, N, K, act);
+                dim3(THREADS), smem, st, (unsigned)splits, ta, tt, t1, t2, out, ldo, M, N, K, act,
+                tail_box_rows(M));
   return check_launch("gemm_gated_cluster_kernel");
 }
 
 // Launched like gemm_pair_kernel: without programmatic serialisation.
-static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& t1, const CUtensorMap& t2,
-                             bf16* out, int64_t ldo, int M, int N, int K, int act,
+static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& tt, const CUtensorMap& t1,
+                             const CUtensorMap& t2, bf16* out, int64_t ldo, int M, int N, int K, int act,
                              cudaStream_t st) {
   const size_t smem = sizeof(Smem2) + 1024;
   if (!smem_attr<gemm_gated_pair_kernel>((int)smem))
@@ -1351,38 +1405,41 @@ static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& t1, const
   const int lim = g_max_ctas.load(std::memory_order_relaxed);
   if (lim > 0 && lim / 2 < cap) cap = lim / 2 > 0 ? lim / 2 : 1;
   cfg.gridDim = dim3((unsigned)(2 * (tiles < cap ? tiles : cap)));
-  cudaLaunchKernelEx(&cfg, gemm_gated_pair_kernel, ta, t1, t2, out, ldo, M, N, K, act);
+  cudaLaunchKernelEx(&cfg, gemm_gated_pair_kernel, ta, tt, t1, t2, out, ldo, M, N, K, act,
+                     tail_box_rows(M));
   return check_launch("gemm_gated_pair_kernel");
 }
 
-// Cost of a choice: operand bytes (rows of 128 B) through the busiest SM, i.e.
-// waves x (BM + BN) x K blocks of its slice.  One row tile (decode batches): the
-// cheapest of the cluster kernel's one-wave (BN, splits) and the persistent
-// kernel's BN (7B shape, 11008 outputs: BN 160 makes 138 tiles on 148 SMs).
+// The cheapest by `steps`: SM pairs, the persistent kernel's widths and,
+// for one row tile (decode batches), the cluster kernel's (BN, splits) that run in
+// one wave.  A wave of fewer tiles than SMs is bound by HBM there, so 160 columns
+// are among them: the 7B shape (11008 outputs) makes 138 tiles of 148, the 40B
+// shape (22528) 282 of 296.
 static Plan plan_gated(int M, int N, int K) {
   const long long mt = (M + BM - 1) / BM;
   const int sms = num_sms(), kblocks = K / (BKB / 2);
-  if (M >= PAIR_MIN_M && N >= BN2 / 2) return {BN2, 0, true};
+  auto tiles = [&](int bn) { return mt * ((N + bn / 2 - 1) / (bn / 2)); };
   Plan best = {0, 0};
   long long best_cost = 0;
-  for (int bn : {256, 192, 128, 64}) {
-    const long long tiles = mt * ((N + bn / 2 - 1) / (bn / 2));
-    const long long cost = ((tiles + sms - 1) / sms) * (BM + bn) * kblocks;
+  for (int bn : {256, 192, 160, 128, 64}) {
+    const long long cost = steps(tiles(bn), sms, bn, false) * kblocks;
     if (best.bn == 0 || cost < best_cost) {
       best = {bn, 0};
       best_cost = cost;
     }
   }
-  if (mt == 1) {
-    for (int bn : {256, 192, 160, 128, 64}) {
-      const long long tiles = (N + bn / 2 - 1) / (bn / 2);
-      for (int sp = 1; sp <= (bn >= 256 ? 3 : 4); ++sp) {
-        if (tiles * sp > sms || (sp > 1 && kblocks / sp < 2)) break;
-        const long long cost = (long long)(BM + bn) * ((kblocks + sp - 1) / sp);
-        if (cost < best_cost) {
-          best = {bn, sp};
-          best_cost = cost;
-        }
+  if (M > BM) {
+    if (100 * pair_steps(M, (N + BN2 / 2 - 1) / (BN2 / 2)) * kblocks <= 93 * best_cost)
+      return {BN2, 0, true};
+    return best;
+  }
+  for (int bn : {256, 192, 160, 128, 64}) {
+    for (int sp = 1; sp <= (bn >= 256 ? 3 : 4); ++sp) {
+      if (tiles(bn) * sp > sms || (sp > 1 && kblocks / sp < 2)) break;
+      const long long cost = tile_step(bn) * ((kblocks + sp - 1) / sp);
+      if (cost < best_cost || (cost == best_cost && best.splits == 0)) {
+        best = {bn, sp};
+        best_cost = cost;
       }
     }
   }
@@ -1405,26 +1462,28 @@ static int launch_gated(const void* A, int64_t lda, const void* B1, int64_t ldb1
              "gated GEMM leading dimensions too small");
   bf16* out = static_cast<bf16*>(outv);
   const Plan pl = plan_gated(M, N, K);
-  CUtensorMap ta, t1, t2;
+  CUtensorMap ta, tt, t1, t2;
   int rc = make_map(&ta, A, false, (uint64_t)K, (uint64_t)M, (uint64_t)lda, BM);
+  if (!rc) rc = make_map(&tt, A, false, (uint64_t)K, (uint64_t)M, (uint64_t)lda, (uint32_t)tail_box_rows(M));
   if (!rc) rc = make_map(&t1, B1, false, (uint64_t)K, (uint64_t)N, (uint64_t)ldb1, (uint32_t)pl.bn / 2);
   if (!rc) rc = make_map(&t2, B2, false, (uint64_t)K, (uint64_t)N, (uint64_t)ldb2, (uint32_t)pl.bn / 2);
   if (rc) return rc;
-  if (pl.pair) return launch_gated_pair(ta, t1, t2, out, ldo, M, N, K, act, st);
+  if (pl.pair) return launch_gated_pair(ta, tt, t1, t2, out, ldo, M, N, K, act, st);
   if (pl.splits > 0) {
     switch (pl.bn) {
-      case 256: return launch_gated_cluster<256>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
-      case 192: return launch_gated_cluster<192>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
-      case 160: return launch_gated_cluster<160>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
-      case 128: return launch_gated_cluster<128>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
-      default: return launch_gated_cluster<64>(ta, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      case 256: return launch_gated_cluster<256>(ta, tt, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      case 192: return launch_gated_cluster<192>(ta, tt, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      case 160: return launch_gated_cluster<160>(ta, tt, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      case 128: return launch_gated_cluster<128>(ta, tt, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
+      default: return launch_gated_cluster<64>(ta, tt, t1, t2, out, ldo, M, N, K, act, pl.splits, st);
     }
   }
   switch (pl.bn) {
-    case 256: return launch_gated_bn<256>(ta, t1, t2, out, ldo, M, N, K, act, st);
-    case 192: return launch_gated_bn<192>(ta, t1, t2, out, ldo, M, N, K, act, st);
-    case 128: return launch_gated_bn<128>(ta, t1, t2, out, ldo, M, N, K, act, st);
-    default: return launch_gated_bn<64>(ta, t1, t2, out, ldo, M, N, K, act, st);
+    case 256: return launch_gated_bn<256>(ta, tt, t1, t2, out, ldo, M, N, K, act, st);
+    case 160: return launch_gated_bn<160>(ta, tt, t1, t2, out, ldo, M, N, K, act, st);
+    case 192: return launch_gated_bn<192>(ta, tt, t1, t2, out, ldo, M, N, K, act, st);
+    case 128: return launch_gated_bn<128>(ta, tt, t1, t2, out, ldo, M, N, K, act, st);
+    default: return launch_gated_bn<64>(ta, tt, t1, t2, out, ldo, M, N, K, act, st);
   }
 }
 

@@ -24,6 +24,7 @@ namespace hb {
 
 constexpr int KV_THREADS = 256;
 constexpr int KV_MAX_HALF = 64;  // head_dim / 2
+constexpr int U = 2;             // items of a thread in flight
 
 struct KvAppendParams {
   hyena_kv_append_args a;
@@ -53,6 +54,42 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
   const int tid = (int)threadIdx.x;
   const int half = A.kv.head_dim / 2;
   const long long t0 = (long long)blockIdx.x * TB;
+  // ---- a batch's loads (the first one's before anything else: they wait for
+  // nothing but the previous kernel)
+  const int oct_bits = half == 64 ? 3 : 2;  // 8-element pieces of a half
+  const int hq = A.q != nullptr ? A.heads : 0, hkv = A.kv.kv_heads;
+  const int items = (hq + 2 * hkv) << oct_bits;  // of a token
+  const int all = (int)min((long long)TB, A.T - t0) * items;
+  uint4 a[U], b[U];
+  auto split = [&](int i, int& tok, int& h, int& oct) {
+    tok = 0;
+#pragma unroll
+    for (int k = 1; k < TB; ++k) tok += i >= k * items;
+    i -= tok * items;
+    h = i >> oct_bits;
+    oct = i - (h << oct_bits);
+  };
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * KV_THREADS;
+      if (i >= all) continue;
+      int tok, h, oct;
+      split(i, tok, h, oct);
+      const long long t = t0 + tok;
+      const bf16* src;
+      if (h < hq)
+        src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
+      else if (h < hq + hkv)
+        src = static_cast<const bf16*>(A.k) + t * A.k_token_stride + (h - hq) * A.k_head_stride;
+      else
+        src = static_cast<const bf16*>(A.v) + t * A.v_token_stride + (h - hq - hkv) * A.v_head_stride;
+      a[u] = *reinterpret_cast<const uint4*>(src + oct * 8);
+      b[u] = *reinterpret_cast<const uint4*>(src + half + oct * 8);
+    }
+  };
+  load(tid);
+
   if (tid < TB) {
     const long long t = t0 + tid;
     int ok = 0;
@@ -90,54 +127,29 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
   }
   __syncthreads();
 
-  const int oct_bits = half == 64 ? 3 : 2;  // 8-element pieces of a half
-  const int hq = A.q != nullptr ? A.heads : 0, hkv = A.kv.kv_heads;
-  const int items = (hq + 2 * hkv) << oct_bits;
-  constexpr int U = 4;
-  for (int i0 = tid; i0 < TB * items; i0 += U * KV_THREADS) {
-    uint4 a[U], b[U];
-    bf16* dst[U];
-    int oct[U], token[U];
-    bool turned[U];
+  for (int i0 = tid; i0 < all; i0 += U * KV_THREADS) {
+    if (i0 != tid) load(i0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      int i = i0 + u * KV_THREADS;
-      dst[u] = nullptr;
-      if (i >= TB * items) continue;
-      int tok = 0;
-#pragma unroll
-      for (int k = 1; k < TB; ++k) tok += i >= k * items;
+      const int i = i0 + u * KV_THREADS;
+      if (i >= all) continue;
+      int tok, h, oct;
+      split(i, tok, h, oct);
       if (!live[tok]) continue;
-      i -= tok * items;
-      token[u] = tok;
-      const long long t = t0 + tok;
-      int h = i >> oct_bits;
-      oct[u] = i - (h << oct_bits);
-      const bf16* src;
-      turned[u] = h < hq + hkv;
+      bf16* dst;
       if (h < hq) {
-        src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
-        dst[u] = static_cast<bf16*>(A.q_out) + t * A.q_out_token_stride + h * A.q_out_head_stride;
-      } else if (turned[u]) {
-        h -= hq;
-        src = static_cast<const bf16*>(A.k) + t * A.k_token_stride + h * A.k_head_stride;
-        if (koff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.k) + koff[tok] + h * A.kv.k_head_stride;
+        dst = static_cast<bf16*>(A.q_out) + (t0 + tok) * A.q_out_token_stride + h * A.q_out_head_stride;
+      } else if (h < hq + hkv) {
+        if (koff[tok] < 0) continue;
+        dst = static_cast<bf16*>(A.kv.k) + koff[tok] + (h - hq) * A.kv.k_head_stride;
       } else {
-        h -= hq + hkv;
-        src = static_cast<const bf16*>(A.v) + t * A.v_token_stride + h * A.v_head_stride;
-        if (voff[tok] >= 0) dst[u] = static_cast<bf16*>(A.kv.v) + voff[tok] + h * A.kv.v_head_stride;
+        if (voff[tok] < 0) continue;
+        dst = static_cast<bf16*>(A.kv.v) + voff[tok] + (h - hq - hkv) * A.kv.v_head_stride;
       }
-      if (dst[u] == nullptr) continue;
-      a[u] = *reinterpret_cast<const uint4*>(src + oct[u] * 8);
-      b[u] = *reinterpret_cast<const uint4*>(src + half + oct[u] * 8);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (dst[u] == nullptr) continue;
-      if (turned[u]) {
+      if (h < hq + hkv) {
         uint32_t* aw = reinterpret_cast<uint32_t*>(&a[u]);
         uint32_t* bw = reinterpret_cast<uint32_t*>(&b[u]);
-        const float4* tab = reinterpret_cast<const float4*>(&cs[token[u]][oct[u] * 8]);
+        const float4* tab = reinterpret_cast<const float4*>(&cs[tok][oct * 8]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float4 r = tab[w];  // cos, sin of two pairs
@@ -146,8 +158,8 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
           bw[w] = as_u32(pack2_rn(make_float2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w)));
         }
       }
-      *reinterpret_cast<uint4*>(dst[u] + oct[u] * 8) = a[u];
-      *reinterpret_cast<uint4*>(dst[u] + half + oct[u] * 8) = b[u];
+      *reinterpret_cast<uint4*>(dst + oct * 8) = a[u];
+      *reinterpret_cast<uint4*>(dst + half + oct * 8) = b[u];
     }
   }
 }

@@ -280,6 +280,16 @@ def test_many_samples_of_one_prompt():
     b.check(b.call(**sharing((150, 3000))))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 32, 128), (32, 32, 64), (64, 8, 128)])
+@pytest.mark.parametrize("samples,shared", [(18, 4100), (64, 3000), (150, 2050), (40, 1024), (64, 1024),
+                                            (128, 1024), (128, 520), (300, 1024)])
+def test_long_shared_runs(heads, kv_heads, dim, samples, shared):
+    """Chunks of several key tiles, few and many rows, many heads."""
+    reqs = [(1, shared + 1 + 3 * (i % 5)) for i in range(samples)]
+    b = Batch(reqs, heads, kv_heads, dim, page=64, groups=[(range(samples), shared)])
+    b.check(b.call(**sharing((samples, shared))))
+
+
 def test_sharing_is_only_a_hint():
     """A shared run longer than a member's keys is cut to what all see; requests
     outside every group have their own keys only; a padded first member (no keys,
