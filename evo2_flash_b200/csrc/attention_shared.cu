@@ -62,7 +62,7 @@ struct __align__(1024) TcSmem {
   uint8_t ring[Tc<D, NT>::SLOTS][Tc<D, NT>::TILE_BYTES];
   uint64_t full[Tc<D, NT>::SLOTS], empty[Tc<D, NT>::SLOTS];
   uint64_t q_full;
-  uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT];  // [..][score buffer]
+  uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT], o_done[NT];  // [..][score buffer]
   uint32_t bad[8];  // 16-key blocks of a tile whose page is out of range
   uint32_t tmem;
   unsigned long long best[16];
@@ -147,6 +147,7 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
         mbar_init(&S.p_full[t][b], 128);
       }
       mbar_init(&S.pv_done[t], 1);
+      mbar_init(&S.o_done[t], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -294,6 +295,8 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
 #pragma unroll
         for (int ks = 0; ks < TILE_KEYS / 16; ++ks)
           mma_ts(d, p + ks * 8, sw128_mn_desc(v + ks * 2048, T::HALF_BYTES), ID_O, acc || ks != 0);
+        // waited for only where O is rescaled, at most one product behind: a parity
+        // tells no more than neighbours apart, so the item's end has o_done
         mma_commit(&S.pv_done[t]);
       };
       auto slot_full = [&](uint32_t slot_u) {
@@ -326,6 +329,7 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
             if (!ok) break;
             fence_after();
             values(t, gi, u + 1, i != 0);
+            if (!more) mma_commit(&S.o_done[t]);
             if (t == NT - 1) mma_commit(&S.empty[(u + 1) % T::SLOTS]);
             if constexpr (NT > 1) {
               if (more) {
@@ -347,7 +351,7 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     const float scale = P.scale == 0.0f ? 1.0f : fabsf(P.scale);
     const uint2 sign = query_sign(P.scale);
     const int slots = P.slots_s + P.slots;
-    uint32_t gi = 0;
+    uint32_t gi = 0, n_item = 0;
     bool ok = true;
     for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x) {
       const Item I = item_of<D, NT>(P, S, item);
@@ -382,32 +386,74 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
         fence_after();
         if (active) {
           const uint32_t scol = tmem + lanes + T::S_COL + uint32_t((T::NBUF == 2 ? b : t) * TILE_KEYS);
-          uint32_t x[TILE_KEYS];
-#pragma unroll
-          for (int c = 0; c < TILE_KEYS / 32; ++c)
-            tmem_ld32_async(scol + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
-          tmem_wait_ld();
           const int keys = I.k1 - (I.k0 + i * TILE_KEYS);
           const uint32_t bad = S.bad[gi & 7];
-          if (keys < TILE_KEYS || bad != 0) {
+          const bool partial = keys < TILE_KEYS || bad != 0;
+          uint32_t x[2][32], p[TILE_KEYS / 2];
+          // The next 32 scores are on their way from TMEM while these are used.
+          auto scores = [&](auto&& use) {
+            tmem_ld32_async(scol, x[0]);
 #pragma unroll
-            for (int j = 0; j < TILE_KEYS; ++j)
-              if (j >= keys || ((bad >> (j / BOX_MIN)) & 1u)) x[j] = 0xff800000u;  // -inf
-          }
-          float top[4];
+            for (int c = 0; c < TILE_KEYS / 32; ++c) {
+              tmem_wait_ld();
+              tmem_settle(x[c & 1]);
+              if (c + 1 < TILE_KEYS / 32) tmem_ld32_async(scol + (c + 1) * 32, x[(c + 1) & 1]);
+              if (partial) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) top[k] = __uint_as_float(x[k]);
+                for (int j = 0; j < 32; ++j)
+                  if (c * 32 + j >= keys || ((bad >> ((c * 32 + j) / BOX_MIN)) & 1u))
+                    x[c & 1][j] = 0xff800000u;  // -inf
+              }
+              use(c, x[c & 1]);
+            }
+          };
+          auto set_m = [&]() {  // m: the row's largest score of this tile
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            scores([&](int, const uint32_t (&v)[32]) {
 #pragma unroll
-          for (int j = 4; j < TILE_KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(x[j]));
-          float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-          if (mx != mx) mx = -INFINITY;  // 0 * inf: the row's NaN comes from its weights
-          const bool grow = mx > m + RESCALE_LOG2 || (m == -INFINITY && mx > m);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float mn = grow ? mx : m;
-            const float keep = grow ? exp2_approx(m - mn) : 1.0f;
-            m = mn;
-            l *= keep;
-            if (i > 0) {
+              for (int j = 0; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(v[j]));
+            });
+            return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+          };
+          float part;      // sum of the weights
+          bf162 most;      // their largest, in pairs
+          auto weights = [&]() {
+            const float base = m == -INFINITY ? 0.0f : m;
+            const f2 sc2 = f2_make(scale, scale), nb2 = f2_make(-base, -base);
+            f2 sum[2] = {f2_make(0.0f, 0.0f), f2_make(0.0f, 0.0f)};
+            bf162 big[2] = {as_bf162(0u), as_bf162(0u)};
+            scores([&](int c, const uint32_t (&v)[32]) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float2 y =
+                    f2_split(f2_fma(f2_make(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), sc2, nb2));
+                const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                sum[(j >> 1) & 1] = f2_add(sum[(j >> 1) & 1], f2_make(w.x, w.y));
+                const bf162 r = pack2_rn(w);
+                big[(j >> 1) & 1] = __hmax2(big[(j >> 1) & 1], r);
+                p[c * 16 + j / 2] = as_u32(r);
+              }
+            });
+            const float2 a = f2_split(f2_add(sum[0], sum[1]));
+            part = a.x + a.y;
+            most = __hmax2(big[0], big[1]);
+          };
+          if (i == 0) m = set_m();
+          weights();
+          if (i > 0) {
+            // Weights above 2^RESCALE_LOG2 (the rows' m is that far behind): the rare
+            // tile where m moves, O and l follow, and the weights are made again.
+            const float2 big = unpack2(most);
+            const bool grow = fmaxf(big.x, big.y) > exp2_approx(RESCALE_LOG2) || (m == -INFINITY && part > 0.0f);
+            if (__any_sync(0xffffffffu, grow)) {
+              float keep = 1.0f;
+              const float mx = set_m();
+              if (grow) {
+                keep = exp2_approx(m - mx);
+                m = mx;
+              }
+              l *= keep;
+              weights();
               ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
               if (!ok) break;
               fence_after();
@@ -422,36 +468,17 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
               }
             }
           }
-          const float base = m == -INFINITY ? 0.0f : m;
-          const f2 sc2 = f2_make(scale, scale), nb2 = f2_make(-base, -base);
-          f2 sum[2] = {f2_make(0.0f, 0.0f), f2_make(0.0f, 0.0f)};
-#pragma unroll
-          for (int h = 0; h < TILE_KEYS; h += 64) {
-            uint32_t p[32];
-#pragma unroll
-            for (int j = h; j < h + 64; j += 2) {
-              const float2 y = f2_split(
-                  f2_fma(f2_make(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), sc2, nb2));
-              const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-              sum[(j >> 1) & 1] = f2_add(sum[(j >> 1) & 1], f2_make(w.x, w.y));
-              p[(j - h) / 2] = as_u32(pack2_rn(w));
-            }
-            tmem_st32(scol + h / 2, p);
-          }
-          const float2 a = f2_split(f2_add(sum[0], sum[1]));
-          l += a.x + a.y;
+          l += part;
+          tmem_st32(scol, p);
+          tmem_st32(scol + 32, p + 32);
           tmem_wait_st();
         }
-        // Every phase of pv_done is seen in turn, since a parity tells only
-        // neighbours apart: with two score buffers the product before last is known
-        // to be complete here, the last one need not be (it ran under this softmax).
-        if (gi > 0) ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
-        if (!ok) break;
         fence_before();
         mbar_arrive(&S.p_full[t][b]);
       }
       if (!ok) break;
-      ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
+      ok = __all_sync(0xffffffffu, wait(&S.o_done[t], n_item & 1, A.error_flags));
+      ++n_item;
       if (!ok) break;
       fence_after();
       if (active) {
