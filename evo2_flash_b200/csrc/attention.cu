@@ -40,8 +40,8 @@ constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int ROWS = 16;        // rows of a unit
 constexpr int STAGES = 3;       // tiles in flight per warp
-constexpr int MIN_TILES = 4;    // tiles of an item, and how many items a warp should get
-constexpr int ITEMS_PER_WARP = 8;
+constexpr int MIN_TILES = 2;     // tiles of an item at least
+constexpr int ITEMS_PER_WARP = 8;  // that a warp should get
 constexpr int MAX_SEGMENTS = 2048;
 constexpr int TC_MIN_ROWS = 16;  // mean rows of a group and key/value head
 
@@ -107,10 +107,16 @@ __device__ void make_plan(const Params& P, Plan& L) {
     work += wsum[w];
     longest = max(longest, wlong[w]);
   }
-  // at most P.slots items a unit
-  const long long want = (long long)gridDim.x * (WARPS * ITEMS_PER_WARP);
-  const long long even = (work + want - 1) / want;
-  L.chunk = (int)max(max(even, (long long)ceil_div(longest, P.slots)), (long long)MIN_TILES);
+  // Some ITEMS_PER_WARP items a warp, for balance; but an item has its start and
+  // leaves a piece to be joined (each of its rows 8 D bytes there and back, as much
+  // as D / 16 of a tile), so not below 8 tiles and one for each of its rows while
+  // every warp still gets one; at most P.slots items a unit.
+  const int warps = (int)gridDim.x * WARPS;
+  const long long even = (work + (long long)warps * ITEMS_PER_WARP - 1) / ((long long)warps * ITEMS_PER_WARP);
+  const long long each = (work + warps - 1) / warps;
+  const int mean_rows = min(P.a.T / max(P.a.num_requests, 1) * P.per, ROWS);
+  const long long few = min(each, (long long)(8 + mean_rows));
+  L.chunk = (int)max(max(even, few), (long long)max(ceil_div(longest, P.slots), MIN_TILES));
   int sum = 0;
   for (int s = s0; s < s1; ++s) {
     const int4 x = L.info[s];
@@ -252,6 +258,10 @@ stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
+  }
   pdl_entry();
   Plan L;
   L.info = reinterpret_cast<int4*>(smem + LT::PLAN);
@@ -269,7 +279,7 @@ stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
   uint8_t* ring = smem + warp * LT::RING;
   const uint32_t ring_u = su32(ring);
   const int g8 = lane >> 2, t4 = lane & 3;
-  const int warps = (int)gridDim.x * WARPS, first = warp * (int)gridDim.x + (int)blockIdx.x;
+  const int warps = (int)gridDim.x * WARPS, first = (int)blockIdx.x * WARPS + warp;
   if (first >= L.items) return;
 
   // ---- loads, STAGES - 1 tiles ahead; a lane holds the page of one of 32
@@ -718,8 +728,10 @@ static int launch(const hyena_paged_attention_args& A, const Slots& S, void* ws,
   int rc = cache_map(&map_k, A.kv, true, KT);
   if (!rc) rc = cache_map(&map_v, A.kv, false, KT);
   if (rc) return rc;
+  // each launch is checked before the next, which reads what it leaves
   launch_kernel(stream_kernel<D>, dim3((unsigned)(2 * num_sms())), dim3(THREADS), smem, st, 0u, P, map_k,
                 map_v);
+  if ((rc = check_launch("paged_attention"))) return rc;
   if (P.tc && (rc = shared_launch(P, map_k, map_v, st))) return rc;
   // a block a row while those fill one wave of 16 blocks an SM
   if (rows <= 16ll * num_sms())

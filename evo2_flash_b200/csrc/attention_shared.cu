@@ -160,13 +160,17 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
   }
 
   // ---- plan: the chunk length (in tiles) that lets the CTAs finish soonest,
-  // waves x (tiles of an item + its overhead), over the chunk counts of the
-  // longest run; then the groups' first items
+  // waves x (tiles of an item + its overhead) and the pieces to be joined, over the
+  // chunk counts of the longest run; then the groups' first items
   shared_runs<T::THREADS>(P, S.shared, S.leader);
   {
     int longest = 0;
     for (int g = 0; g < G; ++g) longest = max(longest, S.shared[g]);
     const int most = ceil_div(longest, TILE_KEYS);
+    // joining: a piece of every query row, there and back, in sixteenths of a tile's
+    // time (some 13 MB of memory traffic for two row tiles, 8 MB for one)
+    const unsigned long long piece = (unsigned long long)((long long)A.T * A.heads * (D + 2)) * 8 * 16 /
+                                     (NT == 1 ? 8000000u : 13000000u);
     unsigned long long best = ~0ull;
     for (int c = tid + 1; c <= P.slots_s && c <= max(most, 1); c += T::THREADS) {
       const int n = max(ceil_div(most, c), 1);
@@ -177,8 +181,8 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
         items += (long long)ceil_div(rows, NT * 128) * hkv *
                  ceil_div(ceil_div(S.shared[g], TILE_KEYS), n);
       }
-      const unsigned long long cost = (unsigned long long)((items + gridDim.x - 1) / gridDim.x) *
-                                      (unsigned long long)(n + ITEM_OVERHEAD);
+      const unsigned long long waves = (unsigned long long)((items + gridDim.x - 1) / gridDim.x);
+      const unsigned long long cost = 16 * waves * (unsigned long long)(n + ITEM_OVERHEAD) + c * piece;
       best = min(best, (cost << 24) | (unsigned long long)min(n, (1 << 24) - 1));
     }
 #pragma unroll

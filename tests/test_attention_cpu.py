@@ -107,7 +107,7 @@ def test_workspace_is_bounded(lib):
     """The plan, and a few pieces a row: at most what the pages hold, and 256 MB
     beyond the plan while one piece a row allows it."""
     size = lambda **kw: lib.hyena_paged_attention_workspace_size(C.byref(attention_args(**kw)))  # noqa: E731
-    assert size(kv_pages_per_request=8) == 256 + 3 * 4 * 2 * 130 * 4  # 128 keys: two pieces a row
+    assert size(kv_pages_per_request=8) == 256 + 3 * 4 * 4 * 130 * 4  # 128 keys: four pieces a row
     assert size(kv_pages_per_request=1, shared_lens=4096, num_groups=1) == 256 + 3 * 4 * 2 * 130 * 4
     assert size(kv_pages_per_request=1) == 256 + 3 * 4 * 130 * 4
     for T in (1, 64, 1024):
