@@ -99,7 +99,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ uint2 query_sign(float scale) {
   return make_uint2(scale < 0.0f ? 0x80008000u : 0u, scale == 0.0f ? 0u : 0xffffffffu);
 }
-// O is rescaled when a score exceeds the m it is scaled by by more than this.
+// O is rescaled when weights reach 2^RESCALE_LOG2: below it bf16 and fp32 round
+// as well as at 1.
 constexpr float RESCALE_LOG2 = 8.0f;
 constexpr unsigned long long WAIT_NS = 4000000000ull;  // 4 s
 

@@ -15,8 +15,8 @@
 //                values take turns in one ring
 // Every row sees every key of the run, so only the run's last tile has a mask.
 //
-// O is rescaled only when a row's maximum has grown by more than 2^8 since the m
-// it is scaled by: the weights then stay below 2^8, where bf16 and fp32 round as
+// O is rescaled only when the weights of a row's tile sum to more than 2^8, its
+// scores having outgrown the m it is scaled by: the weights stay below 2^8, where bf16 and fp32 round as
 // well as at 1, and the pass over O's columns (TMEM -> registers -> TMEM) is rare
 // instead of once a tile.  m and l leave with the piece, so nothing is lost.
 //
@@ -31,6 +31,7 @@
 // thread waits at its end instead, so that the join kernel, which waits for this
 // one, finds both complete.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 
@@ -282,11 +283,11 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
       auto score = [&](int t, uint32_t no, uint32_t slot_u) {  // S_t of tile `no`
         const int b = T::NBUF == 2 ? (no & 1) : 0;
         const uint32_t d = tmem + T::S_COL + uint32_t((T::NBUF == 2 ? b : t) * TILE_KEYS);
-        const uint8_t* k = S.ring[slot_u % T::SLOTS];
+        const uint64_t q = sw128_desc(S.q[t]), k = sw128_desc(S.ring[slot_u % T::SLOTS]);
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const int off = (ks / 4) * T::HALF_BYTES + (ks % 4) * 32;
-          mma_ss(d, sw128_desc(S.q[t] + off), sw128_desc(k + off), ID_S, ks != 0);
+        for (int ks = 0; ks < D / 16; ++ks) {  // (addresses in descriptors count 16 bytes)
+          const uint64_t off = ((ks / 4) * T::HALF_BYTES + (ks % 4) * 32) / 16;
+          mma_ss(d, q + off, k + off, ID_S, ks != 0);
         }
         mma_commit(&S.s_full[t][b]);
         mbar_arrive(&S.s_full[t][b]);  // passes on what the loading warp wrote for the tile
@@ -295,10 +296,10 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
         const int b = T::NBUF == 2 ? (no & 1) : 0;
         const uint32_t p = tmem + T::S_COL + uint32_t((T::NBUF == 2 ? b : t) * TILE_KEYS);
         const uint32_t d = tmem + T::O_COL + uint32_t(t * D);
-        const uint8_t* v = S.ring[slot_u % T::SLOTS];
+        const uint64_t v = sw128_mn_desc(S.ring[slot_u % T::SLOTS], T::HALF_BYTES);
 #pragma unroll
         for (int ks = 0; ks < TILE_KEYS / 16; ++ks)
-          mma_ts(d, p + ks * 8, sw128_mn_desc(v + ks * 2048, T::HALF_BYTES), ID_O, acc || ks != 0);
+          mma_ts(d, p + ks * 8, v + ks * (2048 / 16), ID_O, acc || ks != 0);
         // waited for only where O is rescaled, at most one product behind: a parity
         // tells no more than neighbours apart, so the item's end has o_done
         mma_commit(&S.pv_done[t]);
@@ -395,14 +396,16 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
           const bool partial = keys < TILE_KEYS || bad != 0;
           uint32_t x[2][32], p[TILE_KEYS / 2];
           // The next 32 scores are on their way from TMEM while these are used.
-          auto scores = [&](auto&& use) {
+          // (Tiles with a mask have code of their own: a branch a chunk keeps the
+          // compiler from overlapping the chunks.)
+          auto scores = [&](auto masked, auto&& use) {
             tmem_ld32_async(scol, x[0]);
 #pragma unroll
             for (int c = 0; c < TILE_KEYS / 32; ++c) {
               tmem_wait_ld();
               tmem_settle(x[c & 1]);
               if (c + 1 < TILE_KEYS / 32) tmem_ld32_async(scol + (c + 1) * 32, x[(c + 1) & 1]);
-              if (partial) {
+              if constexpr (decltype(masked)::value) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                   if (c * 32 + j >= keys || ((bad >> ((c * 32 + j) / BOX_MIN)) & 1u))
@@ -413,51 +416,46 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
           };
           auto set_m = [&]() {  // m: the row's largest score of this tile
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            scores([&](int, const uint32_t (&v)[32]) {
+            scores(std::true_type{}, [&](int, const uint32_t (&v)[32]) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(v[j]));
             });
             return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
           };
           float part;      // sum of the weights
-          bf162 most;      // their largest, in pairs
-          auto weights = [&]() {
+          auto weights = [&](auto masked) {
             const float base = m == -INFINITY ? 0.0f : m;
             const f2 sc2 = f2_make(scale, scale), nb2 = f2_make(-base, -base);
             f2 sum[2] = {f2_make(0.0f, 0.0f), f2_make(0.0f, 0.0f)};
-            bf162 big[2] = {as_bf162(0u), as_bf162(0u)};
-            scores([&](int c, const uint32_t (&v)[32]) {
+            scores(masked, [&](int c, const uint32_t (&v)[32]) {
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 const float2 y =
                     f2_split(f2_fma(f2_make(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), sc2, nb2));
                 const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                 sum[(j >> 1) & 1] = f2_add(sum[(j >> 1) & 1], f2_make(w.x, w.y));
-                const bf162 r = pack2_rn(w);
-                big[(j >> 1) & 1] = __hmax2(big[(j >> 1) & 1], r);
-                p[c * 16 + j / 2] = as_u32(r);
+                p[c * 16 + j / 2] = as_u32(pack2_rn(w));
               }
             });
             const float2 a = f2_split(f2_add(sum[0], sum[1]));
             part = a.x + a.y;
-            most = __hmax2(big[0], big[1]);
           };
           if (i == 0) m = set_m();
-          weights();
+          if (partial) weights(std::true_type{});
+          else weights(std::false_type{});
           if (i > 0) {
-            // Weights above 2^RESCALE_LOG2 (the rows' m is that far behind): the rare
+            // A sum above 2^RESCALE_LOG2 (the row's m is that far behind): the rare
             // tile where m moves, O and l follow, and the weights are made again.
-            const float2 big = unpack2(most);
-            const bool grow = fmaxf(big.x, big.y) > exp2_approx(RESCALE_LOG2) || (m == -INFINITY && part > 0.0f);
+            const bool grow = part > exp2_approx(RESCALE_LOG2) || (m == -INFINITY && part > 0.0f);
             if (__any_sync(0xffffffffu, grow)) {
               float keep = 1.0f;
               const float mx = set_m();
-              if (grow) {
+              if (grow && mx > m) {
                 keep = exp2_approx(m - mx);
                 m = mx;
               }
               l *= keep;
-              weights();
+              weights(std::true_type{});
               ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
               if (!ok) break;
               fence_after();
