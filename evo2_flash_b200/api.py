@@ -380,6 +380,9 @@ class Evo2:
         (evo2_flash/api.py:839-982): the prompts are prefilled in packed steps,
         then every step decodes one token per prompt from the paged mixer state
         and the attention cache.  `seed` seeds prompt i's sampler with seed + i.
+        With the model's native_blocks, a prompt given several times (samples of one
+        prompt) is prefilled once: the others fork its state and share the pages of
+        its keys and values, which every step then reads once for all of them.
         `cached_generation` and `force_prompt_threshold` are accepted and
         ignored (decoding always continues from the cached state)."""
         _sampling_args(temperature, top_k, top_p)
@@ -398,27 +401,49 @@ class Evo2:
         gens = [None if seed is None else torch.Generator().manual_seed(seed + i)
                 for i in range(len(ids))]
         m = self.model
+        # row of the decode steps -> prompt; sequence of a prompt
+        rows, sid = list(range(len(ids))), list(range(len(ids)))
+        prompts, source = ids, {}
+        if getattr(m, "cache", None) is not None:
+            first = {}
+            for i, x in enumerate(ids):
+                first.setdefault(tuple(x), []).append(i)
+            groups = list(first.values())
+            rows = [i for g in groups for i in g]  # samples of a prompt side by side
+            prompts = [ids[g[0]] for g in groups]
+            extra = len(groups)
+            for u, g in enumerate(groups):
+                sid[g[0]] = u
+                for i in g[1:]:
+                    sid[i] = extra
+                    source[extra] = u
+                    extra += 1
         last = [None] * len(ids)
         with torch.no_grad():
-            for h, segs in m.prefill_steps([torch.tensor(x, dtype=torch.long) for x in ids],
-                                           self.max_tokens_per_step, keep_cache=True):
-                for a, b, sid, p0 in segs:
-                    if p0 + (b - a) == len(ids[sid]):
-                        last[sid] = h[b - 1]
-            h = torch.stack(last)
+            for h, segs in m.prefill_steps([torch.tensor(x, dtype=torch.long) for x in prompts],
+                                           self.max_tokens_per_step, keep_cache=True,
+                                           state_blocks=len(ids) + 1):
+                for a, b, j, p0 in segs:
+                    if p0 + (b - a) == len(prompts[j]):
+                        last[j] = h[b - 1]
+            for copy, u in source.items():
+                m.fork(u, copy, len(prompts[u]))
+                last[copy] = last[u]
+            h = torch.stack([last[sid[i]] for i in rows])
             toks = [[] for _ in ids]
             lps = [[] for _ in ids]
             try:
                 for step in range(n_tokens):
                     lg = F.linear(h, m.embed).float()
                     lp = torch.log_softmax(lg, -1)
-                    nxt = [sample_token(lg[i], temperature, top_k, top_p, gens[i])
-                           for i in range(len(ids))]
-                    for i, t in enumerate(nxt):
+                    nxt = [sample_token(lg[r], temperature, top_k, top_p, gens[i])
+                           for r, i in enumerate(rows)]
+                    for r, (i, t) in enumerate(zip(rows, nxt)):
                         toks[i].append(t)
-                        lps[i].append(float(lp[i, t]))
+                        lps[i].append(float(lp[r, t]))
                     if step + 1 < n_tokens:
-                        h = m.decode_step(nxt, [len(x) + step for x in ids], range(len(ids)))
+                        h = m.decode_step(nxt, [len(ids[i]) + step for i in rows],
+                                          [sid[i] for i in rows])
             finally:
                 m.release_all()
         seqs = [self.tokenizer.detokenize(t) for t in toks]

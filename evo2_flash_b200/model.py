@@ -15,7 +15,11 @@ plain torch, since the engine is not part of this path):
                        (model.py:200-245, 335-356)
 
 Hyena layers are `HyenaFIRMixer` / `HyenaIIRMixer` from this package (the hot
-path); attention, MLP and norms are torch ops (outside the mixer path).
+path); attention, MLP and norms are torch ops (outside the mixer path).  With
+`StripedHyena2Config.native_blocks` the attention layers keep their keys and values
+in a paged cache (kv_cache.py) that ops.kv_append fills and, for steps of few tokens
+a sequence, ops.paged_attention reads, and the MLP is ops.gated_mlp: fewer roundings
+than the torch ops, so results differ from theirs in the last bits.
 `score` runs teacher-forced prefill over packed varlen steps -- a long sequence
 may be split across steps, which exercises the mixers' state continuation -- and
 returns each sequence's mean -log p(x_t | x_<t) over t >= 1 with an fp32
@@ -33,6 +37,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .forward_context import set_forward_metadata
+from .kv_cache import PagedKVCache, PagedStep
 
 
 @dataclass
@@ -56,6 +61,7 @@ class StripedHyena2Config:
     rope_theta: float = 10000.0
     use_fp8_input_projections: bool = True
     extra: dict = field(default_factory=dict)
+    native_blocks: bool = False  # attention cache, decode attention and MLP on this package's kernels
 
     @classmethod
     def evo2_7b(cls, **kw):
@@ -130,8 +136,9 @@ class Evo2RMSNorm(nn.Module):
 
 
 class Evo2MLP(nn.Module):
-    def __init__(self, hidden, inner, use_act, device=None):
+    def __init__(self, hidden, inner, use_act, device=None, native=False):
         super().__init__()
+        self.native = native
         kw = dict(bias=False, device=device, dtype=torch.bfloat16)
         self.l1 = nn.Linear(hidden, inner, **kw)
         self.l2 = nn.Linear(hidden, inner, **kw)
@@ -141,6 +148,12 @@ class Evo2MLP(nn.Module):
             p.requires_grad_(False)
 
     def forward(self, x):
+        # (a hook on a projection, as the embedding names use, wants its own output)
+        if self.native and not any(m._forward_hooks for m in (self.l1, self.l2, self.l3)):
+            from . import ops
+
+            return ops.gated_mlp(x, self.l1.weight, self.l2.weight, self.l3.weight,
+                                 "gelu" if self.use_act else "none")
         z1 = self.l1(x)
         if self.use_act:
             z1 = F.gelu(z1)
@@ -158,12 +171,19 @@ def _rope_neox(x, positions, theta):
     return torch.cat([a * cos - b * sin, b * cos + a * sin], -1).to(x.dtype)
 
 
+# Steps of at most this many new tokens a sequence attend over the paged cache;
+# longer ones (prompts) through torch's attention on the sequence's gathered pages.
+PAGED_ATTENTION_TOKENS = 64
+
+
 class Evo2Attention(nn.Module):
     """MHA with RoPE over packed segments; keys/values of sequences that continue
-    in a later step are kept in `self.kv[seq_id]`."""
+    in a later step are kept in `self.kv[seq_id]`, or, when the segments come as a
+    PagedStep, in layer `index` of its cache."""
 
-    def __init__(self, cfg, device=None):
+    def __init__(self, cfg, device=None, index=0):
         super().__init__()
+        self.index = index
         h = cfg.hidden_size
         self.heads = cfg.num_attention_heads
         self.hd = h // self.heads
@@ -174,8 +194,34 @@ class Evo2Attention(nn.Module):
             p.requires_grad_(False)
         self.kv = {}
 
+    def _paged(self, q, k, v, step):
+        from . import ops
+
+        k_cache, v_cache = step.cache.layer(self.index)
+        q = ops.kv_append(q, k, v, step.positions, k_cache, v_cache, step.table, step.starts,
+                          rope_theta=self.theta)
+        if step.longest <= PAGED_ATTENTION_TOKENS:
+            return ops.paged_attention(q, k_cache, v_cache, step.table, step.seq_lens, step.starts,
+                                       **step.shared)
+        out = torch.empty_like(q)
+        for i, (a, b, _, p0) in enumerate(step):
+            n = p0 + b - a
+            pages = step.table[i, :-(-n // step.cache.page_size)].long()
+            ks, vs = (t[pages].flatten(0, 1)[:n].transpose(0, 1)[None] for t in (k_cache, v_cache))
+            mask = None
+            if p0:
+                mask = (torch.arange(n, device=q.device)[None]
+                        <= torch.arange(p0, n, device=q.device)[:, None])
+            o = F.scaled_dot_product_attention(q[a:b].transpose(0, 1)[None], ks, vs, attn_mask=mask,
+                                               is_causal=not p0, scale=self.hd ** -0.5)
+            out[a:b] = o[0].transpose(0, 1)
+        return out
+
     def forward(self, x, positions, segments):
         q, k, v = self.qkv_proj(x).split(x.shape[-1], dim=-1)
+        if isinstance(segments, PagedStep):
+            out = self._paged(*(t.unflatten(-1, (self.heads, self.hd)) for t in (q, k, v)), segments)
+            return self.o_proj(out.reshape(x.shape[0], -1))
         q = _rope_neox(q.view(-1, self.heads, self.hd), positions, self.theta)
         k = _rope_neox(k.view(-1, self.heads, self.hd), positions, self.theta)
         v = v.view(-1, self.heads, self.hd)
@@ -217,11 +263,12 @@ class Evo2DecoderLayer(nn.Module):
         self.pre_norm = Evo2RMSNorm(h, cfg.rms_norm_eps, device)
         self.post_norm = Evo2RMSNorm(h, cfg.rms_norm_eps, device)
         if self.kind == "attn":
-            self.mixer = Evo2Attention(cfg, device)
+            self.mixer = Evo2Attention(cfg, device, sorted(cfg.attn_layer_idxs).index(i))
         else:
             k = cfg.inner_filter_length(i) if self.kind != "hcl" else 0
             self.mixer = mixer_factory(cfg, i, self.kind, k, f"layers.{i}.mixer", device)
-        self.mlp = Evo2MLP(h, cfg.intermediate_size, use_act=(i == 0), device=device)
+        self.mlp = Evo2MLP(h, cfg.intermediate_size, use_act=(i == 0), device=device,
+                           native=cfg.native_blocks)
 
     def forward(self, x, positions, segments, add=None, input_ids=None):
         """One block (model.py:190-198) on the residual stream x, which it updates
@@ -256,6 +303,15 @@ class StripedHyena2(nn.Module):
         self.layers = nn.ModuleList(Evo2DecoderLayer(cfg, i, device, factory)
                                     for i in range(cfg.num_hidden_layers))
         self.norm = Evo2RMSNorm(h, cfg.rms_norm_eps, device)
+        self.cache = None
+        if cfg.native_blocks:
+            head_dim = h // cfg.num_attention_heads
+            if self.device.type != "cuda":
+                raise ValueError("native_blocks needs a CUDA device")
+            if head_dim not in (64, 128):
+                raise ValueError(f"native_blocks needs heads of 64 or 128, got {head_dim}")
+            self.cache = PagedKVCache(len(cfg.attn_layer_idxs), cfg.num_attention_heads, head_dim,
+                                      device=self.device)
 
     # ---- weights --------------------------------------------------------------
     def random_tensors(self, seed=0, gen_device="cpu", input_scale=8.0 / 448.0):
@@ -325,6 +381,8 @@ class StripedHyena2(nn.Module):
         chunk in the step.  `block_outputs`: a dict whose integer keys name
         blocks; each gets that block's output residual stream (m + x + mlp,
         the reference's block output, model.py:189-198) as a new tensor."""
+        if self.cache is not None and len(segments):
+            segments = self.cache.step(segments, positions)
         x = self.embed[input_ids]
         add = None
         with set_forward_metadata(meta):
@@ -339,7 +397,8 @@ class StripedHyena2(nn.Module):
         return torch.log_softmax(logits, -1).gather(1, targets[:, None]).squeeze(1)
 
     @torch.no_grad()
-    def prefill_steps(self, seqs, max_tokens_per_step=None, block_outputs=None, keep_cache=False):
+    def prefill_steps(self, seqs, max_tokens_per_step=None, block_outputs=None, keep_cache=False,
+                      state_blocks=None):
         """Teacher-forced prefill of `seqs` (1-D int token tensors) packed in
         order into steps of at most `max_tokens_per_step` tokens (default: all
         in one step); a sequence that does not fit finishes in later steps from
@@ -348,16 +407,15 @@ class StripedHyena2(nn.Module):
         keep_cache the attention entries stay after the last step, so that
         decode_step can continue the sequences (else each is dropped once its
         sequence is done).  Yields (h, segments) per step: h (rows, H) after
-        the final norm.
+        the final norm.  `state_blocks`: mixer state blocks to allocate (default: one
+        a sequence and the null block), for sequences that fork adds later.
         `block_outputs` (a set of block indices) adds a third item, the dict of
         those blocks' outputs for the step's rows."""
         dev = self.device
         lens = [int(s.numel()) for s in seqs]
         budget = max_tokens_per_step or max(1, sum(lens))
-        self.allocate_state(len(seqs) + 1)
-        for layer in self.layers:
-            if layer.kind == "attn":
-                layer.mixer.kv.clear()
+        self.allocate_state(state_blocks or len(seqs) + 1)
+        self.release_all()
         done = [0] * len(seqs)
         nxt = 0
         while nxt < len(seqs) and lens[nxt] == 0:
@@ -383,9 +441,7 @@ class StripedHyena2(nn.Module):
             for a, b, sid, p0 in segs:
                 done[sid] = p0 + (b - a)
                 if done[sid] == lens[sid] and not keep_cache:
-                    for layer in self.layers:
-                        if layer.kind == "attn":
-                            layer.mixer.release(sid)
+                    self.release(sid)
             while nxt < len(seqs) and done[nxt] == lens[nxt]:
                 nxt += 1
 
@@ -463,9 +519,7 @@ class StripedHyena2(nn.Module):
             for a, b, sid, p0 in segs:
                 done[sid] = p0 + (b - a)
                 if done[sid] == lens[sid]:
-                    for layer in self.layers:
-                        if layer.kind == "attn":
-                            layer.mixer.release(sid)
+                    self.release(sid)
             while nxt < len(seqs) and done[nxt] == lens[nxt]:
                 nxt += 1
         return [-s / c if c else math.nan for s, c in zip(sums, cnt)]
@@ -483,8 +537,31 @@ class StripedHyena2(nn.Module):
         meta = _decode_meta([int(sid) + 1 for sid in seq_ids], dev)
         return self(ids, pos.to(dev), meta, segs)
 
+    def fork(self, src, dst, length):
+        """Sequence `dst` becomes a copy of sequence `src`, whose first `length` tokens
+        have been run: its mixer states are copied, its attention keys and values
+        shared (native_blocks) until either continues in the same page."""
+        for layer in self.layers:
+            if layer.kind != "attn":
+                for t in layer.mixer.kv_cache:
+                    t[dst + 1] = t[src + 1]
+            elif self.cache is None:
+                layer.mixer.kv[dst] = layer.mixer.kv[src]
+        if self.cache is not None:
+            self.cache.fork(src, dst, length)
+
+    def release(self, sid):
+        """Drops a sequence's attention key/value cache."""
+        for layer in self.layers:
+            if layer.kind == "attn":
+                layer.mixer.release(sid)
+        if self.cache is not None:
+            self.cache.release(sid)
+
     def release_all(self):
         """Drops every sequence's attention key/value cache."""
+        if self.cache is not None:
+            self.cache.clear()
         for layer in self.layers:
             if layer.kind == "attn":
                 layer.mixer.kv.clear()

@@ -635,7 +635,7 @@ def kv_append(q, k, v, positions, k_cache, v_cache, page_table, query_start_loc=
             raise ValueError(f"q has {n} tokens, k {T}")
         heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty((T, heads, dim), dtype=BF16, device=k.device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             out_token, out_head = heads * dim, dim
         else:
             n, out_token, out_head = _rows3(q_out, "q_out", heads, dim)
@@ -708,7 +708,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
     elif group_start is not None:
         raise ValueError("group_start without shared_lens")
     if out is None:
-        out = torch.empty((T, heads, dim), dtype=BF16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         out_token, out_head = heads * dim, dim
     else:
         n, out_token, out_head = _rows3(out, "out", heads, dim)
@@ -724,8 +724,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
     lib = _lib.load()
     with _On(device) as stream:
         n = lib.hyena_paged_attention_workspace_size(args)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        rc = lib.hyena_paged_attention(args, 0 if ws is None else ws.data_ptr(), n, stream)
+        ws = q.new_empty(n // 2)  # bf16 elements
+        rc = lib.hyena_paged_attention(args, ws.data_ptr(), n, stream)
     del table  # alive until the launch returned
     if rc:
         _lib.check(rc, "hyena_paged_attention")

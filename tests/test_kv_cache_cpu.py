@@ -1,0 +1,121 @@
+"""The paged key/value cache's host bookkeeping, on the CPU: page tables, growth,
+forks with copy on write, and the shared runs it reports."""
+
+import pytest
+import torch
+
+from evo2_flash_b200.kv_cache import PagedKVCache
+
+
+def cache(page=16, layers=2):
+    return PagedKVCache(layers, heads=2, head_dim=4, page_size=page, device="cpu", dtype=torch.float32)
+
+
+def write(c, table, row, positions, value):
+    for i in range(c.layers):
+        k, v = c.layer(i)
+        for p in positions:
+            k[table[row, p // c.page_size], p % c.page_size] = value + p + 1000 * i
+            v[table[row, p // c.page_size], p % c.page_size] = -(value + p)
+
+
+def read(c, table, row, n, layer=0):
+    k, _ = c.layer(layer)
+    return torch.stack([k[table[row, p // c.page_size], p % c.page_size] for p in range(n)])[:, 0, 0]
+
+
+def test_pages_follow_the_lengths_and_come_back():
+    c = cache()
+    c.extend(0, 0, 40)
+    c.extend(1, 0, 16)
+    table, shared = c.table([0, 1])
+    assert table.shape == (2, 3) and table.dtype == torch.int32 and shared == {}
+    used = table[0].tolist() + table[1, :1].tolist()
+    assert len(set(used)) == 4
+    c.extend(1, 16, 17)
+    assert c.table([1])[0].shape == (1, 2)
+    c.release(0)
+    c.extend(2, 0, 33)  # freed pages are used again
+    assert set(c.table([2])[0][0].tolist()) <= set(range(16))
+    with pytest.raises(ValueError, match="cannot continue"):
+        c.extend(2, 60, 61)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        cache(page=24)
+
+
+def test_growth_keeps_what_is_stored():
+    c = cache()
+    c.extend(0, 0, 30)
+    write(c, c.table([0])[0], 0, range(30), 5.0)
+    before = read(c, c.table([0])[0], 0, 30)
+    c.extend(1, 0, 16 * 100)
+    assert c.layer(0)[0].shape[0] >= 102
+    assert torch.equal(read(c, c.table([0])[0], 0, 30), before)
+    assert torch.equal(read(c, c.table([0])[0], 0, 30, layer=1), before + 1000)
+
+
+def test_beginning_anew_releases_the_old_pages():
+    c = cache()
+    for _ in range(50):
+        c.extend(0, 0, 160)
+    assert c.layer(0)[0].shape[0] <= 32
+
+
+def test_fork_shares_until_written():
+    c = cache()
+    n = 40  # two whole pages and half of one
+    c.extend(0, 0, n)
+    write(c, c.table([0])[0], 0, range(n), 0.0)
+    c.fork(0, 1, n)
+    c.fork(0, 2, n)
+    table, shared = c.table([0, 1, 2])
+    assert torch.equal(table[0], table[1]) and torch.equal(table[0], table[2])
+    assert shared["shared_lens"].tolist() == [48] and shared["group_start"].tolist() == [0, 3]
+    c.extend(1, n, n + 1)  # writes into the third page: its own copy
+    table, shared = c.table([0, 1, 2])
+    assert torch.equal(table[0, :2], table[1, :2]) and table[0, 2] != table[1, 2]
+    assert torch.equal(table[0], table[2])
+    assert shared["shared_lens"].tolist() == [32]
+    write(c, table, 1, [n], 500.0)
+    assert torch.equal(read(c, table, 1, n), read(c, table, 0, n))
+    c.extend(0, n, n + 1)
+    c.extend(2, n, n + 1)
+    assert len(set(c.table([0, 1, 2])[0][:, 2].tolist())) == 3
+    c.release(0)  # the others keep the shared pages
+    assert torch.equal(read(c, c.table([2])[0], 0, n), torch.arange(n, dtype=torch.float32))
+    with pytest.raises(ValueError, match="fewer"):
+        c.fork(1, 3, 1000)
+
+
+def test_shared_runs_of_several_groups():
+    c = cache()
+    for s, n in ((0, 64), (10, 20), (20, 33)):
+        c.extend(s, 0, n)
+    for d in (1, 2):
+        c.fork(0, d, 64)
+    c.fork(20, 21, 33)
+    order = [0, 1, 2, 10, 20, 21]
+    _, shared = c.table(order)
+    assert shared["group_start"].tolist() == [0, 3, 4, 6]
+    assert shared["shared_lens"].tolist() == [64, 0, 48]
+    assert c.table([10, 0])[1] == {}
+    assert c.table([1, 10, 2])[1] == {}  # not side by side: nothing read together
+
+
+def test_step_arguments():
+    c = cache()
+    step = c.step([(0, 3, 5, 0), (3, 5, 7, 0)], torch.arange(5))
+    assert list(step) == [(0, 3, 5, 0), (3, 5, 7, 0)]
+    assert step.starts.tolist() == [0, 3, 5] and step.seq_lens.tolist() == [3, 2]
+    assert step.longest == 3 and step.positions.dtype == torch.int32
+    step = c.step([(0, 1, 5, 3), (1, 2, 7, 2)], torch.tensor([3, 2]))
+    assert step.starts is None and step.seq_lens.tolist() == [4, 3] and step.longest == 1
+
+
+def test_native_blocks_need_cuda_and_a_head_size():
+    from evo2_flash_b200.model import StripedHyena2, StripedHyena2Config
+    from tests.helpers import OracleMixer
+
+    with pytest.raises(ValueError, match="CUDA"):
+        StripedHyena2(StripedHyena2Config.small(hidden=128, native_blocks=True), device="cpu",
+                      mixer_factory=OracleMixer)
