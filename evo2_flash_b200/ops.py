@@ -497,22 +497,24 @@ def _same_device(names, *tensors):
     """The index of the one CUDA device that the given tensors (None: absent) are
     on; refuses others, and tensors that need a gradient: these operators have no
     backward pass."""
-    device = None
+    device = tensors[0].get_device()
     grad = torch.is_grad_enabled()
-    for i, t in enumerate(tensors):
+    for t in tensors:
+        if t is not None and (t.get_device() != device or (grad and t.requires_grad)):
+            break
+    else:
+        if device >= 0:
+            return device
+    for name, t in zip(names.split(), tensors):
         if t is None:
             continue
-        d = t.get_device()
-        if d < 0:
-            raise ValueError(f"{names.split()[i]} must be a CUDA tensor")
-        if device is None:
-            device = d
-        elif d != device:
-            raise ValueError(f"{names.split()[i]} is on cuda:{d}, not on cuda:{device}")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if t.get_device() != device:
+            raise ValueError(f"{name} is on {t.device}, not on {tensors[0].device}")
         if grad and t.requires_grad:
-            raise ValueError(f"{names.split()[i]} requires grad: this operator has no backward pass "
+            raise ValueError(f"{name} requires grad: this operator has no backward pass "
                              "(call it under torch.no_grad())")
-    return device
 
 
 class _On:
@@ -552,8 +554,9 @@ def _rows3(t, name, heads, dim):
 
 def _ints(t, name, at_least):
     """A 1-D contiguous int32 tensor (converted if need be) of at least `at_least` elements."""
-    if t.dim() != 1 or t.shape[0] < at_least:
-        raise ValueError(f"{name} must be 1-D with at least {at_least} elements, got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 1 or shape[0] < at_least:
+        raise ValueError(f"{name} must be 1-D with at least {at_least} elements, got {tuple(shape)}")
     if t.dtype is not torch.int32:
         if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
             raise ValueError(f"{name} must hold integers, got {t.dtype}")
@@ -561,35 +564,34 @@ def _ints(t, name, at_least):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _cache_shape(k_cache, v_cache):
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.dim() != 4 or t.dtype is not BF16 or t.stride(3) != 1:
-            raise ValueError(f"{name} must be (pages, page size, kv heads, head_dim) bf16 with unit "
-                             f"last stride, got {tuple(t.shape)} {t.dtype}")
-    shape = k_cache.shape
-    if shape != v_cache.shape:
+def _paged_kv(k_cache, v_cache, page_table, requests):
+    """The fields of hyena_paged_kv, and the page table they point to (None requests:
+    as many as the table has rows)."""
+    shape, k_strides, v_strides = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if (len(shape) != 4 or v_cache.shape != shape or k_cache.dtype is not BF16
+            or v_cache.dtype is not BF16 or k_strides[3] != 1 or v_strides[3] != 1):
+        for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if t.dim() != 4 or t.dtype is not BF16 or t.stride(3) != 1:
+                raise ValueError(f"{name} must be (pages, page size, kv heads, head_dim) bf16 with unit "
+                                 f"last stride, got {tuple(t.shape)} {t.dtype}")
         raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)} differ")
-    return shape
-
-
-def _paged_kv(k_cache, v_cache, shape, page_table, requests):
-    """The fields of hyena_paged_kv, and the page table they point to."""
-    if page_table.dim() != 2 or page_table.shape[0] < requests or page_table.is_floating_point():
-        raise ValueError(f"page_table must be (>= {requests} requests, pages) int, "
-                         f"got {tuple(page_table.shape)} {page_table.dtype}")
-    row, one = page_table.stride()
-    if page_table.dtype is not torch.int32 or (one != 1 and page_table.shape[1] > 1):
-        page_table = page_table.to(torch.int32).contiguous()
-        row = page_table.stride(0)
-    kp, kt, kh, _ = k_cache.stride()
-    vp, vt, vh, _ = v_cache.stride()
-    pages, _, heads, _ = shape
+    kp, kt, kh, _ = k_strides
+    vp, vt, vh, _ = v_strides
+    pages, size, heads, dim = shape
     if pages == 1:
         kp = vp = 0
     if heads == 1:
         kh = vh = 0
+    table = page_table.shape
+    if len(table) != 2 or (requests is not None and table[0] < requests) or page_table.is_floating_point():
+        raise ValueError(f"page_table must be (>= {requests or 0} requests, pages) int, "
+                         f"got {tuple(table)} {page_table.dtype}")
+    row, one = page_table.stride()
+    if page_table.dtype is not torch.int32 or (one != 1 and table[1] > 1):
+        page_table = page_table.to(torch.int32).contiguous()
+        row = page_table.stride(0)
     return (k_cache.data_ptr(), v_cache.data_ptr(), kp, kt, kh, vp, vt, vh, page_table.data_ptr(), row,
-            page_table.shape[1], *shape), page_table
+            table[1], pages, size, heads, dim), page_table
 
 
 def _flags_ptr(error_flags):
@@ -621,8 +623,14 @@ def kv_append(q, k, v, positions, k_cache, v_cache, page_table, query_start_loc=
     device = _same_device("k v positions k_cache v_cache page_table q query_start_loc q_out error_flags",
                           k, v, positions, k_cache, v_cache, page_table, q, query_start_loc, q_out,
                           error_flags)
-    shape = _cache_shape(k_cache, v_cache)
-    kv_heads, dim = shape[2], shape[3]
+    requests, starts = None, 0
+    if query_start_loc is not None:
+        query_start_loc = _ints(query_start_loc, "query_start_loc", 1)
+        requests, starts = query_start_loc.shape[0] - 1, query_start_loc.data_ptr()
+    kv, table = _paged_kv(k_cache, v_cache, page_table, requests)
+    if requests is None:
+        requests = table.shape[0]
+    kv_heads, dim = kv[13], kv[14]
     T, k_token, k_head = _rows3(k, "k", kv_heads, dim)
     n, v_token, v_head = _rows3(v, "v", kv_heads, dim)
     if n != T:
@@ -645,13 +653,6 @@ def kv_append(q, k, v, positions, k_cache, v_cache, page_table, query_start_loc=
     elif q_out is not None:
         raise ValueError("q_out without q")
     positions = _ints(positions, "positions", T)
-    requests = page_table.shape[0]
-    starts = 0
-    if query_start_loc is not None:
-        query_start_loc = _ints(query_start_loc, "query_start_loc", 1)
-        requests = query_start_loc.shape[0] - 1
-        starts = query_start_loc.data_ptr()
-    kv, table = _paged_kv(k_cache, v_cache, shape, page_table, requests)
     if T == 0 or requests == 0:
         return q_out
     args = _KV_APPEND.pack(q_ptr, q_token, q_head, out_ptr, out_token, out_head, k.data_ptr(), k_token,
@@ -687,12 +688,12 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
     device = _same_device("q k_cache v_cache page_table seq_lens query_start_loc shared_lens group_start "
                           "out error_flags", q, k_cache, v_cache, page_table, seq_lens, query_start_loc,
                           shared_lens, group_start, out, error_flags)
-    shape = _cache_shape(k_cache, v_cache)
-    dim = shape[3]
-    T, q_token, q_head = _rows3(q, "q", None, dim)
-    heads = q.shape[1]
     seq_lens = _ints(seq_lens, "seq_lens", 0)
     requests = seq_lens.shape[0]
+    kv, table = _paged_kv(k_cache, v_cache, page_table, requests)
+    dim = kv[14]
+    T, q_token, q_head = _rows3(q, "q", None, dim)
+    heads = q.shape[1]
     starts = shared = group = groups = 0
     if query_start_loc is not None:
         query_start_loc = _ints(query_start_loc, "query_start_loc", requests + 1)
@@ -714,7 +715,6 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
         n, out_token, out_head = _rows3(out, "out", heads, dim)
         if n != T:
             raise ValueError(f"out has {n} tokens, q {T}")
-    kv, table = _paged_kv(k_cache, v_cache, shape, page_table, requests)
     if T == 0 or requests == 0:
         return out
     args = _PAGED_ATTENTION.pack(
