@@ -1411,8 +1411,9 @@ static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& tt, const
 }
 
 // The cheapest by `steps`: SM pairs, the persistent kernel's widths and,
-// for one row tile (decode batches), the cluster kernel's (BN, splits) that run in
-// one wave.  A wave of fewer tiles than SMs is bound by HBM there, so 160 columns
+// for one row tile (decode batches), the cluster kernel's (BN, splits) of one wave,
+// which cut K where the tiles alone leave SMs idle (one split measures as the
+// persistent kernel).  A wave is bound by HBM there, so 160 columns
 // are among them: the 7B shape (11008 outputs) makes 138 tiles of 148, the 40B
 // shape (22528) 282 of 296.
 static Plan plan_gated(int M, int N, int K) {
@@ -1434,10 +1435,10 @@ static Plan plan_gated(int M, int N, int K) {
     return best;
   }
   for (int bn : {256, 192, 160, 128, 64}) {
-    for (int sp = 1; sp <= (bn >= 256 ? 3 : 4); ++sp) {
-      if (tiles(bn) * sp > sms || (sp > 1 && kblocks / sp < 2)) break;
+    for (int sp = 2; sp <= (bn >= 256 ? 3 : 4); ++sp) {
+      if (tiles(bn) * sp > sms || kblocks / sp < 2) break;
       const long long cost = tile_step(bn) * ((kblocks + sp - 1) / sp);
-      if (cost < best_cost || (cost == best_cost && best.splits == 0)) {
+      if (cost < best_cost) {
         best = {bn, sp};
         best_cost = cost;
       }
