@@ -12,15 +12,17 @@
 // Work.  A segment is either the shared keys of a group, seen by every query of
 // its requests, or the own keys of one request; a unit is a segment x key/value
 // head x 16-row tile (rows = queries x heads of one key/value head), and an item
-// is `chunk` 16-key tiles of a unit.  Warps take items in turn, those of a
-// segment ordered by position, then head: the warps of the GPU sweep through the
-// cache together, a page's heads at about the same time.  (Giving each warp one
-// long run of tiles instead evens the work out exactly, but spreads the warps
-// over the whole cache: 343 us instead of 3XX for 32 requests of up to 8000
-// keys, the memory's pages and translations being hit at random.)  A warp's
-// loads run on across its items.  Every length is read on the device (one
-// captured graph serves growing contexts), so each CTA first derives the same
-// list from them, a prefix sum over segments.
+// is `chunk` 16-key tiles of a unit.  A segment's items are ordered by position,
+// then head, and warps take them one after the other: the warps of the GPU sweep
+// through the cache together, a page's heads at about the same time.  (Giving each
+// warp one long run of tiles instead evens the work out exactly, but spreads the
+// warps over the whole cache: 343 us instead of 331 for 32 requests of up to 8000
+// keys, items being taken in turn in both.)  A warp's loads run on across its
+// items.  Every length is read on the device (one captured graph serves growing
+// contexts), and the list of items with it, a prefix sum over segments: by
+// plan_kernel, which the warps then ask for their next item (305 us for the 32
+// requests: an SM that is further from the memory takes fewer), or, where the items
+// are few, by each CTA, its warps taking them in turn.
 //
 // `shared_lens` says what may be read once, never what is seen: a group's
 // shared run is cut to what every query of the group sees and to whole 16-key
@@ -40,10 +42,18 @@ constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int ROWS = 16;        // rows of a unit
 constexpr int STAGES = 3;       // tiles in flight per warp
+constexpr int QUEUE = 8;        // items between a warp's loads and its products, at most STAGES
 constexpr int MIN_TILES = 2;     // tiles of an item at least
 constexpr int ITEMS_PER_WARP = 8;  // that a warp should get
 constexpr int MAX_SEGMENTS = 2048;
 constexpr int TC_MIN_ROWS = 16;  // mean rows of a group and key/value head
+// Without a shared kernel, plan_kernel plans from this many requests and bytes of keys
+// and values (as many as their page tables can name) on, else each CTA for itself, its
+// warps taking items in turn.  With the plan kernel and without: one request of 777
+// keys 17.5 and 11.5 us; 32 heads, 16 requests of 1024 keys (0.27 GB) 57 and 55 us, 8
+// of 8192 (1.07 GB) 172 and 176 us, 32 of up to 8000 (2.0 GB) 305 and 331 us.
+constexpr int PLANNED_REQUESTS = 5;
+constexpr long long PLANNED_BYTES = 512ll << 20;
 
 struct Plan {
   int chunk;   // tiles of an item
@@ -64,14 +74,16 @@ __device__ __forceinline__ int own_tiles(int len, int k_begin) {
 }
 
 // Every thread of the CTA.
+template <int NTHREADS>
 __device__ void make_plan(const Params& P, Plan& L) {
-  __shared__ long long wsum[WARPS];
-  __shared__ int wlong[WARPS], wfirst[WARPS];
+  constexpr int W = NTHREADS / 32;
+  __shared__ long long wsum[W];
+  __shared__ int wlong[W], wfirst[W];
   const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = P.groups, n = G + P.a.num_requests;
-  shared_runs<THREADS>(P, L.shared, L.leader);
+  shared_runs<NTHREADS>(P, L.shared, L.leader);
   // a thread takes a run of consecutive segments
-  const int per = ceil_div(n, THREADS);
+  const int per = ceil_div(n, NTHREADS);
   const int s0 = min(tid * per, n), s1 = min(s0 + per, n);
   auto tiles_of = [&](int s, const int4& x) { return s < G ? x.z / KT : own_tiles(x.z, x.w); };
   long long work = 0;
@@ -103,7 +115,7 @@ __device__ void make_plan(const Params& P, Plan& L) {
   __syncthreads();
   work = 0;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
+  for (int w = 0; w < W; ++w) {
     work += wsum[w];
     longest = max(longest, wlong[w]);
   }
@@ -111,7 +123,7 @@ __device__ void make_plan(const Params& P, Plan& L) {
   // leaves a piece to be joined (each of its rows 8 D bytes there and back, as much
   // as D / 16 of a tile), so not below 8 tiles and one for each of its rows while
   // every warp still gets one; at most P.slots items a unit.
-  const int warps = (int)gridDim.x * WARPS;
+  const int warps = P.warps;
   const long long even = (work + (long long)warps * ITEMS_PER_WARP - 1) / ((long long)warps * ITEMS_PER_WARP);
   const long long each = (work + warps - 1) / warps;
   const int mean_rows = min(P.a.T / max(P.a.num_requests, 1) * P.per, ROWS);
@@ -133,7 +145,7 @@ __device__ void make_plan(const Params& P, Plan& L) {
   __syncthreads();
   int at = scan - sum, total = 0;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w < warp) at += wfirst[w];
     total += wfirst[w];
   }
@@ -141,6 +153,25 @@ __device__ void make_plan(const Params& P, Plan& L) {
   if (tid == 0) L.first[n] = total;
   L.items = total;
   __syncthreads();
+}
+
+// The plan in a kernel of its own: one CTA instead of every CTA of the stream
+// kernel, and the counter from which that kernel's warps then take their items (an
+// SM that is far from its memory, or busy with the shared kernel, takes fewer).
+constexpr int PLAN_THREADS = 256;
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constant__ Params P) {
+  pdl_entry();
+  Plan L{0, 0, P.first, P.info, P.shared, P.leader};
+  make_plan<PLAN_THREADS>(P, L);
+  if (threadIdx.x == 0) {
+    P.head[SHARED_TILES] = P.head[CHUNK] = L.chunk;
+    P.head[ITEMS] = L.items;
+    P.head[NEXT] = 0;
+  }
+  if (P.tc) {
+    plan_shared<PLAN_THREADS>(P, P.shared, P.tc_first, P.head + TC_TILES);
+    if (threadIdx.x == 0) P.head[SHARED_TILES] = P.head[TC_TILES] * (TILE_KEYS / KT);
+  }
 }
 
 // ---------------------------------------------------------------- fragments
@@ -240,13 +271,14 @@ __device__ __forceinline__ Item item_at(const Params& P, const Plan& L, int item
 // tile), masks only in the tiles that need them, and a maximum that is compared
 // by one vote: m moves, and O is rescaled, only when a score exceeds it by 2^8
 // (the weights stay below 2^8, where bf16 and fp32 round as well as at 1).
-template <int D>
+template <int D, bool PLANNED>
 __global__ void __launch_bounds__(THREADS, 2)
 stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensorMap map_k,
               const __grid_constant__ CUtensorMap map_v) {
   using LT = Layout<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_s[WARPS][STAGES];
+  __shared__ int queue_s[WARPS][PLANNED ? QUEUE : 1];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   const hyena_paged_attention_args& A = P.a;
@@ -262,31 +294,57 @@ stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
   }
-  pdl_entry();
+  if (PLANNED && P.tc == 2)
+    pdl_trigger();  // the plan is complete: see attention_shared.cu
+  else
+    pdl_entry();
   Plan L;
   L.info = reinterpret_cast<int4*>(smem + LT::PLAN);
   L.first = reinterpret_cast<int*>(L.info + (G + B));
   L.shared = reinterpret_cast<int*>(L.first + (G + B + 1));
   L.leader = L.shared + G;
-  make_plan(P, L);
-  if (blockIdx.x == 0) {  // for the join
-    if (tid == 0) {
-      if (!P.tc) P.plan[0] = L.chunk * KT;
-      P.plan[1] = L.chunk;
+  if (PLANNED) {
+    for (int i = tid; i <= G + B; i += THREADS) {
+      L.first[i] = __ldcg(P.first + i);
+      if (i < G + B) L.info[i] = __ldcg(P.info + i);
     }
-    for (int g = tid; g < G; g += THREADS) P.plan[2 + g] = L.shared[g];
+    L.chunk = __ldcg(P.head + CHUNK);
+    L.items = __ldcg(P.head + ITEMS);
+    __syncthreads();
+  } else {
+    make_plan<THREADS>(P, L);
+    if (blockIdx.x == 0) {  // for the join
+      if (tid == 0 && !P.tc) P.head[SHARED_TILES] = L.chunk;
+      if (tid == 0) P.head[CHUNK] = L.chunk;
+      for (int g = tid; g < G; g += THREADS) P.shared[g] = L.shared[g];
+    }
   }
   uint8_t* ring = smem + warp * LT::RING;
   const uint32_t ring_u = su32(ring);
   const int g8 = lane >> 2, t4 = lane & 3;
-  const int warps = (int)gridDim.x * WARPS, first = (int)blockIdx.x * WARPS + warp;
-  if (first >= L.items) return;
+  // Items in turn; or from the counter, the next one asked for when the loads of one
+  // begin, and a queue that passes them on from the loads to the products.
+  int* queue = queue_s[warp];
+  const int first = (int)blockIdx.x * WARPS + warp;
+  int asked = 0;
+  auto ask = [&]() {
+    if (lane == 0) asked = atomicAdd(P.head + NEXT, 1);
+  };
+  if (PLANNED) ask();
+  int next = PLANNED ? __shfl_sync(0xffffffffu, asked, 0) : first;
+  if (next >= L.items) {
+    if (PLANNED && P.tc == 2) pdl_wait();
+    return;
+  }
+  if (PLANNED) {
+    if (lane == 0) queue[0] = next;
+    ask();
+  }
 
   // ---- loads, STAGES - 1 tiles ahead; a lane holds the page of one of 32
   // consecutive page-table entries
-  int next = first;                       // the item being loaded
-  Item N = item_at(P, L, next, -1);
-  int tile = 0, page_at = 0, page_index = 0, window = -64, window_of = -1, pages = 0;
+  Item N = item_at(P, L, next, -1);  // the item being loaded
+  int loaded = 0, tile = 0, page_at = 0, page_index = 0, window = -64, window_of = -1, pages = 0;
   uint32_t bad = 0;  // stages whose page is out of range
   int load_stage = 0;
   page_index = N.k0 / kv.page_size;
@@ -329,8 +387,14 @@ stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     }
     if (++tile == N.n) {
       tile = 0;
-      next += warps;
+      if (PLANNED) {
+        next = __shfl_sync(0xffffffffu, asked, 0);
+        if (lane == 0) queue[++loaded % QUEUE] = next;
+      } else {
+        next += P.warps;
+      }
       if (next < L.items) {
+        if (PLANNED) ask();
         N = item_at(P, L, next, N.seg);
         page_index = N.k0 / kv.page_size;
         page_at = N.k0 - page_index * kv.page_size;
@@ -347,7 +411,10 @@ stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
   int s = 0, seg = -1;
   uint32_t parity = 0;
 #pragma unroll 1
-  for (int item = first; item < L.items; item += warps) {
+  for (int k = 0;; ++k) {
+    if (PLANNED) __syncwarp();
+    const int item = PLANNED ? queue[k % QUEUE] : first + k * P.warps;
+    if (item >= L.items) break;
     const Item U = item_at(P, L, item, seg);
     seg = U.seg;
     const bool two = U.rows - U.row0 > 8;  // rows 8-15 exist
@@ -376,170 +443,170 @@ stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
 
 #pragma unroll 1
     for (int i_tile = 0; i_tile < U.n; ++i_tile) {
-    load();
-    const int kpos = U.k0 + i_tile * KT;
-    if (!__all_sync(0xffffffffu, wait(&full[s], parity, A.error_flags))) {
-      // gave up: what else was issued lands (waits bounded too) before the warp leaves
-      for (int k = 1; k < STAGES; ++k) {
-        if (++s == STAGES) {
-          s = 0;
-          parity ^= 1u;
-        }
-        if (s != load_stage) wait(&full[s], parity, A.error_flags);
-      }
-      return;
-    }
-    if (kpos < U.k1 && !((bad >> s) & 1u)) {
-      const uint32_t ks_u = ring_u + uint32_t(s * LT::STAGE), vs_u = ks_u + LT::TILE;
-      // scores of 16 rows x 16 keys
-      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t b[4];  // keys 0-7 (k 0-7, 8-15), keys 8-15 (k 0-7, 8-15)
-        ldsm4(ks_u + tile_at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), b);
-        mma_bf16(sc[0], qf[ks], b[0], b[1]);
-        mma_bf16(sc[1], qf[ks], b[2], b[3]);
-      }
-      const bool partial = kpos + KT > U.all_see;  // some row does not see some key of the tile
-      if (partial) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = U.row0 + g8 + 8 * i;
-          int end = U.k1 - kpos;  // keys of the tile this row sees
-          if (U.seg >= G && row < U.rows) end = min(end, U.len - U.nq + row / P.per + 1 - kpos);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
-            if (key >= end) sc[e >> 1][i * 2 + (e & 1)] = -INFINITY;
+      load();
+      const int kpos = U.k0 + i_tile * KT;
+      if (!__all_sync(0xffffffffu, wait(&full[s], parity, A.error_flags))) {
+        // gave up: what else was issued lands (waits bounded too) before the warp leaves
+        for (int k = 1; k < STAGES; ++k) {
+          if (++s == STAGES) {
+            s = 0;
+            parity ^= 1u;
           }
+          if (s != load_stage) wait(&full[s], parity, A.error_flags);
         }
+        if (PLANNED && P.tc == 2) pdl_wait();
+        return;
       }
-      float top[2];
+      if (kpos < U.k1 && !((bad >> s) & 1u)) {
+        const uint32_t ks_u = ring_u + uint32_t(s * LT::STAGE), vs_u = ks_u + LT::TILE;
+        // scores of 16 rows x 16 keys
+        float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        top[i] = fmaxf(fmaxf(sc[0][i * 2], sc[0][i * 2 + 1]), fmaxf(sc[1][i * 2], sc[1][i * 2 + 1])) * scale;
-      bool grow = top[0] > m[0] + RESCALE_LOG2;
-      if (two) grow = grow || top[1] > m[1] + RESCALE_LOG2;
-      if (__any_sync(0xffffffffu, grow)) {
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t b[4];  // keys 0-7 (k 0-7, 8-15), keys 8-15 (k 0-7, 8-15)
+          ldsm4(ks_u + tile_at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), b);
+          mma_bf16(sc[0], qf[ks], b[0], b[1]);
+          mma_bf16(sc[1], qf[ks], b[2], b[3]);
+        }
+        const bool partial = kpos + KT > U.all_see;  // some row does not see some key of the tile
+        if (partial) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float x = top[i] == top[i] ? top[i] : -INFINITY;
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          if (x > m[i] + RESCALE_LOG2) {  // by the row alone
-            const float keep = exp2_approx(m[i] - x);
-            m[i] = x;
-            l[i] *= keep;
+          for (int i = 0; i < 2; ++i) {
+            const int row = U.row0 + g8 + 8 * i;
+            int end = U.k1 - kpos;  // keys of the tile this row sees
+            if (U.seg >= G && row < U.rows) end = min(end, U.len - U.nq + row / P.per + 1 - kpos);
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              o[n][i * 2] *= keep;
-              o[n][i * 2 + 1] *= keep;
+            for (int e = 0; e < 4; ++e) {
+              const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
+              if (key >= end) sc[e >> 1][i * 2 + (e & 1)] = -INFINITY;
             }
           }
         }
-      }
-      // The weights are rounded to bf16 for the product, as the values are; l
-      // sums them before that rounding, which is unbiased.
-      float p[2][4];
-      uint32_t pa[4] = {0u, 0u, 0u, 0u};
-      auto weights = [&](int i) {
-        const float base = m[i] == -INFINITY ? 0.0f : m[i];
+        float top[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          p[e >> 1][i * 2 + (e & 1)] = exp2_approx(fmaf(sc[e >> 1][i * 2 + (e & 1)], scale, -base));
-        l[i] += (p[0][i * 2] + p[0][i * 2 + 1]) + (p[1][i * 2] + p[1][i * 2 + 1]);
-        pa[i] = as_u32(pack2_rn(make_float2(p[0][i * 2], p[0][i * 2 + 1])));
-        pa[2 + i] = as_u32(pack2_rn(make_float2(p[1][i * 2], p[1][i * 2 + 1])));
-      };
-      weights(0);
-      if (two) weights(1);
-      if (partial) {
-        // Keys that some row of the tile does not see (a later token of the same
-        // step, or beyond the last): those that another row sees are added row by
-        // row, so that a masked value, whatever it holds, meets no product; then
-        // zeros take their place for the mma.
-        const int j0 = max(U.all_see - kpos, 0), j1 = min(U.k1 - kpos, KT);
-        uint8_t* vt = ring + s * LT::STAGE + LT::TILE;
-        for (int j = j0; j < j1; ++j) {
+        for (int i = 0; i < 2; ++i)
+          top[i] = fmaxf(fmaxf(sc[0][i * 2], sc[0][i * 2 + 1]), fmaxf(sc[1][i * 2], sc[1][i * 2 + 1])) * scale;
+        bool grow = top[0] > m[0] + RESCALE_LOG2;
+        if (two) grow = grow || top[1] > m[1] + RESCALE_LOG2;
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (i == 1 && !two) continue;
-            const uint32_t pw0 = __shfl_sync(0xffffffffu, __float_as_uint(j < 8 ? p[0][i * 2] : p[1][i * 2]),
-                                             (lane & ~3) | ((j & 7) >> 1));
-            const uint32_t pw1 = __shfl_sync(
-                0xffffffffu, __float_as_uint(j < 8 ? p[0][i * 2 + 1] : p[1][i * 2 + 1]),
-                (lane & ~3) | ((j & 7) >> 1));
-            const float w = __uint_as_float(j & 1 ? pw1 : pw0);
-            const int row = U.row0 + g8 + 8 * i;
-            if (row < U.rows && kpos + j < U.len - U.nq + row / P.per + 1) {
+            float x = top[i] == top[i] ? top[i] : -INFINITY;
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            if (x > m[i] + RESCALE_LOG2) {  // by the row alone
+              const float keep = exp2_approx(m[i] - x);
+              m[i] = x;
+              l[i] *= keep;
 #pragma unroll
               for (int n = 0; n < D / 8; ++n) {
-                const float2 v = unpack2(*reinterpret_cast<const bf162*>(vt + tile_at(j, n) + t4 * 4));
-                o[n][i * 2] = fmaf(w, v.x, o[n][i * 2]);
-                o[n][i * 2 + 1] = fmaf(w, v.y, o[n][i * 2 + 1]);
+                o[n][i * 2] *= keep;
+                o[n][i * 2 + 1] *= keep;
               }
             }
           }
         }
-        __syncwarp();
-        for (int c = lane; c < (KT - j0) * (D / 8); c += 32)
-          *reinterpret_cast<uint4*>(vt + tile_at(j0 + c / (D / 8), c % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA fills the stage again
-        __syncwarp();
-        const int key = t4 * 2;
-        const uint32_t lo0 = key < j0 ? 0xFFFFu : 0u, hi0 = key + 1 < j0 ? 0xFFFF0000u : 0u;
-        const uint32_t lo1 = key + 8 < j0 ? 0xFFFFu : 0u, hi1 = key + 9 < j0 ? 0xFFFF0000u : 0u;
-        pa[0] &= lo0 | hi0;
-        pa[1] &= lo0 | hi0;
-        pa[2] &= lo1 | hi1;
-        pa[3] &= lo1 | hi1;
-      }
+        // The weights are rounded to bf16 for the product, as the values are; l
+        // sums them before that rounding, which is unbiased.
+        float p[2][4];
+        uint32_t pa[4] = {0u, 0u, 0u, 0u};
+        auto weights = [&](int i) {
+          const float base = m[i] == -INFINITY ? 0.0f : m[i];
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        uint32_t b[4];  // values of keys 0-7 and 8-15, columns 16n + 0-7 then 16n + 8-15
-        ldsm4_trans(vs_u + tile_at(lane & 15, n * 2 + (lane >> 4)), b);
-        mma_bf16(o[2 * n], pa, b[0], b[1]);
-        mma_bf16(o[2 * n + 1], pa, b[2], b[3]);
+          for (int e = 0; e < 4; ++e)
+            p[e >> 1][i * 2 + (e & 1)] = exp2_approx(fmaf(sc[e >> 1][i * 2 + (e & 1)], scale, -base));
+          l[i] += (p[0][i * 2] + p[0][i * 2 + 1]) + (p[1][i * 2] + p[1][i * 2 + 1]);
+          pa[i] = as_u32(pack2_rn(make_float2(p[0][i * 2], p[0][i * 2 + 1])));
+          pa[2 + i] = as_u32(pack2_rn(make_float2(p[1][i * 2], p[1][i * 2 + 1])));
+        };
+        weights(0);
+        if (two) weights(1);
+        if (partial) {
+          // Keys that some row of the tile does not see (a later token of the same
+          // step, or beyond the last): those that another row sees are added row by
+          // row, so that a masked value, whatever it holds, meets no product; then
+          // zeros take their place for the mma.
+          const int j0 = max(U.all_see - kpos, 0), j1 = min(U.k1 - kpos, KT);
+          uint8_t* vt = ring + s * LT::STAGE + LT::TILE;
+          for (int j = j0; j < j1; ++j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (i == 1 && !two) continue;
+              const uint32_t pw0 = __shfl_sync(0xffffffffu, __float_as_uint(j < 8 ? p[0][i * 2] : p[1][i * 2]),
+                                               (lane & ~3) | ((j & 7) >> 1));
+              const uint32_t pw1 = __shfl_sync(
+                  0xffffffffu, __float_as_uint(j < 8 ? p[0][i * 2 + 1] : p[1][i * 2 + 1]),
+                  (lane & ~3) | ((j & 7) >> 1));
+              const float w = __uint_as_float(j & 1 ? pw1 : pw0);
+              const int row = U.row0 + g8 + 8 * i;
+              if (row < U.rows && kpos + j < U.len - U.nq + row / P.per + 1) {
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) {
+                  const float2 v = unpack2(*reinterpret_cast<const bf162*>(vt + tile_at(j, n) + t4 * 4));
+                  o[n][i * 2] = fmaf(w, v.x, o[n][i * 2]);
+                  o[n][i * 2 + 1] = fmaf(w, v.y, o[n][i * 2 + 1]);
+                }
+              }
+            }
+          }
+          __syncwarp();
+          for (int c = lane; c < (KT - j0) * (D / 8); c += 32)
+            *reinterpret_cast<uint4*>(vt + tile_at(j0 + c / (D / 8), c % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA fills the stage again
+          __syncwarp();
+          const int key = t4 * 2;
+          const uint32_t lo0 = key < j0 ? 0xFFFFu : 0u, hi0 = key + 1 < j0 ? 0xFFFF0000u : 0u;
+          const uint32_t lo1 = key + 8 < j0 ? 0xFFFFu : 0u, hi1 = key + 9 < j0 ? 0xFFFF0000u : 0u;
+          pa[0] &= lo0 | hi0;
+          pa[1] &= lo0 | hi0;
+          pa[2] &= lo1 | hi1;
+          pa[3] &= lo1 | hi1;
+        }
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          uint32_t b[4];  // values of keys 0-7 and 8-15, columns 16n + 0-7 then 16n + 8-15
+          ldsm4_trans(vs_u + tile_at(lane & 15, n * 2 + (lane >> 4)), b);
+          mma_bf16(o[2 * n], pa, b[0], b[1]);
+          mma_bf16(o[2 * n + 1], pa, b[2], b[3]);
+        }
       }
-    }
-    __syncwarp();  // the stage is read before it is filled again
-    if (++s == STAGES) {
-      s = 0;
-      parity ^= 1u;
-    }
+      __syncwarp();  // the stage is read before it is filled again
+      if (++s == STAGES) {
+        s = 0;
+        parity ^= 1u;
+      }
 
     }
     // ---- the piece is complete
-    {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const int row = U.row0 + g8 + 8 * i;
-        if (row >= U.rows) continue;
-        const int qi = row / P.per;
-        const long long token = U.begin + qi;
-        const int head = U.head * P.per + row - qi * P.per;
-        if (U.only) {
-          const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
-          bf16* dst = static_cast<bf16*>(A.out) + token * A.out_token_stride +
-                      (long long)head * A.out_head_stride + t4 * 2;
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      const int row = U.row0 + g8 + 8 * i;
+      if (row >= U.rows) continue;
+      const int qi = row / P.per;
+      const long long token = U.begin + qi;
+      const int head = U.head * P.per + row - qi * P.per;
+      if (U.only) {
+        const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
+        bf16* dst = static_cast<bf16*>(A.out) + token * A.out_token_stride +
+                    (long long)head * A.out_head_stride + t4 * 2;
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<uint32_t*>(dst + n * 8) =
-                as_u32(pack2_rn(make_float2(o[n][i * 2] * inv, o[n][i * 2 + 1] * inv)));
-        } else {
-          const long long slot = (token * A.heads + head) * (P.slots_s + P.slots) +
-                                 (U.seg >= G ? P.slots_s : 0) + U.index;
-          if (t4 == 0) P.ml[slot] = make_float2(m[i], l[i]);
-          float* dst = P.o + slot * D + t4 * 2;
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<uint32_t*>(dst + n * 8) =
+              as_u32(pack2_rn(make_float2(o[n][i * 2] * inv, o[n][i * 2 + 1] * inv)));
+      } else {
+        const long long slot = (token * A.heads + head) * (P.slots_s + P.slots) +
+                               (U.seg >= G ? P.slots_s : 0) + U.index;
+        if (t4 == 0) P.ml[slot] = make_float2(m[i], l[i]);
+        float* dst = P.o + slot * D + t4 * 2;
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][i * 2], o[n][i * 2 + 1]);
-        }
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][i * 2], o[n][i * 2 + 1]);
       }
     }
   }
+  if (PLANNED && P.tc == 2) pdl_wait();  // the shared kernel: the join waits for this one alone
 }
 
 // Joins the pieces of the rows that have more than one: a warp a row, or
@@ -563,9 +630,10 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
     return;
   }
   const int g = group_of(P, r), len = length(P, r);
-  const int sh = g >= 0 && len > 0 ? P.plan[2 + g] : 0;
-  const int ns = sh > 0 ? ceil_div(sh, P.plan[0]) : 0;
-  const int no = ceil_div(own_tiles(len, sh), P.plan[1]);
+  // (through L1: read from L2 by every warp, these words cost 4 us of 85)
+  const int sh = g >= 0 && len > 0 ? P.shared[g] : 0;
+  const int ns = sh > 0 ? ceil_div(sh / KT, P.head[SHARED_TILES]) : 0;
+  const int no = ceil_div(own_tiles(len, sh), P.head[CHUNK]);
   if (ns == 0 && no == 1) return;  // written already
   const long long base = row * (P.slots_s + P.slots);
   float m = -INFINITY, l = 0.0f, acc[E];
@@ -674,7 +742,9 @@ static Slots slots_of(const hyena_paged_attention_args& A) {
   Slots S;
   S.o = (int)n;
   S.s = shared ? (int)n : 0;
-  S.header = (8 + 4 * (size_t)A.num_groups + 255) & ~size_t(255);  // the plan
+  const size_t G = A.num_groups, R = A.num_requests;
+  S.header = (4 * (HEAD_INTS + 3 * G + 1 + G + R + 1) + 15) / 16 * 16 + 16 * (G + R);  // the plan
+  S.header = (S.header + 255) & ~size_t(255);
   S.bytes = S.header + (size_t)(rows * (S.s + S.o)) * row_bytes;
   return S;
 }
@@ -711,28 +781,46 @@ static int launch(const hyena_paged_attention_args& A, const Slots& S, void* ws,
   P.scale = A.scale * 1.4426950408889634f;
   P.slots_s = S.s;
   P.slots = S.o;
-  // Shared runs of more rows than one 16-row tile go to the tcgen05 kernel.
-  P.tc = S.s > 0 && A.num_groups <= MAX_TC_GROUPS &&
-         (long long)A.T * P.per > (long long)TC_MIN_ROWS * A.num_groups;
+  // Shared runs of more rows than one 16-row tile go to the tcgen05 kernel, with two
+  // row tiles where a group's mean rows need them.
+  const long long mean = A.num_groups > 0 ? (long long)A.T * P.per / A.num_groups : 0;
+  P.tc = A.num_groups > MAX_TC_GROUPS || mean <= TC_MIN_ROWS ? 0 : mean <= 128 ? 1 : 2;
+  const long long most = (long long)A.num_requests * A.kv.pages_per_request * A.kv.page_size;
+  P.planned = P.tc == 2 || (P.tc == 0 && A.num_requests >= PLANNED_REQUESTS &&
+                            most >= PLANNED_BYTES / (4ll * A.kv.kv_heads * D));
+  P.warps = 2 * num_sms() * WARPS;
+  P.ctas = (int)std::min<long long>(
+      num_sms(), ((long long)A.T * P.per / std::max(P.tc * 128, 1) + A.num_groups) * A.kv.kv_heads *
+                     std::max(S.s, 1));
   const long long rows = (long long)A.T * A.heads;
+  const int G = A.num_groups, segs = A.num_groups + A.num_requests;
   uint8_t* w = static_cast<uint8_t*>(ws);
-  P.plan = reinterpret_cast<int32_t*>(w);
+  P.head = reinterpret_cast<int32_t*>(w);
+  P.shared = P.head + HEAD_INTS;
+  P.leader = P.shared + G;
+  P.tc_first = P.leader + G;
+  P.first = P.tc_first + G + 1;
+  P.info = reinterpret_cast<int4*>(w + (4 * (size_t)(HEAD_INTS + 3 * G + 1 + segs + 1) + 15) / 16 * 16);
   P.o = reinterpret_cast<float*>(w + S.header);  // 16-byte pieces first
   P.ml = reinterpret_cast<float2*>(w + S.header + (size_t)(rows * (S.s + S.o)) * D * 4);
-  const int segments = A.num_requests + A.num_groups;
-  const size_t smem = 1024 + Layout<D>::PLAN + (size_t)segments * 20 + 4 + (size_t)A.num_groups * 8;
+  const size_t smem = 1024 + Layout<D>::PLAN + (size_t)segs * 20 + 4 + (size_t)G * 8;
   constexpr int smem_max = 1024 + Layout<D>::PLAN + MAX_SEGMENTS * 28 + 4;
-  if (!smem_attr<stream_kernel<D>>(smem_max))
+  if (!smem_attr<stream_kernel<D, false>>(smem_max) || !smem_attr<stream_kernel<D, true>>(smem_max))
     return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(paged_attention) failed");
   CUtensorMap map_k, map_v;
   int rc = cache_map(&map_k, A.kv, true, KT);
   if (!rc) rc = cache_map(&map_v, A.kv, false, KT);
   if (rc) return rc;
   // each launch is checked before the next, which reads what it leaves
-  launch_kernel(stream_kernel<D>, dim3((unsigned)(2 * num_sms())), dim3(THREADS), smem, st, 0u, P, map_k,
-                map_v);
+  if (P.planned) {
+    launch_kernel(plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, 0u, P);
+    if ((rc = check_launch("paged_attention plan"))) return rc;
+  }
+  if (P.tc == 2 && (rc = shared_launch(P, map_k, map_v, st))) return rc;
+  launch_kernel(P.planned ? stream_kernel<D, true> : stream_kernel<D, false>,
+                dim3((unsigned)(P.warps / WARPS)), dim3(THREADS), smem, st, 0u, P, map_k, map_v);
   if ((rc = check_launch("paged_attention"))) return rc;
-  if (P.tc && (rc = shared_launch(P, map_k, map_v, st))) return rc;
+  if (P.tc == 1 && (rc = shared_launch(P, map_k, map_v, st))) return rc;
   // a block a row while those fill one wave of 16 blocks an SM
   if (rows <= 16ll * num_sms())
     launch_kernel(join_kernel<D, WARPS>, dim3((unsigned)rows), dim3(THREADS), 0, st, 0u, P);

@@ -19,10 +19,28 @@ struct Params {
   int per;         // query heads of one key/value head
   float scale;     // scale * log2(e)
   int slots_s, slots;  // pieces a row may have: of the shared run, of its own keys
-  int32_t* plan;   // {keys of a piece of a shared run, tiles of an own piece}, each group's shared run
-  int tc;          // the shared runs go to attention_shared.cu
+  int tc;          // row tiles of the shared kernel, which takes the shared runs (0: none does)
+  int planned;     // plan_kernel makes the plan; else each CTA its own
+  int warps;       // of the stream kernel
+  int ctas;        // of the shared kernel
+  // the plan, in the workspace (where not `planned`, what the join kernel reads of it)
+  int32_t* head;   // see Head
+  int* shared;     // [groups] the shared runs
+  int* leader;     // [groups] the requests whose page tables stand for them
+  int* tc_first;   // [groups + 1] first items of the shared kernel
+  int* first;      // [groups + requests + 1] first items of the stream kernel
+  int4* info;      // [groups + requests], see Plan
   float2* ml;      // [T * heads][slots]: (m, l)
   float* o;        // [T * heads][slots][D]
+};
+
+enum Head {
+  SHARED_TILES,  // KT-key tiles of a piece of a shared run
+  CHUNK,         // and of a piece of own keys
+  ITEMS,         // of the stream kernel
+  NEXT,          // the item that its next free warp takes
+  TC_TILES,      // 128-key tiles of an item of the shared kernel
+  HEAD_INTS = 8
 };
 
 __device__ __forceinline__ int query_begin(const Params& P, int r) {
@@ -99,6 +117,57 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ uint2 query_sign(float scale) {
   return make_uint2(scale < 0.0f ? 0x80008000u : 0u, scale == 0.0f ? 0u : 0xffffffffu);
 }
+// ---------------------------------------------------------------- shared kernel
+constexpr int TILE_KEYS = 128;
+constexpr int ITEM_OVERHEAD = 3;  // tiles that an item's start and end cost
+
+// Its part of the plan: the chunk length (in tiles) that lets its CTAs finish
+// soonest, waves x (tiles of an item + its overhead) and the pieces to be joined,
+// over the chunk counts of the longest run; then the groups' first items
+// (first[groups]: their number).  Every thread of the CTA; thread 0 leaves first
+// and the tiles of an item.
+template <int NTHREADS>
+__device__ __forceinline__ void plan_shared(const Params& P, const int* shared, int* first, int* tiles) {
+  __shared__ unsigned long long best_s[NTHREADS / 32];
+  const int tid = (int)threadIdx.x, G = P.groups, hkv = P.a.kv.kv_heads, rows_item = P.tc * 128;
+  int longest = 0;
+  for (int g = 0; g < G; ++g) longest = max(longest, shared[g]);
+  const int most = ceil_div(longest, TILE_KEYS);
+  // joining: a piece of every query row, there and back, in sixteenths of a tile's
+  // time (some 13 MB of memory traffic for two row tiles, 8 MB for one)
+  const unsigned long long piece =
+      (unsigned long long)((long long)P.a.T * P.a.heads * (P.a.kv.head_dim + 2)) * 8 * 16 /
+      (P.tc == 1 ? 8000000u : 13000000u);
+  auto units = [&](int g) {
+    int begin;
+    return ceil_div(group_queries(P, g, begin) * P.per, rows_item) * hkv;
+  };
+  unsigned long long best = ~0ull;
+  for (int c = tid + 1; c <= P.slots_s && c <= max(most, 1); c += NTHREADS) {
+    const int n = max(ceil_div(most, c), 1);
+    long long items = 0;
+    for (int g = 0; g < G; ++g) items += (long long)units(g) * ceil_div(ceil_div(shared[g], TILE_KEYS), n);
+    const unsigned long long waves = (unsigned long long)((items + P.ctas - 1) / P.ctas);
+    const unsigned long long cost = 16 * waves * (unsigned long long)(n + ITEM_OVERHEAD) + c * piece;
+    best = min(best, (cost << 24) | (unsigned long long)min(n, (1 << 24) - 1));
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, d));
+  if (tid % 32 == 0) best_s[tid / 32] = best;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < NTHREADS / 32; ++w) best = min(best, best_s[w]);
+    const int n = (int)(best & 0xFFFFFFull);
+    int at = 0;
+    for (int g = 0; g < G; ++g) {
+      first[g] = at;
+      at += units(g) * ceil_div(ceil_div(shared[g], TILE_KEYS), n);
+    }
+    first[G] = at;
+    *tiles = n;
+  }
+}
+
 // O is rescaled when weights reach 2^RESCALE_LOG2: below it bf16 and fp32 round
 // as well as at 1.
 constexpr float RESCALE_LOG2 = 8.0f;

@@ -25,11 +25,18 @@
 // whose softmax and matrix products alternate.  Bound by the keys' bytes up to
 // about 128 rows, beyond by the exponentials and the tensor pipe.
 //
-// Launched after the stream kernel as its programmatic dependent, it does not
-// wait for it at entry: that kernel's CTAs trigger only after their own wait, so
-// the kernels before it have completed, and the two share no data.  Every
-// thread waits at its end instead, so that the join kernel, which waits for this
-// one, finds both complete.
+// It and the stream kernel share no data, and the second of the two does not wait
+// for the first at entry: the first one's CTAs trigger only after their own wait,
+// so that all before them is complete when the second starts, whose CTAs take SMs
+// as the first one leaves them.  The second waits at its end instead, so that the
+// join kernel, which waits for it alone, finds both complete.
+//   NT = 2 goes first, after a plan kernel, and the stream kernel's items, which
+// are then taken as they come, fill the SMs that its last wave leaves: 353 us for
+// 256 samples of one prompt of 32768 keys, 382 us the other way round.
+//   NT = 1 goes second, each CTA of either planning for itself: both are bound by
+// the keys' bytes, and this one fills the end of the two better.  85 us for 64
+// samples of 16384 keys and 99 us for 3 prompts being verified; with the plan
+// kernel 95 and 112 us, with NT = 2's order 98 and 104 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -40,9 +47,7 @@ namespace attn {
 
 using namespace tc;
 
-constexpr int TILE_KEYS = 128;
 constexpr int BOX_MIN = 16;
-constexpr int ITEM_OVERHEAD = 3;  // tiles that an item's start and end cost
 
 template <int D, int NT>
 struct Tc {
@@ -66,8 +71,7 @@ struct __align__(1024) TcSmem {
   uint64_t s_full[NT][2], p_full[NT][2], pv_done[NT], o_done[NT];  // [..][score buffer]
   uint32_t bad[8];  // 16-key blocks of a tile whose page is out of range
   uint32_t tmem;
-  unsigned long long best[16];
-  int chunk_tiles, items;
+  int chunk_tiles;
   int first[MAX_TC_GROUPS + 1], shared[MAX_TC_GROUPS], leader[MAX_TC_GROUPS];
 };
 
@@ -134,7 +138,7 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const hyena_paged_attention_args& A = P.a;
   const int tid = (int)threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int G = P.groups, hkv = A.kv.kv_heads;
+  const int G = P.groups;
 
   if (tid == 0) {
     for (int s = 0; s < T::SLOTS; ++s) {
@@ -160,57 +164,27 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
 
-  // ---- plan: the chunk length (in tiles) that lets the CTAs finish soonest,
-  // waves x (tiles of an item + its overhead) and the pieces to be joined, over the
-  // chunk counts of the longest run; then the groups' first items
-  shared_runs<T::THREADS>(P, S.shared, S.leader);
-  {
-    int longest = 0;
-    for (int g = 0; g < G; ++g) longest = max(longest, S.shared[g]);
-    const int most = ceil_div(longest, TILE_KEYS);
-    // joining: a piece of every query row, there and back, in sixteenths of a tile's
-    // time (some 13 MB of memory traffic for two row tiles, 8 MB for one)
-    const unsigned long long piece = (unsigned long long)((long long)A.T * A.heads * (D + 2)) * 8 * 16 /
-                                     (NT == 1 ? 8000000u : 13000000u);
-    unsigned long long best = ~0ull;
-    for (int c = tid + 1; c <= P.slots_s && c <= max(most, 1); c += T::THREADS) {
-      const int n = max(ceil_div(most, c), 1);
-      long long items = 0;
-      for (int g = 0; g < G; ++g) {
-        int begin;
-        const int rows = group_queries(P, g, begin) * P.per;
-        items += (long long)ceil_div(rows, NT * 128) * hkv *
-                 ceil_div(ceil_div(S.shared[g], TILE_KEYS), n);
+  if (NT == 2) {
+    pdl_wait();  // the plan
+    pdl_trigger();
+    for (int g = tid; g <= G; g += T::THREADS) {
+      S.first[g] = __ldcg(P.tc_first + g);
+      if (g < G) {
+        S.shared[g] = __ldcg(P.shared + g);
+        S.leader[g] = __ldcg(P.leader + g);
       }
-      const unsigned long long waves = (unsigned long long)((items + gridDim.x - 1) / gridDim.x);
-      const unsigned long long cost = 16 * waves * (unsigned long long)(n + ITEM_OVERHEAD) + c * piece;
-      best = min(best, (cost << 24) | (unsigned long long)min(n, (1 << 24) - 1));
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, d));
-    if (lane == 0) S.best[warp] = best;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < T::THREADS / 32; ++w) best = min(best, S.best[w]);
-      const int n = (int)(best & 0xFFFFFFull);
-      int at = 0;
-      for (int g = 0; g < G; ++g) {
-        int begin;
-        const int rows = group_queries(P, g, begin) * P.per;
-        S.first[g] = at;
-        at += ceil_div(rows, NT * 128) * hkv * ceil_div(ceil_div(S.shared[g], TILE_KEYS), n);
-      }
-      S.first[G] = at;
-      S.items = at;
-      S.chunk_tiles = n;
-      if (blockIdx.x == 0) P.plan[0] = n * TILE_KEYS;
-    }
+    if (tid == 0) S.chunk_tiles = __ldcg(P.head + TC_TILES);
+  } else {
+    shared_runs<T::THREADS>(P, S.shared, S.leader);
+    plan_shared<T::THREADS>(P, S.shared, S.first, &S.chunk_tiles);
+    if (blockIdx.x == 0 && tid == 0) P.head[SHARED_TILES] = S.chunk_tiles * (TILE_KEYS / KT);
   }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = S.tmem;
-  const int items = S.items;
+  const int items = S.first[G];
 
   if (warp == 4 * NT + 1) {
     // ---------------------------------------------------------------- loads
@@ -510,8 +484,10 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
                  "r"(T::TMEM_COLS)
                  : "memory");
   }
-  pdl_trigger();
-  pdl_wait();  // the stream kernel: see above
+  if (NT == 1) {
+    pdl_trigger();
+    pdl_wait();  // the stream kernel: the join waits for this one alone
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -528,18 +504,15 @@ static int launch_tc(const Params& P, const CUtensorMap& k16, const CUtensorMap&
   static_assert(sizeof(TcSmem<D, NT>) + 1024 <= 232448, "shared memory of a CTA");
   if (!smem_attr<shared_kernel<D, NT>>((int)smem))
     return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(paged_attention shared) failed");
-  const long long row_tiles = (long long)P.a.T * P.per / (NT * 128) + P.groups;
-  const long long ctas = std::min<long long>(num_sms(), row_tiles * kv.kv_heads * P.slots_s);
-  launch_kernel(shared_kernel<D, NT>, dim3((unsigned)ctas), dim3(Tc<D, NT>::THREADS), smem, st, 0u, P,
+  launch_kernel(shared_kernel<D, NT>, dim3((unsigned)P.ctas), dim3(Tc<D, NT>::THREADS), smem, st, 0u, P,
                 k, v, k16, v16, box);
   return check_launch("paged_attention shared");
 }
 
 int shared_launch(const Params& P, const CUtensorMap& k16, const CUtensorMap& v16, cudaStream_t st) {
-  const bool two = (long long)P.a.T * P.per > 128ll * P.groups;  // mean rows of a group
   if (P.a.kv.head_dim == 128)
-    return two ? launch_tc<128, 2>(P, k16, v16, st) : launch_tc<128, 1>(P, k16, v16, st);
-  return two ? launch_tc<64, 2>(P, k16, v16, st) : launch_tc<64, 1>(P, k16, v16, st);
+    return P.tc == 2 ? launch_tc<128, 2>(P, k16, v16, st) : launch_tc<128, 1>(P, k16, v16, st);
+  return P.tc == 2 ? launch_tc<64, 2>(P, k16, v16, st) : launch_tc<64, 1>(P, k16, v16, st);
 }
 
 int shared_wait_timeouts(int32_t* count, int reset) { return read_wait_timeouts(count, reset); }

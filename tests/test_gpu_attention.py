@@ -290,6 +290,112 @@ def test_long_shared_runs(heads, kv_heads, dim, samples, shared):
     b.check(b.call(**sharing((samples, shared))))
 
 
+def widen(b, keys):
+    """Page tables that could hold `keys` keys a request."""
+    more = keys // b.page - b.table.shape[1]
+    pad = torch.full((len(b.requests), more), b.spare_page, dtype=torch.int32, device=DEV)
+    b.table = torch.cat([b.table, pad], 1)
+    return b
+
+
+MIXES = [
+    [(1, n) for n in LENS],
+    [(1, 1), (8, 9), (3, 400), (2, 2), (7, 64), (5, 129), (1, 0), (2, 1)],
+    [(70, 70), (33, 200), (1, 5), (1, 3000), (40, 41)],
+    [(1, 1 + 97 * i % 700) for i in range(70)],
+]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 128), (8, 2, 64), (5, 1, 128)])
+@pytest.mark.parametrize("requests", MIXES)
+def test_wide_page_tables(heads, kv_heads, dim, requests):
+    """Room for long contexts (half a GB a step and more), whatever the lengths are."""
+    b = widen(Batch(requests, heads, kv_heads, dim, page=16), 2 ** 19)
+    b.check(b.call())
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (8, 4)])
+def test_wide_page_tables_and_groups(heads, kv_heads):
+    groups = [(3, 200), (1, 500), (5, 0), (2, 1111), (2, 48)]
+    reqs, spec, r = [], [], 0
+    for m, sh in groups:
+        reqs += [(1, sh + 3 + 37 * i) for i in range(m)]
+        spec.append((range(r, r + m), sh))
+        r += m
+    b = widen(Batch(reqs, heads, kv_heads, page=16, groups=spec), 2 ** 19)
+    b.check(b.call(**sharing(*groups)))
+
+
+@pytest.mark.parametrize("keys", [None, 2 ** 15])
+def test_many_requests(keys):
+    reqs = [(1 + (i % 7 == 0), (i * 31) % 40 + 2 * (i % 3)) for i in range(2040)]
+    b = Batch(reqs, 2, 2, 64, page=16)
+    if keys:
+        widen(b, keys)
+    out = b.call()
+    at = 0
+    for i, (n, length) in enumerate(reqs):  # every seventh, for the oracle's time
+        if i % 7 == 0:
+            k, v = b.keys[i]
+            ref, tol = attend(b.q[at:at + n], k, v, length - n + 1, 64 ** -0.5)
+            assert ((out[at:at + n].double() - ref).abs() <= tol).all(), i
+        at += n
+    assert torch.isfinite(out).all() and int(b.flags) == 0
+
+
+@pytest.mark.parametrize("groups,members", [(70, 3), (40, 20), (6, 150)])
+def test_many_groups(groups, members):
+    """More groups than the kernel of long shared runs plans for, several of its
+    items a block, and pairs of its row tiles."""
+    spec = [(range(members * g, members * (g + 1)), 16 * (g % 9) + 128) for g in range(groups)]
+    reqs = [(1, sh + 1 + (7 * i) % 23) for m, sh in spec for i, _ in enumerate(m)]
+    b = Batch(reqs, 16, 16 if groups == 6 else 1, page=16, groups=spec)
+    out = b.call(**sharing(*[(len(m), sh) for m, sh in spec]))
+    for i in range(0, len(reqs), 5):
+        ref, tol = attend(b.q[i:i + 1], *b.keys[i], reqs[i][1], 128 ** -0.5)
+        assert ((out[i:i + 1].double() - ref).abs() <= tol).all(), i
+    assert int(b.flags) == 0
+
+
+@pytest.mark.parametrize("samples,keys", [(6, 0), (6, 2 ** 19), (40, 0), (150, 0)])
+def test_unchained_launches_and_graphs(samples, keys):
+    """The same bits with and without programmatic launches, eager and replayed
+    while the lengths grow, each kind of plan."""
+    from evo2_flash_b200 import ops
+
+    b = Batch([(1, 700 + 13 * i) for i in range(samples)], 4, 4, page=16, groups=[(range(samples), 688)])
+    if keys:
+        widen(b, keys)
+    kw = sharing((samples, 688)) if samples > 6 else {}
+    lens, out = b.seq_lens.clone(), torch.empty_like(b.q)
+    b.call(seq_lens=lens, out=out, **kw)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        b.call(seq_lens=lens, out=out, **kw)
+    for n in (1, 60, 689, 720, 10 ** 6):
+        lens.copy_(b.seq_lens.clamp(max=n))
+        g.replay()
+        ops.set_launch_chaining(False)
+        try:
+            plain = b.call(seq_lens=lens, **kw)
+        finally:
+            ops.set_launch_chaining(True)
+        assert torch.equal(plain, out) and torch.equal(b.call(seq_lens=lens, **kw), out)
+    b.check(out)
+
+
+def test_other_device():
+    """Tensors of another device than the current one."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    b = Batch([(1, n) for n in LENS], 4, 4, page=16)
+    here = b.call()
+    b.k, b.v, b.table, b.flags = (t.to("cuda:1") for t in (b.k, b.v, b.table, b.flags))
+    there = b.call(q=b.q.to("cuda:1"), seq_lens=b.seq_lens.to("cuda:1"))
+    assert there.device.index == 1 and torch.equal(there.to(DEV), here)
+
+
 def test_sharing_is_only_a_hint():
     """A shared run longer than a member's keys is cut to what all see; requests
     outside every group have their own keys only; a padded first member (no keys,
