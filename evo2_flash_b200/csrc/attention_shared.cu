@@ -16,14 +16,20 @@
 // Every row sees every key of the run, so only the run's last tile has a mask.
 //
 // O is rescaled only when the weights of a row's tile sum to more than 2^8, its
-// scores having outgrown the m it is scaled by: the weights stay below 2^8, where bf16 and fp32 round as
-// well as at 1, and the pass over O's columns (TMEM -> registers -> TMEM) is rare
-// instead of once a tile.  m and l leave with the piece, so nothing is lost.
+// scores having outgrown the m it is scaled by.  Below that bf16 and fp32 round
+// as well as at 1; the pass over O's columns (TMEM -> registers -> TMEM) is rare
+// instead of once a tile; m and l leave with the piece, so nothing is lost.
 //
 // NT = 1 keeps two score buffers (S of the next tile is computed under the
 // softmax); NT = 2 (256 rows) reads each key and value once for two row tiles,
-// whose softmax and matrix products alternate.  Bound by the keys' bytes up to
-// about 128 rows, beyond by the exponentials and the tensor pipe.
+// whose softmax and matrix products alternate.  Up to about 128 rows it is bound
+// by the keys' bytes.  Beyond, a key tile of 256 rows takes some 3600 cycles, of
+// which the tensor pipe works 2300 (2048 at its peak; Q K^T with both operands in
+// shared memory reads them at all of its bandwidth): a row tile's chain is 1900
+// for the softmax (1024 of them the exponentials alone), 1150 for its two
+// products and 500 from one to the other, and TMEM has no room for a second
+// score buffer.  Two threads a row, a warp instead of a thread issuing the
+// products, 64-key tiles and half tiles of weights all measured the same or worse.
 //
 // It and the stream kernel share no data, and the second of the two does not wait
 // for the first at entry: the first one's CTAs trigger only after their own wait,
@@ -32,7 +38,7 @@
 // join kernel, which waits for it alone, finds both complete.
 //   NT = 2 goes first, after a plan kernel, and the stream kernel's items, which
 // are then taken as they come, fill the SMs that its last wave leaves: 353 us for
-// 256 samples of one prompt of 32768 keys, 382 us the other way round.
+// 256 samples of one prompt of 32768 keys, 382 us the other way round (333 us now).
 //   NT = 1 goes second, each CTA of either planning for itself: both are bound by
 // the keys' bytes, and this one fills the end of the two better.  85 us for 64
 // samples of 16384 keys and 99 us for 3 prompts being verified; with the plan
@@ -145,11 +151,11 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
       mbar_init(&S.full[s], 1);
       mbar_init(&S.empty[s], 1);
     }
-    mbar_init(&S.q_full, NT * 128);
+    mbar_init(&S.q_full, 4 * NT);
     for (int t = 0; t < NT; ++t) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&S.s_full[t][b], 2);
-        mbar_init(&S.p_full[t][b], 128);
+        mbar_init(&S.p_full[t][b], 4);
       }
       mbar_init(&S.pv_done[t], 1);
       mbar_init(&S.o_done[t], 1);
@@ -275,12 +281,12 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
         for (int ks = 0; ks < TILE_KEYS / 16; ++ks)
           mma_ts(d, p + ks * 8, v + ks * (2048 / 16), ID_O, acc || ks != 0);
         // waited for only where O is rescaled, at most one product behind: a parity
-        // tells no more than neighbours apart, so the item's end has o_done
-        mma_commit(&S.pv_done[t]);
+        // tells no more than neighbours apart, so the item's end has o_done.  (NT = 2:
+        // the tile's next scores come after this product, so s_full tells.)
+        if constexpr (NT == 1) mma_commit(&S.pv_done[t]);
       };
       auto slot_full = [&](uint32_t slot_u) {
         ok = ok && wait(&S.full[slot_u % T::SLOTS], (slot_u / T::SLOTS) & 1, A.error_flags);
-        fence_after();
       };
       for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x, ++n_item) {
         const Item I = item_of<D, NT>(P, S, item);
@@ -299,12 +305,14 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
               mma_commit(&S.empty[(u + 2) % T::SLOTS]);
             }
           }
+          // (before the weights are awaited, while products are under way)
+          slot_full(u + 1);
+          if (NT > 1 && more) slot_full(u + 2);
           for (int t = 0; t < NT && ok; ++t) {
             // (a barrier a buffer: a warp without rows is done with the next tile's
             // scores before the others are with this one's)
             ok = ok && wait(&S.p_full[t][T::NBUF == 2 ? (gi & 1) : 0],
                             T::NBUF == 2 ? (gi >> 1) & 1 : gi & 1, A.error_flags);
-            if (t == 0) slot_full(u + 1);
             if (!ok) break;
             fence_after();
             values(t, gi, u + 1, i != 0);
@@ -312,8 +320,6 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
             if (t == NT - 1) mma_commit(&S.empty[(u + 1) % T::SLOTS]);
             if constexpr (NT > 1) {
               if (more) {
-                if (t == 0) slot_full(u + 2);
-                if (!ok) break;
                 score(t, gi + 1, u + 2);
                 if (t == NT - 1) mma_commit(&S.empty[(u + 2) % T::SLOTS]);
               }
@@ -332,6 +338,10 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     const int slots = P.slots_s + P.slots;
     uint32_t gi = 0, n_item = 0;
     bool ok = true;
+    auto warp_arrive = [&](uint64_t* bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
     for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x) {
       const Item I = item_of<D, NT>(P, S, item);
       const int row = I.row0 + t * 128 + row_in;
@@ -353,7 +363,7 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
                                     (((c & 7) ^ (row_in & 7)) << 4)) = x;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&S.q_full);
+        warp_arrive(&S.q_full);
       }
       const bool active = I.row0 + t * 128 + 32 * (warp % 4) < I.rows;  // some row of the warp exists
       float m = -INFINITY, l = 0.0f;  // m: what O and l are scaled by (log2)
@@ -430,8 +440,10 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
               }
               l *= keep;
               weights(std::true_type{});
-              ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
-              if (!ok) break;
+              if constexpr (NT == 1) {
+                ok = __all_sync(0xffffffffu, wait(&S.pv_done[t], (gi - 1) & 1, A.error_flags));
+                if (!ok) break;
+              }
               fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
@@ -450,7 +462,7 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
           tmem_wait_st();
         }
         fence_before();
-        mbar_arrive(&S.p_full[t][b]);
+        warp_arrive(&S.p_full[t][b]);
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, wait(&S.o_done[t], n_item & 1, A.error_flags));
