@@ -10,9 +10,12 @@
 //   next warp    tcgen05.mma issue (one thread): S_t = Q_t K^T (K-major operands),
 //                O_t += P_t V with P_t in TMEM and V read MN-major as it lies in
 //                the cache; O stays in TMEM for the whole item
-//   last warp    TMA: tiles of 128 keys (256 B rows, SWIZZLE_128B, two 64-column
-//                halves) by the largest box that a page holds whole; keys and
-//                values take turns in one ring
+//   last two     TMA: tiles of 128 keys (256 B rows, SWIZZLE_128B, two 64-column
+//                halves) by the largest box that a page holds whole, one warp for
+//                the keys and one for the values, which take turns in one ring (a
+//                warp needs 50 ns a box, 16 of them a tile in pages of 16: 91 us for
+//                verifying 4 tokens of 48 requests on 3 prompts of 2029 keys, 99 us
+//                with one warp for both)
 // Every row sees every key of the run, so only the run's last tile has a mask.
 //
 // O is rescaled only when the weights of a row's tile sum to more than 2^8, its
@@ -41,8 +44,8 @@
 // 256 samples of one prompt of 32768 keys, 382 us the other way round (333 us now).
 //   NT = 1 goes second, each CTA of either planning for itself: both are bound by
 // the keys' bytes, and this one fills the end of the two better.  85 us for 64
-// samples of 16384 keys and 99 us for 3 prompts being verified; with the plan
-// kernel 95 and 112 us, with NT = 2's order 98 and 104 us.
+// samples of a prompt of 8192 keys and 99 us for 3 prompts being verified (91 us
+// now); with the plan kernel 95 and 112 us, with NT = 2's order 98 and 104 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -63,7 +66,7 @@ struct Tc {
   static constexpr int FIT = (224 * 1024 - NT * TILE_BYTES) / TILE_BYTES;
   static constexpr int SLOTS = FIT < 8 ? FIT : 8;
   static constexpr int NBUF = NT == 1 ? 2 : 1;       // score buffers of a row tile
-  static constexpr int THREADS = NT * 128 + 64;
+  static constexpr int THREADS = NT * 128 + 96;
   static constexpr uint32_t S_COL = 0, O_COL = 256;  // TMEM columns
   static constexpr uint32_t TMEM_COLS = 512;
 };
@@ -192,65 +195,66 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
   const uint32_t tmem = S.tmem;
   const int items = S.first[G];
 
-  if (warp == 4 * NT + 1) {
+  if (warp > 4 * NT) {
     // ---------------------------------------------------------------- loads
-    uint32_t u = 0, tile_no = 0;
+    const int kv = warp - 4 * NT - 1;  // keys, or values
+    uint32_t u = (uint32_t)kv, tile_no = 0;
     bool ok = true;
     for (int item = (int)blockIdx.x; item < items && ok; item += (int)gridDim.x) {
       const Item I = item_of<D, NT>(P, S, item);
       const int32_t* table = A.kv.page_table + (long long)I.leader * A.kv.page_table_stride;
-      for (int i = 0; i < I.tiles && ok; ++i, ++tile_no) {
+      // lane j: page of 16-key block j of a tile, looked up a tile ahead
+      auto page_of = [&](int kpos) {
+        const int pos = kpos + lane * BOX_MIN;
+        return lane < TILE_KEYS / BOX_MIN && pos < I.k1 ? __ldg(table + pos / A.kv.page_size) : 0;
+      };
+      int next = page_of(I.k0);
+      for (int i = 0; i < I.tiles && ok; ++i, ++tile_no, u += 2) {
         const int kpos = I.k0 + i * TILE_KEYS;
         const int keys = min(TILE_KEYS, I.k1 - kpos);
-        // lane j: 16-key block j of the tile (its page), and whether it leads a
-        // whole box or stands alone in the tail
-        int page = 0, at = 0;
-        bool mine = lane < TILE_KEYS / BOX_MIN && lane * BOX_MIN < keys, good = true;
+        const int page = next, at = (kpos + lane * BOX_MIN) % A.kv.page_size;
+        next = page_of(kpos + TILE_KEYS);
+        // whether the block leads a whole box or stands alone in the tail
+        const bool mine = lane < TILE_KEYS / BOX_MIN && lane * BOX_MIN < keys;
+        const bool good = !mine || (page >= 0 && page < A.kv.num_pages);
         const bool whole = (lane * BOX_MIN / box + 1) * box <= keys;
-        if (mine) {
-          const int pos = kpos + lane * BOX_MIN;
-          page = __ldg(table + pos / A.kv.page_size);
-          at = pos % A.kv.page_size;
-          good = page >= 0 && page < A.kv.num_pages;
-          if (!good) flag_error(A.error_flags, HYENA_FLAG_BLOCK_RANGE);
-        }
+        if (!good) flag_error(A.error_flags, HYENA_FLAG_BLOCK_RANGE);
         const uint32_t bad = __ballot_sync(0xffffffffu, !good);
         const uint32_t have = __ballot_sync(0xffffffffu, mine && good);
-        if (lane == 0) S.bad[tile_no & 7] = bad;
+        if (kv == 0 && lane == 0) S.bad[tile_no & 7] = bad;
         const bool leads = mine && good && (whole ? lane * BOX_MIN % box == 0 : true);
         const uint32_t bytes = uint32_t(__popc(have)) * BOX_MIN * D * 2;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++u) {  // keys, then values
-          const int s = u % T::SLOTS;
-          ok = __all_sync(0xffffffffu, wait(&S.empty[s], ((u / T::SLOTS) & 1) ^ 1, A.error_flags));
-          if (!ok) break;
-          uint8_t* slot = S.ring[s];
-          if (kv == 1 && have != 0xFFu) {
-            // weights of absent keys are zero, but so must their values be
-            for (int r = lane; r < TILE_KEYS * T::HALVES * 8; r += 32) {
-              const int row = r / 8 % TILE_KEYS;
-              if (!((have >> (row / BOX_MIN)) & 1u))
-                *reinterpret_cast<uint4*>(slot + r * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+        const int s = u % T::SLOTS;
+        ok = __all_sync(0xffffffffu, wait(&S.empty[s], ((u / T::SLOTS) & 1) ^ 1, A.error_flags));
+        if (!ok) break;
+        uint8_t* slot = S.ring[s];
+        if (kv == 1 && have != 0xFFu) {
+          // weights of absent keys are zero, but so must their values be
+          for (int r = lane; r < TILE_KEYS * T::HALVES * 8; r += 32) {
+            const int row = r / 8 % TILE_KEYS;
+            if (!((have >> (row / BOX_MIN)) & 1u))
+              *reinterpret_cast<uint4*>(slot + r * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
-          if (lane == 0) mbar_expect_tx(&S.full[s], bytes);
-          __syncwarp();
-          if (leads) {
-            const CUtensorMap* map = kv == 0 ? (whole ? &map_k : &map_k16) : (whole ? &map_v : &map_v16);
-#pragma unroll
-            for (int h = 0; h < T::HALVES; ++h)
-              tma_load_4d(map, &S.full[s], slot + h * T::HALF_BYTES + lane * BOX_MIN * 128, h * 64, at,
-                          I.head, page);
-          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
+        if (lane == 0) mbar_expect_tx(&S.full[s], bytes);
+        __syncwarp();
+        if (leads) {
+          const CUtensorMap* map = kv == 0 ? (whole ? &map_k : &map_k16) : (whole ? &map_v : &map_v16);
+#pragma unroll
+          for (int h = 0; h < T::HALVES; ++h)
+            tma_load_4d(map, &S.full[s], slot + h * T::HALF_BYTES + lane * BOX_MIN * 128, h * 64, at,
+                        I.head, page);
+        }
+        __syncwarp();
       }
     }
     // Drain: every issued copy has landed, and every slot's release has arrived,
-    // before the CTA can exit.
-    for (uint32_t i = u > (uint32_t)T::SLOTS ? u - T::SLOTS : 0; i < u; ++i) {
+    // before the CTA can exit.  (u is 2 tile_no + kv: the last SLOTS uses of the ring
+    // are those no later use has followed.)
+    for (uint32_t i = (uint32_t)kv; i < u; i += 2) {
+      if (i + T::SLOTS < 2 * tile_no) continue;
       wait(&S.full[i % T::SLOTS], (i / T::SLOTS) & 1, A.error_flags);
       if (ok) wait(&S.empty[i % T::SLOTS], (i / T::SLOTS) & 1, A.error_flags);
     }

@@ -145,8 +145,9 @@ __device__ __forceinline__ float gate(float z1, float z2, int act) {
 // stays in L2 while the activations stream through once.  The gated pair of
 // weights (180 MB) does not fit, so its tiles go in groups of GATED_GROUP row
 // tiles, rows fastest: the group's activations stay in L2 and the weights are
-// read once a group instead of once a row tile.  N fastest against grouped: see
-// gemm_gated_bf16_launch.
+// read once a group instead of once a row tile: 1704 us for 8192 rows of the 7B
+// shape and 828 us for 777 of the 40B shape, N fastest 2039 and 1193 us (groups of 4
+// 1841 and 936, of 16 1705 and 875).
 constexpr int GATED_GROUP = 8;
 template <bool GATED>
 __device__ __forceinline__ void tile_mn(int tile, int m_tiles, int n_tiles, int& m, int& n) {

@@ -15,7 +15,11 @@
 // HBM-bound: 12 bytes an element pair of heads read and written once.  A block
 // owns TB tokens; their cos / sin go to shared memory once and serve every
 // head; a thread then moves U independent items of 8 + 8 elements (16-byte
-// accesses), U loads in flight.
+// accesses), U loads in flight.  TB is 1 up to 8 tokens an SM, so that short steps
+// spread over the GPU, else 4, for which the fp64 angles are formed once a token
+// and not once a head.  65536 tokens of 32 heads take 508 us (499 at the measured copy
+// rate), 4099 tokens of 32 query and 8 key/value heads 22 us (15.6), one token 3.7 us
+// (a launch).  U of 4 and 6 cost registers and gained nothing (prefill 527 us with 6).
 #include <cmath>
 
 #include "attention.cuh"

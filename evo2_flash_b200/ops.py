@@ -682,9 +682,11 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
     run longer than what all of the group's queries see is cut, so the result
     never depends on it.  scale defaults to D ** -0.5.  B + G is at most 2048.
 
-    One launch, and one that joins the pieces of split rows; lengths and tables
-    are read on the device, so a captured graph serves growing contexts.  The
-    workspace comes from torch's caching allocator.  Returns (T, heads, D) bf16."""
+    Two to four kernels (a plan, the shared runs of many rows, all other keys, and
+    joining the pieces of split rows); lengths and tables are read on the device,
+    so a captured graph serves growing contexts, and every call gives the same
+    bits.  The workspace comes from torch's caching allocator.  Returns
+    (T, heads, D) bf16."""
     device = _same_device("q k_cache v_cache page_table seq_lens query_start_loc shared_lens group_start "
                           "out error_flags", q, k_cache, v_cache, page_table, seq_lens, query_start_loc,
                           shared_lens, group_start, out, error_flags)

@@ -405,7 +405,11 @@ HYENA_API int hyena_kv_append(const hyena_kv_append_args* a, void* stream);
  * which are then read once for the group.  What a query sees is not changed by
  * it: a run longer than what every query of the group sees is cut.
  * heads is a multiple of kv_heads (query head h reads head h / (heads / kv_heads)).
- * The lengths are read on the device: one captured launch serves growing contexts. */
+ * Up to four kernels on the stream (a plan, the shared runs of many rows, all other
+ * keys, and joining the pieces of split rows).  The lengths are read on the device,
+ * so captured calls serve growing contexts; the result has the same bits on every
+ * call.  The workspace holds the call's plan and pieces: calls that may run at the
+ * same time (two streams, two graphs replayed side by side) need one each. */
 typedef struct hyena_paged_attention_args {
   const void* q; int64_t q_token_stride, q_head_stride;          /* (T, heads, head_dim) bf16 */
   void* out; int64_t out_token_stride, out_head_stride;
