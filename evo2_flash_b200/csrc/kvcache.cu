@@ -14,12 +14,13 @@
 //
 // HBM-bound: 12 bytes an element pair of heads read and written once.  A block
 // owns TB tokens; their cos / sin go to shared memory once and serve every
-// head; a thread then moves U independent items of 8 + 8 elements (16-byte
-// accesses), U loads in flight.  TB is 1 up to 8 tokens an SM, so that short steps
-// spread over the GPU, else 4, for which the fp64 angles are formed once a token
-// and not once a head.  65536 tokens of 32 heads take 508 us (499 at the measured copy
-// rate), 4099 tokens of 32 query and 8 key/value heads 22 us (15.6), one token 3.7 us
-// (a launch).  U of 4 and 6 cost registers and gained nothing (prefill 527 us with 6).
+// head; a thread then moves items of 8 + 8 elements (16-byte accesses), the first
+// one's loads under way before the cos / sin are formed.  TB is 1 up to 8 tokens an
+// SM, so that short steps spread over the GPU, else 4, which spreads the fp64 angles
+// and the page lookup over more bytes.  65536 tokens of 32 heads take 509 us (499 at
+// the measured copy rate), 4099 tokens of 32 query and 8 key/value heads 20 us
+// (15.6), one token 3.8 us (a launch).  Two items of a thread in flight: 507 and 22-24
+// us, four 550 and 22-25 us (registers); TB of 2: 493 and 21-22 us, of 8: 522 and 22.
 #include <cmath>
 
 #include "attention.cuh"
@@ -28,7 +29,6 @@ namespace hb {
 
 constexpr int KV_THREADS = 256;
 constexpr int KV_MAX_HALF = 64;  // head_dim / 2
-constexpr int U = 2;             // items of a thread in flight
 
 struct KvAppendParams {
   hyena_kv_append_args a;
@@ -58,13 +58,13 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
   const int tid = (int)threadIdx.x;
   const int half = A.kv.head_dim / 2;
   const long long t0 = (long long)blockIdx.x * TB;
-  // ---- a batch's loads (the first one's before anything else: they wait for
+  // ---- an item's loads (the first one's before anything else: they wait for
   // nothing but the previous kernel)
   const int oct_bits = half == 64 ? 3 : 2;  // 8-element pieces of a half
   const int hq = A.q != nullptr ? A.heads : 0, hkv = A.kv.kv_heads;
   const int items = (hq + 2 * hkv) << oct_bits;  // of a token
   const int all = (int)min((long long)TB, A.T - t0) * items;
-  uint4 a[U], b[U];
+  uint4 a, b;
   auto split = [&](int i, int& tok, int& h, int& oct) {
     tok = 0;
 #pragma unroll
@@ -73,24 +73,20 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
     h = i >> oct_bits;
     oct = i - (h << oct_bits);
   };
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * KV_THREADS;
-      if (i >= all) continue;
-      int tok, h, oct;
-      split(i, tok, h, oct);
-      const long long t = t0 + tok;
-      const bf16* src;
-      if (h < hq)
-        src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
-      else if (h < hq + hkv)
-        src = static_cast<const bf16*>(A.k) + t * A.k_token_stride + (h - hq) * A.k_head_stride;
-      else
-        src = static_cast<const bf16*>(A.v) + t * A.v_token_stride + (h - hq - hkv) * A.v_head_stride;
-      a[u] = *reinterpret_cast<const uint4*>(src + oct * 8);
-      b[u] = *reinterpret_cast<const uint4*>(src + half + oct * 8);
-    }
+  auto load = [&](int i) {
+    if (i >= all) return;
+    int tok, h, oct;
+    split(i, tok, h, oct);
+    const long long t = t0 + tok;
+    const bf16* src;
+    if (h < hq)
+      src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
+    else if (h < hq + hkv)
+      src = static_cast<const bf16*>(A.k) + t * A.k_token_stride + (h - hq) * A.k_head_stride;
+    else
+      src = static_cast<const bf16*>(A.v) + t * A.v_token_stride + (h - hq - hkv) * A.v_head_stride;
+    a = *reinterpret_cast<const uint4*>(src + oct * 8);
+    b = *reinterpret_cast<const uint4*>(src + half + oct * 8);
   };
   load(tid);
 
@@ -131,40 +127,35 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
   }
   __syncthreads();
 
-  for (int i0 = tid; i0 < all; i0 += U * KV_THREADS) {
-    if (i0 != tid) load(i0);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * KV_THREADS;
-      if (i >= all) continue;
-      int tok, h, oct;
-      split(i, tok, h, oct);
-      if (!live[tok]) continue;
-      bf16* dst;
-      if (h < hq) {
-        dst = static_cast<bf16*>(A.q_out) + (t0 + tok) * A.q_out_token_stride + h * A.q_out_head_stride;
-      } else if (h < hq + hkv) {
-        if (koff[tok] < 0) continue;
-        dst = static_cast<bf16*>(A.kv.k) + koff[tok] + (h - hq) * A.kv.k_head_stride;
-      } else {
-        if (voff[tok] < 0) continue;
-        dst = static_cast<bf16*>(A.kv.v) + voff[tok] + (h - hq - hkv) * A.kv.v_head_stride;
-      }
-      if (h < hq + hkv) {
-        uint32_t* aw = reinterpret_cast<uint32_t*>(&a[u]);
-        uint32_t* bw = reinterpret_cast<uint32_t*>(&b[u]);
-        const float4* tab = reinterpret_cast<const float4*>(&cs[tok][oct * 8]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 r = tab[w];  // cos, sin of two pairs
-          const float2 x = unpack2(as_bf162(aw[w])), y = unpack2(as_bf162(bw[w]));
-          aw[w] = as_u32(pack2_rn(make_float2(x.x * r.x - y.x * r.y, x.y * r.z - y.y * r.w)));
-          bw[w] = as_u32(pack2_rn(make_float2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w)));
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + oct * 8) = a[u];
-      *reinterpret_cast<uint4*>(dst + half + oct * 8) = b[u];
+  for (int i = tid; i < all; i += KV_THREADS) {
+    if (i != tid) load(i);
+    int tok, h, oct;
+    split(i, tok, h, oct);
+    if (!live[tok]) continue;
+    bf16* dst;
+    if (h < hq) {
+      dst = static_cast<bf16*>(A.q_out) + (t0 + tok) * A.q_out_token_stride + h * A.q_out_head_stride;
+    } else if (h < hq + hkv) {
+      if (koff[tok] < 0) continue;
+      dst = static_cast<bf16*>(A.kv.k) + koff[tok] + (h - hq) * A.kv.k_head_stride;
+    } else {
+      if (voff[tok] < 0) continue;
+      dst = static_cast<bf16*>(A.kv.v) + voff[tok] + (h - hq - hkv) * A.kv.v_head_stride;
     }
+    if (h < hq + hkv) {
+      uint32_t* aw = reinterpret_cast<uint32_t*>(&a);
+      uint32_t* bw = reinterpret_cast<uint32_t*>(&b);
+      const float4* tab = reinterpret_cast<const float4*>(&cs[tok][oct * 8]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 r = tab[w];  // cos, sin of two pairs
+        const float2 x = unpack2(as_bf162(aw[w])), y = unpack2(as_bf162(bw[w]));
+        aw[w] = as_u32(pack2_rn(make_float2(x.x * r.x - y.x * r.y, x.y * r.z - y.y * r.w)));
+        bw[w] = as_u32(pack2_rn(make_float2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w)));
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + oct * 8) = a;
+    *reinterpret_cast<uint4*>(dst + half + oct * 8) = b;
   }
 }
 
