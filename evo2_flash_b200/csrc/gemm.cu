@@ -1411,39 +1411,36 @@ static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& tt, const
   return check_launch("gemm_gated_pair_kernel");
 }
 
-// The cheapest by `steps`: SM pairs, the persistent kernel's widths and,
-// for one row tile (decode batches), the cluster kernel's (BN, splits) of one wave,
-// which cut K where the tiles alone leave SMs idle (one split measures as the
-// persistent kernel).  A wave is bound by HBM there, so 160 columns
-// are among them: the 7B shape (11008 outputs) makes 138 tiles of 148, the 40B
-// shape (22528) 282 of 296.
+// Several row tiles: the cheapest by `steps` of the persistent kernel's widths and SM
+// pairs (those where they are 7% ahead).
+// One row tile (decode batches): the weights' bytes bound it, so the shortest time of
+// the busiest SM; no allowance for the clock in the last wave, which HBM does not know.
+// Hence 160 columns, which the plain GEMMs do not have: the 7B shape (11008 outputs)
+// makes 138 tiles of 148 SMs, 33.4 us for 101 rows (192 columns, 115 tiles: 37.7; 256:
+// 40.8; 128, two waves: 50.3), the 40B shape (22528) 282 of 296.  K is cut (the cluster
+// kernel) where the tiles alone leave SMs idle: 4096 outputs of 4096 take 14-17 us on
+// 43 tiles of 192 in 3 slices, 21 us on 128 of 64.
 static Plan plan_gated(int M, int N, int K) {
   const long long mt = (M + BM - 1) / BM;
   const int sms = num_sms(), kblocks = K / (BKB / 2);
   auto tiles = [&](int bn) { return mt * ((N + bn / 2 - 1) / (bn / 2)); };
   Plan best = {0, 0};
   long long best_cost = 0;
-  for (int bn : {256, 192, 160, 128, 64}) {
-    const long long cost = steps(tiles(bn), sms, bn, false) * kblocks;
+  auto take = [&](int bn, int sp, long long cost) {
     if (best.bn == 0 || cost < best_cost) {
-      best = {bn, 0};
+      best = {bn, sp};
       best_cost = cost;
     }
-  }
+  };
   if (M > BM) {
-    if (100 * pair_steps(M, (N + BN2 / 2 - 1) / (BN2 / 2)) * kblocks <= 93 * best_cost)
-      return {BN2, 0, true};
+    for (int bn : {256, 192, 160, 128, 64}) take(bn, 0, steps(tiles(bn), sms, bn, false));
+    if (100 * pair_steps(M, (N + BN2 / 2 - 1) / (BN2 / 2)) <= 93 * best_cost) return {BN2, 0, true};
     return best;
   }
   for (int bn : {256, 192, 160, 128, 64}) {
-    for (int sp = 2; sp <= (bn >= 256 ? 3 : 4); ++sp) {
-      if (tiles(bn) * sp > sms || kblocks / sp < 2) break;
-      const long long cost = tile_step(bn) * ((kblocks + sp - 1) / sp);
-      if (cost < best_cost) {
-        best = {bn, sp};
-        best_cost = cost;
-      }
-    }
+    take(bn, 0, (tiles(bn) + sms - 1) / sms * tile_step(bn) * kblocks);
+    for (int sp = 2; sp <= (bn >= 256 ? 3 : 4) && tiles(bn) * sp <= sms && kblocks / sp >= 2; ++sp)
+      take(bn, sp, tile_step(bn) * ((kblocks + sp - 1) / sp));
   }
   return best;
 }
