@@ -13,14 +13,14 @@
 // 2^-24 p radians, 0.06 at a position of one million.
 //
 // HBM-bound: 12 bytes an element pair of heads read and written once.  A block
-// owns TB tokens; their cos / sin go to shared memory once and serve every
-// head; a thread then moves items of 8 + 8 elements (16-byte accesses), the first
-// one's loads under way before the cos / sin are formed.  TB is 1 up to 8 tokens an
-// SM, so that short steps spread over the GPU, else 4, which spreads the fp64 angles
-// and the page lookup over more bytes.  65536 tokens of 32 heads take 509 us (499 at
-// the measured copy rate), 4099 tokens of 32 query and 8 key/value heads 20 us
-// (15.6), one token 3.8 us (a launch).  Two items of a thread in flight: 507 and 22-24
-// us, four 550 and 22-25 us (registers); TB of 2: 493 and 21-22 us, of 8: 522 and 22.
+// owns TB tokens, KV_THREADS / TB threads each; their cos / sin are formed once
+// for all heads, in shared memory, and a thread, which stays with eight pairs of its
+// token, keeps theirs in registers (16-byte accesses; the first head's loads under
+// way before the cos / sin are formed).  TB is 1 up to 8 tokens an SM, so that short
+// steps spread over the GPU, else 4.  65536 tokens of 32 heads take 495 us (499 at the
+// measured copy rate), 4099 tokens of 32 query and 8 key/value heads 19-21 us (15.6),
+// one token 3.3 us (a launch).  With cos / sin read from shared memory for every head:
+// 509, 20 and 3.8 us; TB of 2 494, of 8 501 us; blocks of 128 threads 500, of 512 554.
 #include <cmath>
 
 #include "attention.cuh"
@@ -50,7 +50,7 @@ __device__ __forceinline__ int page_of(const hyena_paged_kv& kv, int r, int page
 
 template <int TB>
 __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_constant__ KvAppendParams P) {
-  __shared__ float2 cs[TB][KV_MAX_HALF];
+  __shared__ __align__(16) float2 cs[TB][KV_MAX_HALF];
   __shared__ long long koff[TB], voff[TB];  // element offset of the token's row; -1: not written
   __shared__ int live[TB];
   pdl_entry();
@@ -58,26 +58,17 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
   const int tid = (int)threadIdx.x;
   const int half = A.kv.head_dim / 2;
   const long long t0 = (long long)blockIdx.x * TB;
-  // ---- an item's loads (the first one's before anything else: they wait for
-  // nothing but the previous kernel)
+  // A thread's items: 8 + 8 elements (piece `oct` of both halves) of every step-th
+  // head of one token.
+  constexpr int TPT = KV_THREADS / TB;
   const int oct_bits = half == 64 ? 3 : 2;  // 8-element pieces of a half
-  const int hq = A.q != nullptr ? A.heads : 0, hkv = A.kv.kv_heads;
-  const int items = (hq + 2 * hkv) << oct_bits;  // of a token
-  const int all = (int)min((long long)TB, A.T - t0) * items;
+  const int tok = tid / TPT, oct = tid & ((1 << oct_bits) - 1), step = TPT >> oct_bits;
+  const int hq = A.q != nullptr ? A.heads : 0, hkv = A.kv.kv_heads, all = hq + 2 * hkv;
+  const int h0 = (tid % TPT) >> oct_bits;
+  const long long t = t0 + tok;
   uint4 a, b;
-  auto split = [&](int i, int& tok, int& h, int& oct) {
-    tok = 0;
-#pragma unroll
-    for (int k = 1; k < TB; ++k) tok += i >= k * items;
-    i -= tok * items;
-    h = i >> oct_bits;
-    oct = i - (h << oct_bits);
-  };
-  auto load = [&](int i) {
-    if (i >= all) return;
-    int tok, h, oct;
-    split(i, tok, h, oct);
-    const long long t = t0 + tok;
+  auto load = [&](int h) {
+    if (h >= all || t >= A.T) return;
     const bf16* src;
     if (h < hq)
       src = static_cast<const bf16*>(A.q) + t * A.q_token_stride + h * A.q_head_stride;
@@ -88,7 +79,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
     a = *reinterpret_cast<const uint4*>(src + oct * 8);
     b = *reinterpret_cast<const uint4*>(src + half + oct * 8);
   };
-  load(tid);
+  load(h0);  // before anything else: it waits for nothing but the previous kernel
 
   if (tid < TB) {
     const long long t = t0 + tid;
@@ -117,24 +108,25 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
     voff[tid] = vo;
   }
   for (int i = tid; i < TB * half; i += KV_THREADS) {
-    const int tok = i / half, p = i - tok * half;
-    if (t0 + tok < A.T) {
-      const double turn = (double)__ldg(A.positions + t0 + tok) * P.turns[p];
+    const int k = i / half, p = i - k * half;
+    if (t0 + k < A.T) {
+      const double turn = (double)__ldg(A.positions + t0 + k) * P.turns[p];
       float s, c;
       sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
-      cs[tok][p] = make_float2(c, s);
+      cs[k][p] = make_float2(c, s);
     }
   }
   __syncthreads();
 
-  for (int i = tid; i < all; i += KV_THREADS) {
-    if (i != tid) load(i);
-    int tok, h, oct;
-    split(i, tok, h, oct);
-    if (!live[tok]) continue;
+  if (!live[tok]) return;
+  float4 rot[4];  // cos, sin of this thread's pairs
+#pragma unroll
+  for (int w = 0; w < 4; ++w) rot[w] = reinterpret_cast<const float4*>(&cs[tok][oct * 8])[w];
+  for (int h = h0; h < all; h += step) {
+    if (h != h0) load(h);
     bf16* dst;
     if (h < hq) {
-      dst = static_cast<bf16*>(A.q_out) + (t0 + tok) * A.q_out_token_stride + h * A.q_out_head_stride;
+      dst = static_cast<bf16*>(A.q_out) + t * A.q_out_token_stride + h * A.q_out_head_stride;
     } else if (h < hq + hkv) {
       if (koff[tok] < 0) continue;
       dst = static_cast<bf16*>(A.kv.k) + koff[tok] + (h - hq) * A.kv.k_head_stride;
@@ -145,10 +137,9 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
     if (h < hq + hkv) {
       uint32_t* aw = reinterpret_cast<uint32_t*>(&a);
       uint32_t* bw = reinterpret_cast<uint32_t*>(&b);
-      const float4* tab = reinterpret_cast<const float4*>(&cs[tok][oct * 8]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float4 r = tab[w];  // cos, sin of two pairs
+        const float4 r = rot[w];
         const float2 x = unpack2(as_bf162(aw[w])), y = unpack2(as_bf162(bw[w]));
         aw[w] = as_u32(pack2_rn(make_float2(x.x * r.x - y.x * r.y, x.y * r.z - y.y * r.w)));
         bw[w] = as_u32(pack2_rn(make_float2(y.x * r.x + x.x * r.y, y.y * r.z + x.y * r.w)));
