@@ -149,7 +149,7 @@ class Evo2MLP(nn.Module):
 
     def forward(self, x):
         # (a hook on a projection, as the embedding names use, wants its own output)
-        if self.native and not any(m._forward_hooks for m in (self.l1, self.l2, self.l3)):
+        if self.native and not any(m._forward_hooks or m._forward_pre_hooks for m in (self.l1, self.l2, self.l3)):
             from . import ops
 
             return ops.gated_mlp(x, self.l1.weight, self.l2.weight, self.l3.weight,
@@ -172,7 +172,8 @@ def _rope_neox(x, positions, theta):
 
 
 # Steps of at most this many new tokens a sequence attend over the paged cache;
-# longer ones (prompts) through torch's attention on the sequence's gathered pages.
+# longer ones (prompts), and steps of more sequences than one call takes, through
+# torch's attention on the sequence's gathered pages.
 PAGED_ATTENTION_TOKENS = 64
 
 
@@ -200,7 +201,9 @@ class Evo2Attention(nn.Module):
         k_cache, v_cache = step.cache.layer(self.index)
         q = ops.kv_append(q, k, v, step.positions, k_cache, v_cache, step.table, step.starts,
                           rope_theta=self.theta)
-        if step.longest <= PAGED_ATTENTION_TOKENS:
+        groups = step.shared["shared_lens"].shape[0] if step.shared else 0
+        if (step.longest <= PAGED_ATTENTION_TOKENS
+                and len(step) + groups <= ops.PAGED_ATTENTION_REQUESTS):
             return ops.paged_attention(q, k_cache, v_cache, step.table, step.seq_lens, step.starts,
                                        **step.shared)
         out = torch.empty_like(q)

@@ -488,6 +488,7 @@ def gemm_bf16(a, b, bias=None, out=None):
 # argument structs are packed in one go (layouts as in include/hyena_b200.h,
 # native alignment) and the stream is read without building a torch.cuda.Stream.
 ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2}
+PAGED_ATTENTION_REQUESTS = 2048  # requests and groups of one paged_attention call
 _PAGED_KV = "PP6qPq5i"  # hyena_paged_kv
 _KV_APPEND = struct.Struct("@PqqPqqPqqPqqPP3i" + _PAGED_KV + "dP")          # hyena_kv_append_args
 _PAGED_ATTENTION = struct.Struct("@PqqPqqPPPP4if" + _PAGED_KV + "P")        # hyena_paged_attention_args
@@ -680,7 +681,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
     shared_lens (G,): requests group_start[g] .. group_start[g + 1] - 1 (default:
     one group of all) name the same rows for their first shared_lens[g] keys; a
     run longer than what all of the group's queries see is cut, so the result
-    never depends on it.  scale defaults to D ** -0.5.  B + G is at most 2048.
+    never depends on it.  scale defaults to D ** -0.5.  B + G is at most 2048
+    (PAGED_ATTENTION_REQUESTS).  out may be q itself.
 
     Two to four kernels (a plan, the shared runs of many rows, all other keys, and
     joining the pieces of split rows); lengths and tables are read on the device,

@@ -405,6 +405,7 @@ HYENA_API int hyena_kv_append(const hyena_kv_append_args* a, void* stream);
  * which are then read once for the group.  What a query sees is not changed by
  * it: a run longer than what every query of the group sees is cut.
  * heads is a multiple of kv_heads (query head h reads head h / (heads / kv_heads)).
+ * out may be q (same strides).
  * Up to four kernels on the stream (a plan, the shared runs of many rows, all other
  * keys, and joining the pieces of split rows).  The lengths are read on the device,
  * so captured calls serve growing contexts; the result has the same bits on every

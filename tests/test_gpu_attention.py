@@ -487,6 +487,19 @@ def test_bad_pages_are_flagged_and_not_read():
     assert ((out[:1].double() - ref).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("members,shared", [(0, 0), (3, 64), (12, 640), (40, 640), (150, 640)])
+def test_in_place(members, shared):
+    """out is q: rows of one piece and of several, every kind of shared run."""
+    reqs = [(1 + (i % 5 == 0), shared + 2 + 61 * i % 400) for i in range(members)] + [(2, 30), (1, 3000), (1, 0)]
+    groups = [(range(members), shared)] if members else []
+    b = Batch(reqs, 8, 4, page=16, groups=groups)
+    kw = sharing((members, shared)) if members else {}
+    out = b.call(**kw)
+    b.check(out)
+    q = b.q.clone()
+    assert b.call(q=q, out=q, **kw) is q and torch.equal(q, out)
+
+
 def test_same_bits_every_time():
     reqs = [(1, 2000 + 11 * i) for i in range(40)]
     b = Batch(reqs, 4, 4, page=16, groups=[(range(40), 1999)])

@@ -41,7 +41,8 @@ def inputs(M, K, N, seed=0):
 # rows below, at and beyond a 128-row tile and the SM-pair kernel's switch; K of
 # one block, odd numbers of blocks; N of part of a tile, odd numbers of tiles
 @pytest.mark.parametrize("M,K,N", [
-    (1, 64, 8), (1, 4096, 11008), (7, 192, 72), (101, 256, 512), (128, 512, 1000), (128, 4096, 11008),
+    (1, 64, 8), (1, 4096, 11008), (7, 192, 72), (3, 128, 22528), (128, 192, 22528), (64, 2048, 5504),
+    (90, 512, 30008), (101, 256, 512), (128, 512, 1000), (128, 4096, 11008),
     (129, 320, 136), (300, 512, 2056), (777, 1024, 5504), (4095, 128, 264), (4096, 256, 128),
     (4101, 192, 1160), (5000, 512, 120)])
 @pytest.mark.parametrize("activation", ["none", "gelu", "silu"])

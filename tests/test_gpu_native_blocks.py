@@ -109,6 +109,32 @@ def test_fork_continues_like_the_original(models):
     native.release_all()
 
 
+def test_more_sequences_than_one_call_takes(models, monkeypatch):
+    from evo2_flash_b200 import ops
+
+    _, native = models
+    with torch.no_grad():
+        outs = []
+        for limit in (2048, 4):
+            monkeypatch.setattr(ops, "PAGED_ATTENTION_REQUESTS", limit)
+            list(native.prefill_steps([_tokens(20 + i, i) for i in range(5)], keep_cache=True))
+            outs.append(native.decode_step([65] * 5, [20 + i for i in range(5)], range(5)))
+    native.release_all()
+    assert max_rel_err(outs[1].float().cpu(), outs[0].float().cpu()) < 2 * REL_TOL
+
+
+def test_hooks_before_a_projection_run(models):
+    _, native = models
+    mlp, seen = native.layers[1].mlp, []
+    x = torch.randn(3, 256, device="cuda").to(torch.bfloat16)
+    hook = mlp.l2.register_forward_pre_hook(lambda m, args: seen.append(args[0].shape))
+    try:
+        mlp(x)
+    finally:
+        hook.remove()
+    assert seen == [x.shape]
+
+
 @pytest.mark.parametrize("temperature", [0.0, 1.0])
 def test_generate_samples_of_one_prompt(models, temperature):
     """Four samples of one prompt among others: the results of the prompts given one
