@@ -744,6 +744,11 @@ def _matrix(t, name, cols=None):
         raise ValueError(f"{name} must have {cols} columns, got {tuple(t.shape)}")
 
 
+def _ld(t):
+    """Row stride; a one-row tensor may carry any: its length is what counts."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def gemm_gated_bf16(a, b1, b2, activation="none", out=None):
     """out (M, N) bf16 = act(a . b1^T) * (a . b2^T): a (M, K), b1 and b2 (N, K)
     bf16, activation "none", "gelu" (erf) or "silu", fp32 up to the one rounding
@@ -762,11 +767,9 @@ def gemm_gated_bf16(a, b1, b2, activation="none", out=None):
     else:
         _matrix(out, "out", N)
         _require(out.shape[0] == M, f"out must have {M} rows, got {out.shape[0]}")
-    # a one-row tensor may carry any row stride: its length is what counts
-    ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1]  # noqa: E731
     with _On(device) as stream:
-        rc = _lib.load().hyena_gemm_gated_bf16(a.data_ptr(), ld(a), b1.data_ptr(), ld(b1), b2.data_ptr(),
-                                               ld(b2), out.data_ptr(), ld(out), M, N, K,
+        rc = _lib.load().hyena_gemm_gated_bf16(a.data_ptr(), _ld(a), b1.data_ptr(), _ld(b1), b2.data_ptr(),
+                                               _ld(b2), out.data_ptr(), _ld(out), M, N, K,
                                                ACTIVATIONS[activation], stream)
     if rc:
         _lib.check(rc, "hyena_gemm_gated_bf16")
@@ -789,7 +792,12 @@ def gated_mlp(x, w1, w2, w3, activation="none", out=None):
     h = gemm_gated_bf16(x, w1, w2, activation)
     if out is None:
         out = torch.empty(h.shape[0], w3.shape[0], dtype=BF16, device=h.device)
-    if h.shape[0] == 0:
+    M, N = out.shape
+    if M == 0 or N == 0:
         return out
-    with _On(device):
-        return gemm_bf16(h, w3, out=out)
+    with _On(device) as stream:
+        rc = _lib.load().hyena_gemm_bf16(h.data_ptr(), _ld(h), w3.data_ptr(), _ld(w3), out.data_ptr(), _ld(out),
+                                         M, N, h.shape[1], None, None, 0, stream)
+    if rc:
+        _lib.check(rc, "hyena_gemm_bf16")
+    return out
