@@ -1232,14 +1232,6 @@ static int resident(int bn, int splits) {
   }
 }
 
-// Large M: the persistent kernel (splits = 0) with the N-tile width that gives
-// every SM a tile and the shortest last wave: cost = waves x (BN + 32), the 32
-// standing for a tile's fixed epilogue share; 256 unless another width is at
-// least 10% cheaper (M = 512 x N = 12288: 192-wide tiles, 256 tiles in 2 waves
-// instead of 192 tiles whose second wave is nearly as long as the first).  Small M (decode batches): the cluster kernel with the
-// (BN, splits) that, in one resident wave of at most one CTA per SM, puts the
-// fewest operand bytes through any one SM ((BM + BN) x its K slice; ties: fewer
-// splits), each K slice at least two stages long.
 // Cycles that `tiles` tiles of 128 x bn (pair: 256 x 256 on an SM pair) take for a
 // step of 16 bf16 (32 e4m3) of K on `slots` SMs or pairs.  A tile's step: the
 // tensor pipe's 128 x bn products at 4096 a cycle, or its (128 + bn) 32-byte
@@ -1256,6 +1248,15 @@ static long long pair_steps(int M, int n_tiles) {
   return steps((M + 2 * BM - 1) / (2 * BM) * (long long)n_tiles, num_sms() / 2, BN2, true);
 }
 
+// Large M: the persistent kernel (splits = 0) with the N-tile width that gives
+// every SM a tile and the shortest last wave: cost = waves x (BN + 32), the 32
+// standing for a tile's fixed epilogue share; 256 unless another width is at
+// least 10% cheaper (M = 512 x N = 12288: 192-wide tiles, 256 tiles in 2 waves
+// instead of 192 tiles whose second wave is nearly as long as the first).
+// Small M (decode batches): the cluster kernel with the (BN, splits) that, in one
+// resident wave of at most one CTA per SM, puts the fewest operand bytes through any
+// one SM ((BM + BN) x its K slice; ties: fewer splits), each K slice at least two
+// stages long.
 template <bool FP8>
 static Plan plan(int M, int N, int K) {
   const long long mt = (M + BM - 1) / BM;
