@@ -64,6 +64,18 @@ struct Plan {
   int* leader; // [groups] the request whose pages stand for it
 };
 
+constexpr int PLAN_BYTES = 28;  // of a segment, at most; and 4
+// A plan of n segments, G of them groups, at p (16-byte aligned).
+__device__ __forceinline__ Plan plan_at(uint8_t* p, int G, int n) {
+  Plan L;
+  L.chunk = L.items = 0;
+  L.info = reinterpret_cast<int4*>(p);
+  L.first = reinterpret_cast<int*>(L.info + n);
+  L.shared = L.first + n + 1;
+  L.leader = L.shared + G;
+  return L;
+}
+
 __device__ __forceinline__ int row_tiles(const Params& P, int nq) {
   return (int)(((long long)nq * P.per + ROWS - 1) / ROWS);
 }
@@ -160,16 +172,24 @@ __device__ void make_plan(const Params& P, Plan& L) {
 // SM that is far from its memory, or busy with the shared kernel, takes fewer).
 constexpr int PLAN_THREADS = 256;
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constant__ Params P) {
+  extern __shared__ uint8_t smem_raw[];
+  const int tid = (int)threadIdx.x, G = P.groups, n = G + P.a.num_requests;
   pdl_entry();
-  Plan L{0, 0, P.first, P.info, P.shared, P.leader};
+  Plan L = plan_at(smem_raw, G, n);
   make_plan<PLAN_THREADS>(P, L);
-  if (threadIdx.x == 0) {
+  for (int i = tid; i <= n; i += PLAN_THREADS) {
+    P.first[i] = L.first[i];
+    if (i < n) P.info[i] = L.info[i];
+    if (i < G) P.shared[i] = L.shared[i];
+    if (i < G) P.leader[i] = L.leader[i];
+  }
+  if (tid == 0) {
     P.head[SHARED_TILES] = P.head[CHUNK] = L.chunk;
     P.head[ITEMS] = L.items;
     P.head[NEXT] = 0;
   }
   if (P.tc) {
-    plan_shared<PLAN_THREADS>(P, P.shared, P.tc_first, P.head + TC_TILES);
+    plan_shared<PLAN_THREADS>(P, L.shared, P.tc_first, P.head + TC_TILES);
     if (threadIdx.x == 0) P.head[SHARED_TILES] = P.head[TC_TILES] * (TILE_KEYS / KT);
   }
 }
@@ -298,11 +318,7 @@ stream_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
     pdl_trigger();  // the plan is complete: see attention_shared.cu
   else
     pdl_entry();
-  Plan L;
-  L.info = reinterpret_cast<int4*>(smem + LT::PLAN);
-  L.first = reinterpret_cast<int*>(L.info + (G + B));
-  L.shared = reinterpret_cast<int*>(L.first + (G + B + 1));
-  L.leader = L.shared + G;
+  Plan L = plan_at(smem + LT::PLAN, G, G + B);
   if (PLANNED) {
     for (int i = tid; i <= G + B; i += THREADS) {
       L.first[i] = __ldcg(P.first + i);
@@ -828,9 +844,10 @@ static int launch(const hyena_paged_attention_args& A, const Slots& S, void* ws,
   P.info = reinterpret_cast<int4*>(w + (4 * (size_t)(HEAD_INTS + 3 * G + 1 + segs + 1) + 15) / 16 * 16);
   P.o = reinterpret_cast<float*>(w + S.header);  // 16-byte pieces first
   P.ml = reinterpret_cast<float2*>(w + S.header + (size_t)(rows * (S.s + S.o)) * D * 4);
-  const size_t smem = 1024 + Layout<D>::PLAN + (size_t)segs * 20 + 4 + (size_t)G * 8;
-  constexpr int smem_max = 1024 + Layout<D>::PLAN + MAX_SEGMENTS * 28 + 4;
-  if (!smem_attr<stream_kernel<D, false>>(smem_max) || !smem_attr<stream_kernel<D, true>>(smem_max))
+  const size_t plan = (size_t)segs * 20 + 4 + (size_t)G * 8, smem = 1024 + Layout<D>::PLAN + plan;
+  constexpr int plan_max = MAX_SEGMENTS * PLAN_BYTES + 4, smem_max = 1024 + Layout<D>::PLAN + plan_max;
+  if (!smem_attr<stream_kernel<D, false>>(smem_max) || !smem_attr<stream_kernel<D, true>>(smem_max) ||
+      !smem_attr<plan_kernel>(plan_max))
     return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(paged_attention) failed");
   CUtensorMap map_k, map_v;
   int rc = cache_map(&map_k, A.kv, true, KT);
@@ -838,7 +855,7 @@ static int launch(const hyena_paged_attention_args& A, const Slots& S, void* ws,
   if (rc) return rc;
   // each launch is checked before the next, which reads what it leaves
   if (P.planned) {
-    launch_kernel(plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, 0u, P);
+    launch_kernel(plan_kernel, dim3(1), dim3(PLAN_THREADS), plan, st, 0u, P);
     if ((rc = check_launch("paged_attention plan"))) return rc;
   }
   if (P.tc == 2 && (rc = shared_launch(P, map_k, map_v, st))) return rc;
