@@ -81,8 +81,8 @@ __device__ __forceinline__ int row_tiles(const Params& P, int nq) {
 }
 // Tiles of a unit of an own segment.  A request with queries has a tile even
 // without keys: its rows are written there.
-__device__ __forceinline__ int own_tiles(int len, int k_begin) {
-  return max(ceil_div(max(len - k_begin, 0), KT), 1);
+__device__ __forceinline__ int own_tiles(const Params& P, int len, int k_begin) {
+  return max(ceil_div(max(min(len, capacity(P)) - k_begin, 0), KT), 1);
 }
 
 // Every thread of the CTA.
@@ -97,7 +97,7 @@ __device__ void make_plan(const Params& P, Plan& L) {
   // a thread takes a run of consecutive segments
   const int per = ceil_div(n, NTHREADS);
   const int s0 = min(tid * per, n), s1 = min(s0 + per, n);
-  auto tiles_of = [&](int s, const int4& x) { return s < G ? x.z / KT : own_tiles(x.z, x.w); };
+  auto tiles_of = [&](int s, const int4& x) { return s < G ? x.z / KT : own_tiles(P, x.z, x.w); };
   long long work = 0;
   int longest = 0;
   for (int s = s0; s < s1; ++s) {
@@ -111,6 +111,7 @@ __device__ void make_plan(const Params& P, Plan& L) {
       x.y = queries(P, r, x.x);
       x.z = length(P, r);
       x.w = g >= 0 && x.z > 0 ? L.shared[g] : 0;
+      if (x.y > 0 && x.z > capacity(P)) flag_error(P.a.error_flags, HYENA_FLAG_BLOCK_RANGE);
     }
     L.info[s] = x;
     const int units = row_tiles(P, x.y) * P.a.kv.kv_heads, tiles = tiles_of(s, x);
@@ -263,7 +264,7 @@ __device__ __forceinline__ Item item_at(const Params& P, const Plan& L, int item
   I.len = x.z;
   I.rows = x.y * P.per;
   I.request = own ? seg - G : x.w;
-  const int first_key = own ? x.w : 0, tiles = own ? own_tiles(x.z, x.w) : x.z / KT;
+  const int first_key = own ? x.w : 0, tiles = own ? own_tiles(P, x.z, x.w) : x.z / KT;
   const int tiles_r = ceil_div(I.rows, ROWS), units = tiles_r * P.a.kv.kv_heads;
   const int rem = item - L.first[seg];
   I.index = rem / units;
@@ -273,7 +274,7 @@ __device__ __forceinline__ Item item_at(const Params& P, const Plan& L, int item
   I.n = min(L.chunk, tiles - I.index * L.chunk);
   I.only = own && x.w == 0 && tiles <= L.chunk;
   I.k0 = first_key + I.index * L.chunk * KT;
-  I.k1 = I.all_see = min(x.z, I.k0 + I.n * KT);
+  I.k1 = I.all_see = min(min(x.z, capacity(P)), I.k0 + I.n * KT);
   if (own) {
     const int last = min(I.nq - 1, (I.row0 + ROWS - 1) / P.per);
     I.k1 = min(I.k1, I.len - I.nq + last + 1);
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
   // (through L1: read from L2 by every warp, these words cost 4 us of 85)
   const int sh = g >= 0 && len > 0 ? P.shared[g] : 0;
   const int ns = sh > 0 ? ceil_div(sh / KT, P.head[SHARED_TILES]) : 0;
-  const int no = ceil_div(own_tiles(len, sh), P.head[CHUNK]);
+  const int no = ceil_div(own_tiles(P, len, sh), P.head[CHUNK]);
   if (ns == 0 && no == 1) return;  // written already
   // The statistics of 32 pieces at a time, a lane each; then their O, whose weights
   // are known by then, so that UNROLL loads are on their way at once (one request of

@@ -53,10 +53,15 @@ __device__ __forceinline__ int queries(const Params& P, int r, int& begin) {
   end = end < P.a.T ? end : P.a.T;
   return begin >= 0 && end > begin ? end - begin : 0;
 }
+// Positions that a page table has.
+__device__ __forceinline__ int capacity(const Params& P) {
+  return P.a.kv.pages_per_request * P.a.kv.page_size;
+}
+// Keys of request r as its queries count them, which may be more than its table has
+// (those are not read): the queries' positions go by this length.
 __device__ __forceinline__ int length(const Params& P, int r) {
-  const int cap = P.a.kv.pages_per_request * P.a.kv.page_size;
   const int n = __ldg(P.a.seq_lens + r);
-  return n < 0 ? 0 : n < cap ? n : cap;
+  return n < 0 ? 0 : n;
 }
 // Group of request r, or -1.
 __device__ __forceinline__ int group_of(const Params& P, int r) {
@@ -83,8 +88,7 @@ __host__ __device__ __forceinline__ int ceil_div(int a, int b) { return a / b + 
 // sees, then to whole KT-key tiles.  Padded requests (no keys) do not count.
 template <int NTHREADS>
 __device__ __forceinline__ void shared_runs(const Params& P, int* shared, int* leader) {
-  const int G = P.groups, B = P.a.num_requests, tid = (int)threadIdx.x;
-  const int cap = P.a.kv.pages_per_request * P.a.kv.page_size;
+  const int G = P.groups, B = P.a.num_requests, tid = (int)threadIdx.x, cap = capacity(P);
   if (G == 0) return;
   for (int g = tid; g < G; g += NTHREADS) {
     const int n = __ldg(P.a.shared_lens + g);

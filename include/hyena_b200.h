@@ -396,7 +396,8 @@ HYENA_API int hyena_kv_append(const hyena_kv_append_args* a, void* stream);
 
 /* Causal softmax attention of a step's queries over the paged cache: query i of
  * the n of request r sits at position seq_lens[r] - n + i and sees the keys
- * j <= that position (seq_lens counts the step's own tokens, appended before).
+ * j <= that position (seq_lens counts the step's own tokens, appended before; where
+ * it exceeds the page table, the keys that the table has).
  * A query that sees no key (seq_lens[r] = 0: a padded request) gives zeros;
  * output rows that no request owns are left alone; keys that a query does not see
  * do not touch its result, whatever they hold.
