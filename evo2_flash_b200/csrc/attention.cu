@@ -108,10 +108,12 @@ __device__ void make_plan(const Params& P, Plan& L) {
       x.w = L.leader[s];
     } else {
       const int r = s - G, g = group_of(P, r);
-      x.y = queries(P, r, x.x);
-      x.z = length(P, r);
+      int absent;
+      x.y = queries(P, r, x.x, absent);
+      x.z = length(P, r, absent);
       x.w = g >= 0 && x.z > 0 ? L.shared[g] : 0;
       if (x.y > 0 && x.z > capacity(P)) flag_error(P.a.error_flags, HYENA_FLAG_BLOCK_RANGE);
+      if (bad_queries(P, r)) flag_error(P.a.error_flags, HYENA_FLAG_SEGMENT);
     }
     L.info[s] = x;
     const int units = row_tiles(P, x.y) * P.a.kv.kv_heads, tiles = tiles_of(s, x);
@@ -646,7 +648,9 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ P
   } else if (r >= A.num_requests) {
     return;
   }
-  const int g = group_of(P, r), len = length(P, r);
+  int begin, absent;
+  queries(P, r, begin, absent);
+  const int g = group_of(P, r), len = length(P, r, absent);
   // (through L1: read from L2 by every warp, these words cost 4 us of 85)
   const int sh = g >= 0 && len > 0 ? P.shared[g] : 0;
   const int ns = sh > 0 ? ceil_div(sh / KT, P.head[SHARED_TILES]) : 0;

@@ -46,22 +46,28 @@ enum Head {
 __device__ __forceinline__ int query_begin(const Params& P, int r) {
   return P.a.query_start_loc != nullptr ? __ldg(P.a.query_start_loc + r) : r;
 }
-// Queries of request r and their first row.  Rows beyond T do not exist.
-__device__ __forceinline__ int queries(const Params& P, int r, int& begin) {
+// Queries of request r that exist, and their first row; `absent`: further ones that
+// it claims beyond the T rows.
+__device__ __forceinline__ int queries(const Params& P, int r, int& begin, int& absent) {
   begin = query_begin(P, r);
-  int end = query_begin(P, r + 1);
-  end = end < P.a.T ? end : P.a.T;
+  const int claimed = query_begin(P, r + 1), end = claimed < P.a.T ? claimed : P.a.T;
+  absent = claimed - end;
   return begin >= 0 && end > begin ? end - begin : 0;
+}
+// Whether query_start_loc gives request r no run of rows inside [0, T].
+__device__ __forceinline__ bool bad_queries(const Params& P, int r) {
+  if (P.a.query_start_loc == nullptr) return false;
+  const int begin = query_begin(P, r), end = query_begin(P, r + 1);
+  return begin < 0 || end < begin || end > P.a.T;
 }
 // Positions that a page table has.
 __device__ __forceinline__ int capacity(const Params& P) {
   return P.a.kv.pages_per_request * P.a.kv.page_size;
 }
-// Keys of request r as its queries count them, which may be more than its table has
-// (those are not read): the queries' positions go by this length.
-__device__ __forceinline__ int length(const Params& P, int r) {
-  const int n = __ldg(P.a.seq_lens + r);
-  return n < 0 ? 0 : n;
+// Keys of request r up to that of its last existing query, which may be more than its
+// table has (those are not read): the queries' positions go by this length.
+__device__ __forceinline__ int length(const Params& P, int r, int absent) {
+  return max(max(__ldg(P.a.seq_lens + r), 0) - absent, 0);
 }
 // Group of request r, or -1.
 __device__ __forceinline__ int group_of(const Params& P, int r) {
@@ -97,8 +103,8 @@ __device__ __forceinline__ void shared_runs(const Params& P, int* shared, int* l
   }
   __syncthreads();
   for (int r = tid; r < B; r += NTHREADS) {
-    int begin;
-    const int n = queries(P, r, begin), len = length(P, r), g = group_of(P, r);
+    int begin, absent;
+    const int n = queries(P, r, begin, absent), len = length(P, r, absent), g = group_of(P, r);
     if (n > 0 && len > 0 && g >= 0) {
       atomicMin(&shared[g], max(len - n + 1, 0));
       atomicMin(&leader[g], r);

@@ -677,8 +677,10 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, query_start_loc=N
     for kv_append.  seq_lens (B,): keys of request r, the step's own tokens
     (appended before) included; its n queries sit at the last n positions and see
     the keys up to their own.  Keys beyond the page table, and pages outside the
-    cache, are left out and set HYENA_FLAG_BLOCK_RANGE in error_flags.  A request
-    with seq_lens 0 (padding) gets zeros; rows that no request owns are left alone (uninitialised in a new `out`).
+    cache, are left out and set HYENA_FLAG_BLOCK_RANGE in error_flags; a range of
+    query_start_loc beyond T sets HYENA_FLAG_SEGMENT (its rows that exist keep
+    their positions).  A request with seq_lens 0 (padding) gets zeros; rows that no
+    request owns are left alone (uninitialised in a new `out`).
     shared_lens (G,): requests group_start[g] .. group_start[g + 1] - 1 (default:
     one group of all) name the same rows for their first shared_lens[g] keys; a
     run longer than what all of the group's queries see is cut, so the result

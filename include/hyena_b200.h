@@ -400,7 +400,8 @@ HYENA_API int hyena_kv_append(const hyena_kv_append_args* a, void* stream);
  * it exceeds the page table, the keys that the table has).
  * A query that sees no key (seq_lens[r] = 0: a padded request) gives zeros;
  * output rows that no request owns are left alone; keys that a query does not see
- * do not touch its result, whatever they hold.
+ * do not touch its result, whatever they hold.  A range of query_start_loc that runs
+ * past T or backwards sets HYENA_FLAG_SEGMENT; the rows that exist keep their positions.
  * Sharing: the requests [group_start[g], group_start[g+1]) (NULL: all, one group)
  * name the same key and value rows for their first shared_lens[g] positions,
  * which are then read once for the group.  What a query sees is not changed by

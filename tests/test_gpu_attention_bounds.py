@@ -1,5 +1,6 @@
-"""GPU tests of ops.paged_attention for lengths beyond the page table: queries stay
-at their positions, keys that do not exist are left out, and the error flag tells."""
+"""GPU tests of ops.paged_attention for lengths beyond the page table and token
+ranges beyond the rows of q: queries stay at their positions, what does not exist
+is left out, and the error flags tell (1: pages, 2: token ranges)."""
 
 import pytest
 import torch
@@ -68,3 +69,28 @@ def test_lengths_beyond_the_table_in_a_group(members):
 def test_a_length_at_the_end_of_the_table_is_no_error():
     b = Batch([(4, 64), (1, 64)], 2, 2, page=16)
     b.check(b.call())
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_token_ranges_beyond_the_rows(wide, grouped):
+    """Request 4 claims six tokens where q has four more rows: those four sit at the
+    first four of its six positions."""
+    groups = [([3, 4], 32)] if grouped else []
+    b = Batch([(1, 5), (2, 40), (1, 17), (1, 90), (6, 200), (0, 0)], 4, 2, page=16, groups=groups)
+    if wide:
+        widen(b, 2 ** 18)
+    starts = b.starts.clone()
+    b.q = b.q[:9].contiguous()
+    kw = dict(shared_lens=torch.tensor([32], device=DEV), group_start=torch.tensor([3, 5], device=DEV)) if grouped else {}
+    out = b.call(query_start_loc=starts, **kw)
+    assert int(b.flags) == 2
+    check_rows(b, out, 4, slice(5, 9), 195)
+    check_rows(b, out, 1, slice(1, 3), 39)
+    check_rows(b, out, 3, slice(4, 5), 90)
+
+
+def test_decreasing_token_ranges_are_flagged():
+    b = Batch([(1, 5), (2, 40), (1, 17)], 4, 2, page=16)
+    b.call(query_start_loc=torch.tensor([0, 3, 2, 4], dtype=torch.int32, device=DEV))
+    assert int(b.flags) == 2
