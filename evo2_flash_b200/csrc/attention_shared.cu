@@ -433,8 +433,9 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
           else weights(std::false_type{});
           if (i > 0) {
             // A sum above 2^RESCALE_LOG2 (the row's m is that far behind): the rare
-            // tile where m moves, O and l follow, and the weights are made again.
-            const bool grow = part > exp2_approx(RESCALE_LOG2) || (m == -INFINITY && part > 0.0f);
+            // tile where m moves, O and l follow, and the weights are made again.  So
+            // too where no tile had a score yet: weights against 0 may all vanish.
+            const bool grow = part > exp2_approx(RESCALE_LOG2) || m == -INFINITY;
             if (__any_sync(0xffffffffu, grow)) {
               float keep = 1.0f;
               const float mx = set_m();

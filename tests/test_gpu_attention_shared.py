@@ -109,3 +109,50 @@ def test_bad_pages_of_the_run_are_flagged_and_not_read(shape, first, n):
         return at[(at < lo) | (at >= hi)]
 
     check_some(b, out, keep=keep)
+
+
+def far_below_zero(b):
+    """Scores of -300 (natural) and less in the shared run, so that their weights
+    against a maximum of 0 would vanish; values around 1."""
+    u = torch.ones(b.dim, device=DEV)
+    b.q.mul_(0.5).add_((3.0 * u).to(BF))
+    rewrite(b, lambda k, at: 0.5 * k - 100.0 / b.dim ** 0.5 * u)
+    for r, (k, v) in enumerate(b.keys):
+        v = (v + 1).to(BF)
+        b.keys[r] = (k, v)
+        for j in range(-(-len(v) // b.page)):
+            rows = v[j * b.page:(j + 1) * b.page]
+            b.v[int(b.table[r, j]), :len(rows)] = rows
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("keys", [128, 400])
+def test_low_scores_behind_bad_pages(shape, keys):
+    """A run whose first key tile has no key at all: the others count all the same."""
+    b = samples_of_one_prompt(*shape, seed=5)
+    far_below_zero(b)
+    n = -(-keys // b.page)
+    b.table[:, :n] = -1
+    out = b.call(**sharing((shape[4], shape[5])))
+    assert int(b.flags) == 1
+    check_some(b, out, keep=lambda length: torch.arange(n * b.page, length, device=DEV))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("keys", [100, 128, 400])
+def test_low_scores_behind_scores_of_minus_infinity(shape, keys):
+    """The first keys score -inf (weight 0), for some rows a whole tile of them; the
+    next ones -300.  (The reference leaves the keys of no weight out.)"""
+    b = samples_of_one_prompt(*shape, seed=6)
+    far_below_zero(b)
+
+    def minus_inf(k, at):
+        k = k.clone()
+        k[:keys, :, 0] = float("-inf")
+        return k
+
+    rewrite(b, minus_inf)
+    b.q[:, :, 0] = b.q[:, :, 0].abs() + 0.1
+    out = b.call(**sharing((shape[4], shape[5])))
+    assert int(b.flags) == 0
+    check_some(b, out, keep=lambda length: torch.arange(keys, length, device=DEV))
