@@ -390,8 +390,7 @@ shared_kernel(const __grid_constant__ Params P, const __grid_constant__ CUtensor
             tmem_ld32_async(scol, x[0]);
 #pragma unroll
             for (int c = 0; c < TILE_KEYS / 32; ++c) {
-              tmem_wait_ld();
-              tmem_settle(x[c & 1]);
+              tmem_wait_ld(x[c & 1]);
               if (c + 1 < TILE_KEYS / 32) tmem_ld32_async(scol + (c + 1) * 32, x[(c + 1) & 1]);
               if constexpr (decltype(masked)::value) {
 #pragma unroll

@@ -313,7 +313,7 @@ gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmT, const CUtensorMap& tmB
             tmem_ld16_async(col, r);
             tmem_ld16_async(col + HN, r2);
           }
-          tmem_wait_ld();
+          tmem_wait_ld(r, r2);
 #pragma unroll
           for (int j = 0; j < CW; ++j)
             r[j] = __float_as_uint(gate(__uint_as_float(r[j]), __uint_as_float(r2[j]), act));
@@ -614,9 +614,12 @@ gemm_cluster_body(const CUtensorMap& tmA, const CUtensorMap& tmT, const CUtensor
         uint32_t r[2][32];
         if (have) {
           tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(cb * 32), r[0]);
-          if ((cb + 1) * 32 < BN)
+          if ((cb + 1) * 32 < BN) {
             tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(cb * 32 + 32), r[1]);
-          tmem_wait_ld();
+            tmem_wait_ld(r[0], r[1]);
+          } else {
+            tmem_wait_ld(r[0]);
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[0][j] = r[1][j] = 0u;
@@ -980,7 +983,7 @@ gemm_pair_body(const CUtensorMap& tmA, const CUtensorMap& tmT, const CUtensorMap
           uint32_t r2[32];
           tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN2 + cb * 32), r);
           tmem_ld32_async(tmem + (uint32_t(32 * q) << 16) + uint32_t(b * BN2 + HN + cb * 32), r2);
-          tmem_wait_ld();
+          tmem_wait_ld(r, r2);
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             r[j] = __float_as_uint(gate(__uint_as_float(r[j]), __uint_as_float(r2[j]), act));

@@ -68,22 +68,8 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
           su32(bar))
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// The same load without the wait, so that several can be in flight.
+// 32 consecutive 32-bit columns of this thread's TMEM lane, without the wait (see
+// tmem_wait_ld), so that several loads can be in flight.
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
@@ -98,7 +84,7 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32
       : "r"(taddr));
 }
 // 16 columns, without the wait.
-__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
       "%11, %12, %13, %14, %15}, [%16];"
@@ -107,8 +93,23 @@ __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
         "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_wait_ld() {
+// Waits for this thread's loads, into the given arrays: nothing that uses them moves
+// above the wait.  (Volatile statements keep their order, but the arithmetic on what a
+// load returned depends on the load alone, not on a wait that does not name it.)
+template <int N>
+__device__ __forceinline__ void tmem_settle(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+r"(r[j]));
+}
+template <int... N>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&... r)[N]) {
+  static_assert(sizeof...(r) > 0, "the wait names what was loaded");
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  (tmem_settle(r), ...);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  tmem_ld32_async(taddr, r);
+  tmem_wait_ld(r);
 }
 
 __device__ __forceinline__ void fence_proxy_async_smem() {
@@ -127,11 +128,6 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// After the wait: nothing that uses the loaded registers moves above it.
-__device__ __forceinline__ void tmem_settle(uint32_t (&r)[32]) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) asm volatile("" : "+r"(r[j]));
-}
 // 32 consecutive 32-bit columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(

@@ -1,0 +1,23 @@
+"""Rules of the kernel sources that no run of today's build can show broken: what
+holds only by the compiler's choice of order or placement."""
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parent.parent / "evo2_flash_b200" / "csrc"
+SOURCES = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh"))
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=lambda p: p.name)
+def test_tensor_memory_waits_name_what_was_loaded(path):
+    """A wait for tensor-memory loads orders the arithmetic on the loaded registers
+    only if it names them: tmem_wait_ld does, the instruction by itself does not."""
+    text = path.read_text()
+    assert "tmem_wait_ld()" not in text
+    if path.name != "tcgen05.cuh":
+        assert "tcgen05.wait::ld" not in text
+    else:
+        assert re.findall(r"tcgen05\.wait::ld[^}]*", text) == [
+            'tcgen05.wait::ld.sync.aligned;" ::: "memory");\n  (tmem_settle(r), ...);\n']
