@@ -175,7 +175,7 @@ __device__ void make_plan(const Params& P, Plan& L) {
 // SM that is far from its memory, or busy with the shared kernel, takes fewer).
 constexpr int PLAN_THREADS = 256;
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const __grid_constant__ Params P) {
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(16) uint8_t smem_raw[];
   const int tid = (int)threadIdx.x, G = P.groups, n = G + P.a.num_requests;
   pdl_entry();
   Plan L = plan_at(smem_raw, G, n);
