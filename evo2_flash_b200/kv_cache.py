@@ -46,20 +46,21 @@ class PagedKVCache:
 
     def clear(self):
         """Drops every sequence and the pools."""
-        self._pools = [(None, None)] * self.layers
+        self._pools = [[None, None] for _ in range(self.layers)]
         self._free, self._holders, self._pages = [], [], {}
         self._version, self._tables = 0, {}
 
     # ---- pages ----------------------------------------------------------------
     def _grow(self, pages):
-        def bigger(old):
-            t = torch.empty(pages, self.heads, self.page_size, self.head_dim, dtype=self.dtype,
-                            device=self.device)
-            if old is not None:
-                t[:old.shape[0]] = old
-            return t
-
-        self._pools = [(bigger(k), bigger(v)) for k, v in self._pools]
+        # One tensor after the other, each old one dropped before the next is made: the
+        # old pools, what they grow by and one tensor are all that is held at a time.
+        for pool in self._pools:
+            for i in range(2):
+                t = torch.empty(pages, self.heads, self.page_size, self.head_dim, dtype=self.dtype,
+                                device=self.device)
+                if pool[i] is not None:
+                    t[:pool[i].shape[0]] = pool[i]
+                pool[i] = t
         self._free += range(pages - 1, len(self._holders) - 1, -1)
         self._holders += [0] * (pages - len(self._holders))
 
@@ -77,7 +78,7 @@ class PagedKVCache:
 
     def layer(self, index):
         """(keys, values) of a layer: (pages, page size, heads, head dim)."""
-        k, v = self._pools[index]
+        k, v = (t[:len(self._holders)] for t in self._pools[index])  # (more after a failed growth)
         return k.transpose(1, 2), v.transpose(1, 2)
 
     # ---- sequences ------------------------------------------------------------

@@ -119,3 +119,47 @@ def test_native_blocks_need_cuda_and_a_head_size():
     with pytest.raises(ValueError, match="CUDA"):
         StripedHyena2(StripedHyena2Config.small(hidden=128, native_blocks=True), device="cpu",
                       mixer_factory=OracleMixer)
+
+
+def test_growth_holds_one_old_tensor_too_many_at_most(monkeypatch):
+    """A pool's old tensor is dropped before the next pool's new one is made."""
+    import weakref
+
+    c = cache(layers=3)
+    c.extend(0, 0, 16)
+    old = [weakref.ref(t) for pool in c._pools for t in pool]
+    held, empty = [], torch.empty
+
+    def spy(*args, **kw):
+        held.append(sum(r() is not None for r in old))
+        return empty(*args, **kw)
+
+    monkeypatch.setattr(torch, "empty", spy)
+    c.extend(1, 0, 16 * 40)
+    assert held[:6] == [6, 5, 4, 3, 2, 1]
+    assert all(r() is None for r in old)
+
+
+def test_growth_that_fails_leaves_the_cache_as_it_was(monkeypatch):
+    c = cache(layers=2)
+    c.extend(0, 0, 30)
+    write(c, c.table([0])[0], 0, range(30), 5.0)
+    before, made, empty = read(c, c.table([0])[0], 0, 30), [], torch.empty
+
+    def fails(*args, **kw):
+        made.append(1)
+        if len(made) == 2:
+            raise torch.OutOfMemoryError("no room")
+        return empty(*args, **kw)
+
+    monkeypatch.setattr(torch, "empty", fails)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.extend(1, 0, 16 * 100)
+    monkeypatch.setattr(torch, "empty", empty)
+    k, v = c.layer(0)
+    assert k.shape == v.shape
+    assert torch.equal(read(c, c.table([0])[0], 0, 30), before)
+    c.release(1)
+    c.extend(2, 0, 16 * 100)
+    assert torch.equal(read(c, c.table([0])[0], 0, 30, layer=1), before + 1000)
+    assert c.layer(0)[0].shape == c.layer(1)[1].shape
