@@ -15,6 +15,13 @@ from __future__ import annotations
 import torch
 
 
+def _ints(values, device):
+    """int32 on the device; the copy is in stream order, from pinned memory that torch
+    keeps until it is done."""
+    t = torch.tensor(values, dtype=torch.int32, pin_memory=device.type == "cuda")
+    return t.to(device, non_blocking=True)
+
+
 class PagedStep(list):
     """The segments of one model step, with what the attention layers of the step
     share: positions, page table, offsets and lengths (int32, on the device) and
@@ -24,13 +31,12 @@ class PagedStep(list):
         super().__init__(segments)
         self.cache = cache
         dev = cache.device
-        ints = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
         self.positions = positions.to(torch.int32)
         self.longest = max((b - a for a, b, _, _ in segments), default=0)
         self.table, self.shared = cache.table([sid for _, _, sid, _ in segments])
-        self.seq_lens = ints([p0 + b - a for a, b, _, p0 in segments])
+        self.seq_lens = _ints([p0 + b - a for a, b, _, p0 in segments], dev)
         single = all(a == i and b == i + 1 for i, (a, b, _, _) in enumerate(segments))
-        self.starts = None if single else ints([segments[0][0]] + [b for _, b, _, _ in segments])
+        self.starts = None if single else _ints([segments[0][0]] + [b for _, b, _, _ in segments], dev)
 
 
 class PagedKVCache:
@@ -135,7 +141,7 @@ class PagedKVCache:
             return hit[1]
         rows = [self._pages[s] for s in sids]
         width = max((len(r) for r in rows), default=0)
-        table = torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32).to(self.device)
+        table = _ints([r + [0] * (width - len(r)) for r in rows], self.device)
         made = table, self._shared(rows)
         self._tables = {key: (self._version, made)}
         return made
@@ -159,5 +165,4 @@ class PagedKVCache:
                 for n, b, e in zip(runs, starts, starts[1:] + [len(rows)])]
         if not any(lens):
             return {}
-        ints = lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)  # noqa: E731
-        return dict(shared_lens=ints(lens), group_start=ints(starts + [len(rows)]))
+        return dict(shared_lens=_ints(lens, self.device), group_start=_ints(starts + [len(rows)], self.device))

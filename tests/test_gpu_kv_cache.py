@@ -1,0 +1,36 @@
+"""GPU tests of the paged cache beside its operators: its bookkeeping does not wait for
+the GPU, and scoring leaves no pools behind."""
+
+import pytest
+import torch
+
+from evo2_flash_b200.kv_cache import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+
+def test_bookkeeping_does_not_wait_for_the_gpu():
+    """Under torch's check for synchronising calls: a prompt, forks, and decode steps
+    that copy a shared page, take new ones and grow the pools."""
+    c = PagedKVCache(2, heads=2, head_dim=64, page_size=16)
+    prompt, steps = 40, 600
+    positions = [torch.arange(prompt, device="cuda")]
+    positions += [torch.full((3,), prompt + i, device="cuda") for i in range(steps)]
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        made = [c.step([(0, prompt, 0, 0)], positions[0])]
+        c.fork(0, 1, prompt)
+        c.fork(0, 2, prompt)
+        made += [c.step([(r, r + 1, r, prompt + i) for r in range(3)], positions[1 + i]) for i in range(steps)]
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    # what the copies brought, each from pinned memory of its own until it is done
+    assert made[0].seq_lens.tolist() == [prompt] and made[0].starts.tolist() == [0, prompt]
+    for i, step in enumerate(made[1:]):
+        assert step.seq_lens.tolist() == [prompt + i + 1] * 3 and step.starts is None
+    last = made[-1]
+    assert last.table.tolist() == [c._pages[r] for r in range(3)]
+    assert last.shared["shared_lens"].tolist() == [32] and last.shared["group_start"].tolist() == [0, 3]
+    assert c.layer(1)[1].shape == (128, 16, 2, 64)
