@@ -1099,28 +1099,25 @@ static int launch_bn(const CUtensorMap& ta, const CUtensorMap& tt, const void* B
   return check_launch(FP8 ? "gemm_kernel<e4m3>" : "gemm_kernel<bf16>");
 }
 
-template <bool FP8, int BN>
+template <int BN>
 static size_t cluster_smem() {
   return sizeof(SmemSK<BN>) + 1024;
 }
 
-template <bool FP8, int BN>
-static bool cluster_attr() {
-  return smem_attr<gemm_cluster_kernel<FP8, BN>>((int)cluster_smem<FP8, BN>());
-}
-
-// How many clusters of `splits` CTAs can be resident at once (0 if unknown).
-template <bool FP8, int BN>
-static int resident_clusters(int splits) {
+// How many clusters of `splits` CTAs of a cluster kernel can be resident at once (0 if
+// unknown): a cluster lies inside a GPC, so fewer than the SMs have room for (of 148
+// SMs: 74 clusters of two, 45 of three, 33 of four).
+template <auto Kern>
+static int resident_clusters(size_t smem, int splits) {
   static int cache[9] = {-1, -1, -1, -1, -1, -1, -1, -1, -1};
   if (splits < 1 || splits > 8) return 0;
   if (cache[splits] < 0) {
     int n = 0;
-    if (cluster_attr<FP8, BN>()) {
+    if (smem_attr<Kern>((int)smem)) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)splits, 1, 1);
       cfg.blockDim = dim3(THREADS, 1, 1);
-      cfg.dynamicSmemBytes = cluster_smem<FP8, BN>();
+      cfg.dynamicSmemBytes = smem;
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim.x = (unsigned)splits;
@@ -1128,7 +1125,7 @@ static int resident_clusters(int splits) {
       at[0].val.clusterDim.z = 1;
       cfg.attrs = at;
       cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&n, gemm_cluster_kernel<FP8, BN>, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, Kern, &cfg) != cudaSuccess) {
         cudaGetLastError();
         n = 0;
       }
@@ -1145,10 +1142,11 @@ static int launch_cluster(const CUtensorMap& ta, const CUtensorMap& tt, const vo
   CUtensorMap tb;
   int rc = make_map(&tb, B, FP8, (uint64_t)K, (uint64_t)N, (uint64_t)ldb, BN);
   if (rc) return rc;
-  if (!cluster_attr<FP8, BN>()) return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_cluster) failed");
+  if (!smem_attr<gemm_cluster_kernel<FP8, BN>>((int)cluster_smem<BN>()))
+    return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_cluster) failed");
   const int tiles = ((N + BN - 1) / BN) * ((M + BM - 1) / BM);
   launch_kernel(gemm_cluster_kernel<FP8, BN>, dim3((unsigned)splits, (unsigned)tiles, 1),
-                dim3(THREADS), cluster_smem<FP8, BN>(), st, (unsigned)splits, ta, tt, tb,
+                dim3(THREADS), cluster_smem<BN>(), st, (unsigned)splits, ta, tt, tb,
                 static_cast<bf16*>(out), ldo, M, N, K, sa, sb, static_cast<const bf16*>(bias),
                 tail_box_rows(M));
   return check_launch(FP8 ? "gemm_cluster_kernel<e4m3>" : "gemm_cluster_kernel<bf16>");
@@ -1228,10 +1226,10 @@ constexpr int PAIR_MIN_M = 4096;
 template <bool FP8>
 static int resident(int bn, int splits) {
   switch (bn) {
-    case 256: return resident_clusters<FP8, 256>(splits);
-    case 192: return resident_clusters<FP8, 192>(splits);
-    case 128: return resident_clusters<FP8, 128>(splits);
-    default: return resident_clusters<FP8, 64>(splits);
+    case 256: return resident_clusters<gemm_cluster_kernel<FP8, 256>>(cluster_smem<256>(), splits);
+    case 192: return resident_clusters<gemm_cluster_kernel<FP8, 192>>(cluster_smem<192>(), splits);
+    case 128: return resident_clusters<gemm_cluster_kernel<FP8, 128>>(cluster_smem<128>(), splits);
+    default: return resident_clusters<gemm_cluster_kernel<FP8, 64>>(cluster_smem<64>(), splits);
   }
 }
 
@@ -1367,7 +1365,7 @@ template <int BN>
 static int launch_gated_cluster(const CUtensorMap& ta, const CUtensorMap& tt, const CUtensorMap& t1,
                                 const CUtensorMap& t2, bf16* out, int64_t ldo, int M, int N, int K, int act, int splits,
                                 cudaStream_t st) {
-  const size_t smem = sizeof(SmemSK<BN>) + 1024;
+  const size_t smem = cluster_smem<BN>();
   if (!smem_attr<gemm_gated_cluster_kernel<BN>>((int)smem))
     return fail(HYENA_ERR_CUDA, "cudaFuncSetAttribute(gemm_gated_cluster) failed");
   const int tiles = ((N + BN / 2 - 1) / (BN / 2)) * ((M + BM - 1) / BM);
@@ -1415,6 +1413,16 @@ static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& tt, const
   return check_launch("gemm_gated_pair_kernel");
 }
 
+static int resident_gated(int bn, int splits) {
+  switch (bn) {
+    case 256: return resident_clusters<gemm_gated_cluster_kernel<256>>(cluster_smem<256>(), splits);
+    case 192: return resident_clusters<gemm_gated_cluster_kernel<192>>(cluster_smem<192>(), splits);
+    case 160: return resident_clusters<gemm_gated_cluster_kernel<160>>(cluster_smem<160>(), splits);
+    case 128: return resident_clusters<gemm_gated_cluster_kernel<128>>(cluster_smem<128>(), splits);
+    default: return resident_clusters<gemm_gated_cluster_kernel<64>>(cluster_smem<64>(), splits);
+  }
+}
+
 // Several row tiles: the cheapest by `steps` of the persistent kernel's widths and SM
 // pairs (those where they are 7% ahead).
 // One row tile (decode batches): the weights' bytes bound it, so the shortest time of
@@ -1422,8 +1430,10 @@ static int launch_gated_pair(const CUtensorMap& ta, const CUtensorMap& tt, const
 // Hence 160 columns, which the plain GEMMs do not have: the 7B shape (11008 outputs)
 // makes 138 tiles of 148 SMs, 33.4 us for 101 rows (192 columns, 115 tiles: 37.7; 256:
 // 40.8; 128, two waves: 50.3), the 40B shape (22528) 282 of 296.  K is cut (the cluster
-// kernel) where the tiles alone leave SMs idle: 4096 outputs of 4096 take 14-17 us on
-// 43 tiles of 192 in 3 slices, 21 us on 128 of 64.
+// kernel) where the tiles alone leave SMs idle, in as many slices as still run at once:
+// 4096 outputs of 4096 take 14-17 us on 43 tiles of 192 in 3 slices, 21 us on 128 of 64;
+// 6144 outputs 19.5 us on 64 tiles of 192 in 2 slices, 32.7 us on 48 of 256 in 3, three
+// clusters of which have to wait for the others to end.
 static Plan plan_gated(int M, int N, int K) {
   const long long mt = (M + BM - 1) / BM;
   const int sms = num_sms(), kblocks = K / (BKB / 2);
@@ -1444,7 +1454,7 @@ static Plan plan_gated(int M, int N, int K) {
   for (int bn : {256, 192, 160, 128, 64}) {
     take(bn, 0, (tiles(bn) + sms - 1) / sms * tile_step(bn) * kblocks);
     for (int sp = 2; sp <= (bn >= 256 ? 3 : 4) && tiles(bn) * sp <= sms && kblocks / sp >= 2; ++sp)
-      take(bn, sp, tile_step(bn) * ((kblocks + sp - 1) / sp));
+      if (tiles(bn) <= resident_gated(bn, sp)) take(bn, sp, tile_step(bn) * ((kblocks + sp - 1) / sp));
   }
   return best;
 }
