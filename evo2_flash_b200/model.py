@@ -447,6 +447,8 @@ class StripedHyena2(nn.Module):
                     self.release(sid)
             while nxt < len(seqs) and done[nxt] == lens[nxt]:
                 nxt += 1
+        if not keep_cache:
+            self.release_all()  # every sequence is released: the paged cache's pools too
 
     @torch.no_grad()
     def token_logprobs(self, seqs, max_tokens_per_step=None):
@@ -525,6 +527,7 @@ class StripedHyena2(nn.Module):
                     self.release(sid)
             while nxt < len(seqs) and done[nxt] == lens[nxt]:
                 nxt += 1
+        self.release_all()
         return [-s / c if c else math.nan for s, c in zip(sums, cnt)]
 
     @torch.no_grad()

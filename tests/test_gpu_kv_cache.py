@@ -34,3 +34,32 @@ def test_bookkeeping_does_not_wait_for_the_gpu():
     assert last.table.tolist() == [c._pages[r] for r in range(3)]
     assert last.shared["shared_lens"].tolist() == [32] and last.shared["group_start"].tolist() == [0, 3]
     assert c.layer(1)[1].shape == (128, 16, 2, 64)
+
+
+@pytest.fixture(scope="module")
+def native():
+    from evo2_flash_b200.model import StripedHyena2, StripedHyena2Config
+
+    m = StripedHyena2(StripedHyena2Config.small(hidden=256, use_fp8_input_projections=False, native_blocks=True),
+                      device="cuda")
+    m.load_tensors(m.random_tensors(23))
+    return m
+
+
+def _seqs(*lens):
+    g = torch.Generator().manual_seed(1)
+    return [torch.randint(65, 70, (n,), generator=g) for n in lens]
+
+
+@pytest.mark.parametrize("budget", [None, 50])
+def test_scoring_leaves_no_pools(native, budget):
+    seqs = _seqs(120, 30, 70)
+    for run in (native.score, native.token_logprobs,
+                lambda s, b: list(native.prefill_steps(s, b)),
+                lambda s, b: list(native.prefill_steps(s, b, {1}))):
+        run(seqs, budget)
+        assert native.cache._pages == {}
+        assert all(t is None for pool in native.cache._pools for t in pool)
+    list(native.prefill_steps(seqs, budget, keep_cache=True))
+    assert sorted(native.cache._pages) == [0, 1, 2]  # kept for decode steps
+    native.release_all()
