@@ -201,11 +201,11 @@ class Evo2Attention(nn.Module):
         k_cache, v_cache = step.cache.layer(self.index)
         q = ops.kv_append(q, k, v, step.positions, k_cache, v_cache, step.table, step.starts,
                           rope_theta=self.theta)
-        groups = step.shared["shared_lens"].shape[0] if step.shared else 0
-        if (step.longest <= PAGED_ATTENTION_TOKENS
-                and len(step) + groups <= ops.PAGED_ATTENTION_REQUESTS):
-            return ops.paged_attention(q, k_cache, v_cache, step.table, step.seq_lens, step.starts,
-                                       **step.shared)
+        if step.longest <= PAGED_ATTENTION_TOKENS and len(step) <= ops.PAGED_ATTENTION_REQUESTS:
+            shared = step.shared
+            if shared and len(step) + shared["shared_lens"].shape[0] > ops.PAGED_ATTENTION_REQUESTS:
+                shared = {}  # every sequence reads its keys for itself
+            return ops.paged_attention(q, k_cache, v_cache, step.table, step.seq_lens, step.starts, **shared)
         out = torch.empty_like(q)
         for i, (a, b, _, p0) in enumerate(step):
             n = p0 + b - a

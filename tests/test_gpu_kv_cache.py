@@ -63,3 +63,36 @@ def test_scoring_leaves_no_pools(native, budget):
     list(native.prefill_steps(seqs, budget, keep_cache=True))
     assert sorted(native.cache._pages) == [0, 1, 2]  # kept for decode steps
     native.release_all()
+
+
+@pytest.mark.parametrize("limit,sharing,called", [(2048, True, True), (9, True, True), (8, False, True),
+                                                  (5, False, True), (4, False, False)])
+def test_sequences_and_groups_beyond_one_call(native, monkeypatch, limit, sharing, called):
+    """Five sequences, two of which share a prompt: with the three others' groups nine in
+    all.  Where the groups are too many, the sequences read for themselves."""
+    from evo2_flash_b200 import ops
+    from tests.helpers import REL_TOL, max_rel_err
+
+    seqs, seen, paged = _seqs(100, 20, 30, 40), [], ops.paged_attention
+
+    def spy(*args, **kw):
+        seen.append("shared_lens" in kw)
+        return paged(*args, **kw)
+
+    def step(n):
+        monkeypatch.setattr(ops, "PAGED_ATTENTION_REQUESTS", n)
+        with torch.no_grad():
+            list(native.prefill_steps(seqs, keep_cache=True, state_blocks=6))
+            native.fork(0, 4, 100)
+            monkeypatch.setattr(ops, "paged_attention", spy)
+            try:
+                seen.clear()
+                return native.decode_step([65] * 5, [100, 100, 20, 30, 40], [0, 4, 1, 2, 3])
+            finally:
+                monkeypatch.setattr(ops, "paged_attention", paged)
+                native.release_all()
+
+    want, got = step(2048), step(limit)
+    layers = len(native.cfg.attn_layer_idxs)
+    assert len(seen) == (layers if called else 0) and all(x == sharing for x in seen)
+    assert max_rel_err(got.float().cpu(), want.float().cpu()) < 2 * REL_TOL
