@@ -53,7 +53,7 @@ class PagedKVCache:
     def clear(self):
         """Drops every sequence and the pools."""
         self._pools = [[None, None] for _ in range(self.layers)]
-        self._free, self._holders, self._pages = [], [], {}
+        self._free, self._holders, self._pages, self._lengths = [], [], {}, {}
         self._version, self._tables = 0, {}
 
     # ---- pages ----------------------------------------------------------------
@@ -93,10 +93,10 @@ class PagedKVCache:
         may write; start 0 begins the sequence anew."""
         if start == 0:
             self.release(sid)
+        length = self._lengths.get(sid, 0)
+        if start > length:
+            raise ValueError(f"sequence {sid} has {length} positions, cannot continue at {start}")
         pages = self._pages.setdefault(sid, [])
-        if start > len(pages) * self.page_size:
-            raise ValueError(f"sequence {sid} has {len(pages) * self.page_size} positions at most, "
-                             f"cannot continue at {start}")
         for i in range(start // self.page_size, min(-(-end // self.page_size), len(pages))):
             if self._holders[pages[i]] > 1:  # copy on write
                 new = self._take()
@@ -108,19 +108,21 @@ class PagedKVCache:
         while len(pages) * self.page_size < end:
             pages.append(self._take())
             self._version += 1
+        self._lengths[sid] = max(length, end)
 
     def fork(self, src, dst, length):
         """Sequence `dst` becomes the first `length` positions of `src`, on its pages."""
-        held = self._pages[src][:-(-length // self.page_size)]
-        if len(held) * self.page_size < length:
+        if not 0 <= length <= self._lengths[src]:
             raise ValueError(f"sequence {src} has fewer than {length} positions")
+        held = self._pages[src][:-(-length // self.page_size)]
         for page in held:
             self._holders[page] += 1
         self.release(dst)
-        self._pages[dst] = held
+        self._pages[dst], self._lengths[dst] = held, length
         self._version += 1
 
     def release(self, sid):
+        self._lengths.pop(sid, None)
         for page in self._pages.pop(sid, ()):
             self._drop(page)
         self._version += 1

@@ -163,3 +163,31 @@ def test_growth_that_fails_leaves_the_cache_as_it_was(monkeypatch):
     c.extend(2, 0, 16 * 100)
     assert torch.equal(read(c, c.table([0])[0], 0, 30, layer=1), before + 1000)
     assert c.layer(0)[0].shape == c.layer(1)[1].shape
+
+
+def test_positions_that_were_never_written_are_not_skipped():
+    """Inside a sequence's last page too: what lies between would be read by attention."""
+    c = cache(page=64)
+    c.extend(0, 0, 10)
+    with pytest.raises(ValueError, match="has 10 positions, cannot continue at 11"):
+        c.extend(0, 11, 12)
+    with pytest.raises(ValueError, match="has 0 positions, cannot continue at 5"):
+        c.extend(1, 5, 6)
+    assert 1 not in c._pages
+    for length in (11, 64, -1):
+        with pytest.raises(ValueError, match="fewer than"):
+            c.fork(0, 1, length)
+    c.fork(0, 1, 10)
+    c.fork(0, 2, 7)
+    c.extend(1, 10, 11)
+    with pytest.raises(ValueError, match="has 7 positions"):
+        c.extend(2, 10, 11)
+    c.extend(0, 10, 14)
+    c.extend(0, 12, 13)  # back, as after rejected tokens; what was written may be continued
+    c.extend(0, 14, 15)
+    c.extend(0, 0, 3)  # anew
+    with pytest.raises(ValueError, match="has 3 positions"):
+        c.extend(0, 4, 5)
+    c.release(0)
+    with pytest.raises(ValueError, match="has 0 positions"):
+        c.extend(0, 3, 4)
