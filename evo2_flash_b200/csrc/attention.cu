@@ -49,9 +49,11 @@ constexpr int MAX_SEGMENTS = 2048;
 constexpr int TC_MIN_ROWS = 16;  // mean rows of a group and key/value head
 // Without a shared kernel, plan_kernel plans from this many requests and bytes of keys
 // and values (as many as their page tables can name) on, else each CTA for itself, its
-// warps taking items in turn.  With the plan kernel and without: one request of 777
-// keys 17.5 and 11.5 us; 32 heads, 16 requests of 1024 keys (0.27 GB) 57 and 55 us, 8
-// of 8192 (1.07 GB) 172 and 176 us, 32 of up to 8000 (2.0 GB) 305 and 331 us.
+// warps taking items in turn.  With the plan kernel and without, 32 heads: one request of
+// 777 keys 16.7 and 10.5 us; 16 requests of 1024 keys (0.27 GB) 57 and 54 us, 8 of 4096
+// (0.54 GB) 94 and 97 us, 8 of 8192 (1.07 GB) 171 and 178, 32 of up to 8000 (2.0 GB of
+// keys, 4.2 GB that the tables can name) 305 and 337.  Tables that are half full lose at
+// the border: 64 requests of up to 500 keys (0.54 GB) 58 and 53 us.
 constexpr int PLANNED_REQUESTS = 5;
 constexpr long long PLANNED_BYTES = 512ll << 20;
 

@@ -41,7 +41,8 @@
 // join kernel, which waits for it alone, finds both complete.
 //   NT = 2 goes first, after a plan kernel, and the stream kernel's items, which
 // are then taken as they come, fill the SMs that its last wave leaves: 353 us for
-// 256 samples of one prompt of 32768 keys, 382 us the other way round (331 us now).
+// 256 samples of one prompt of 32768 keys, 382 us the other way round (332 us now in runs
+// of a few ms, 377 in longer ones, for which the power cap lowers the clock).
 //   NT = 1 goes second, each CTA of either planning for itself: both are bound by
 // the keys' bytes, and this one fills the end of the two better.  85 us for 64
 // samples of a prompt of 8192 keys and 99 us for 3 prompts being verified (91 us

@@ -1238,8 +1238,11 @@ static int resident(int bn, int splits) {
 // tensor pipe's 128 x bn products at 4096 a cycle, or its (128 + bn) 32-byte
 // operand rows at the some 72 bytes a cycle that an SM takes in, whichever is
 // longer (256 columns: 171, the 74% of the tensor rate seen there); a pair 141
-// (91%).  The power cap holds long runs at 1 / 1.36 of the clock, so a last wave
-// that is mostly empty costs less than it would at full clock.
+// (91%).  Under the power cap the clock follows the work (gated GEMMs of 8192 x 22528 run
+// on and on at some 1180 MHz with 777 rows, 1090 with 8192, of 1965), so a last wave that
+// is mostly empty costs less than it would at full clock: hence a floor of 1.36 times the
+// work itself.  The factor is fitted: with 1.0, 1.2, 1.36 and 1.42 the choices between
+// pairs and single SMs on the 52 shapes of plan_gated lose 0.8, 0.9, 0.7 and 1.7 %.
 static long long tile_step(int bn) { return std::max(bn / 2, (BM + bn) * 32 / 72); }
 static long long steps(long long tiles, long long slots, int bn, bool pair) {
   const long long step = pair ? 141 : tile_step(bn);
@@ -1279,7 +1282,10 @@ static Plan plan(int M, int N, int K) {
     if (pick != 0 && cost256 >= 0 && pick != 256 && 10 * pick_cost > 9 * cost256) pick = 256;
     // Between the persistent kernels (same sums in the same order, so the same
     // bits): the SM pairs where their waves are a tenth shorter.  M = 777 x 4096
-    // x 11008: 107 us with 128-column tiles, 65 us with pairs.
+    // x 11008: 109 us with 128-column tiles, 65 us with pairs.  Over 30 shapes (129 to 3000
+    // rows; K 2048 to 22528, N 4096 to 12288) that picks the faster kernel or one within
+    // 2 %, but for the pairs that it passes over at 520, 777 and 1300 rows of K 4096, N
+    // 12288 (6, 8 and 11 %) and 1300 of K 22528, N 8192 (9 %).
     if (!FP8 && pick != 0 && M > BM && N >= BN2 &&
         10 * pair_steps(M, (N + BN2 - 1) / BN2) <= 9 * steps(mt * ((N + pick - 1) / pick), sms, pick, false))
       return {BN2, 0, true};
@@ -1424,7 +1430,10 @@ static int resident_gated(int bn, int splits) {
 }
 
 // Several row tiles: the cheapest by `steps` of the persistent kernel's widths and SM
-// pairs (those where they are 7% ahead).
+// pairs (those where they are 7% ahead).  Over 52 shapes (129 to 4101 rows; 1024 x 4096,
+// 2048 x 5504, 4096 x 11008, 8192 x 22528) that picks the faster of the two or one within
+// 2 %, but for the pairs at 400 and 1024 rows of 1024 x 4096 (11.6 us for 9.6, 17.5 for
+// 16.4): 300 rows of 4096 x 11008 60 us, with pairs 73; 1300 rows 205, with pairs 182.
 // One row tile (decode batches): the weights' bytes bound it, so the shortest time of
 // the busiest SM; no allowance for the clock in the last wave, which HBM does not know.
 // Hence 160 columns, which the plain GEMMs do not have: the 7B shape (11008 outputs)

@@ -173,7 +173,12 @@ def _rope_neox(x, positions, theta):
 
 # Steps of at most this many new tokens a sequence attend over the paged cache;
 # longer ones (prompts), and steps of more sequences than one call takes, through
-# torch's attention on the sequence's gathered pages.
+# torch's attention on the sequence's gathered pages.  A layer of 32 heads of 128, the
+# kernel and torch's, host included: 64 new tokens of one sequence at 500, 8192 and 32768
+# 30 and 74, 97 and 496, 245 and 1845 us; of 32 sequences at 2000 0.56 and 4.9 ms; of one
+# prompt from its start 24 and 30 us.  It is ahead up to 256 tokens (one prompt 38 and
+# 42 us, 8 sequences at 4096 1.0 and 2.1 ms; 512: 64 and 52 us, 2.0 and 2.3 ms), but its
+# pieces take 520 bytes a token and head, 17 KB a token of 32 heads in a packed step.
 PAGED_ATTENTION_TOKENS = 64
 
 
